@@ -160,6 +160,113 @@ int ntl_fa2_fwd_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uin
 #define NTL_FA2_GRID_PER_BLOCK 2
 int ntl_fa2_set_causal_grid(int mode);
 
+/* ---- Paged key/value cache.  No reference counterpart (its kernels have no cache).
+ *
+ * A cache is [layers, pages, page_size, kv_heads, head_dim] values of 16 bits; K and V have the same
+ * strides (in values, multiples of 8), and head_dim is dense.  A sequence is a row of a page table
+ * (int32 page numbers, -1 = no page) and a length in tokens (int32, device memory).  Page numbers
+ * and lengths are read on the device: what is out of range is skipped, a length is cut to
+ * max_pages * page_size, and a position without a page is not visible and takes no row.  All
+ * entry points work in stream order; those with a workspace take one of the size that the matching
+ * size function gives, which calls on different streams must not share. */
+enum { NTL_F16 = 0, NTL_BF16 = 1 };
+
+typedef struct {
+  void* k;
+  void* v;
+  int64_t layers, pages, page_size, kv_heads, head_dim;
+  int64_t layer_stride, page_stride, row_stride, head_stride; /* in values */
+  int64_t dtype;                                              /* NTL_F16 or NTL_BF16 */
+} ntl_cache_t;
+
+/* New tokens of `seqs` sequences: q [seqs, tokens, heads, head_dim] (strided, head_dim dense),
+ * o the same, dense; sequence b's tokens are the last n_b of its lens[b] cached ones, n_b =
+ * q_lens[b] (NULL: tokens), at most lens[b].  Query head h reads key head h / (heads / kv_heads).
+ * Rows t >= n_b of o are set to 0. */
+typedef struct {
+  const void* q;
+  void* o;
+  int64_t seqs, tokens, heads;
+  int64_t seq_stride, token_stride, head_stride; /* of q, in values */
+  const int32_t* table;
+  int64_t table_stride, max_pages;
+  const int32_t* lens;
+  const int32_t* q_lens;
+  double scale; /* of q . k, > 0 */
+} ntl_query_t;
+
+/* Attention of drafted tokens over one layer of a cache: token t sees every key before the n_b
+ * drafts, and draft s where bit s % 32 of word s / 32 of tree[b, t] is set (tree: [seqs, tokens,
+ * ceil(tokens / 32)] words, tree_stride words from one sequence to the next, 0 to share one tree).
+ * o = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s), s_j = scale q . k_j, statistics and sums
+ * in fp32, the exponentials rounded to the cache's type for the product with V; a row that sees
+ * nothing gives 0.  page_size: a multiple of 8; head_dim 64 or 128; heads / kv_heads up to 128. */
+int ntl_tree_attention(const ntl_cache_t* cache, const ntl_query_t* query, const uint32_t* tree, int64_t tree_stride,
+                       void* workspace, uint64_t workspace_bytes, ntl_stream_t stream);
+
+/* The same with a sliding window: the token at position i sees keys j <= i with j > i - window or
+ * j < sinks. */
+int ntl_window_attention(const ntl_cache_t* cache, const ntl_query_t* query, int64_t window, int64_t sinks,
+                         void* workspace, uint64_t workspace_bytes, ntl_stream_t stream);
+
+/* Workspace of either attention call (16-byte aligned; its contents need no preparation). */
+int ntl_cache_attention_workspace(const ntl_cache_t* cache, const ntl_query_t* query, uint64_t* bytes_out);
+
+/* words[b, t] (ceil(tokens / 32) words): bit s set where s is t or an ancestor of t, from
+ * parents [seqs, tokens] (stride in entries); a parent that is not an earlier token ends the walk. */
+int ntl_tree_mask(const int32_t* parents, int64_t stride, int64_t seqs, int64_t tokens, uint32_t* words,
+                  ntl_stream_t stream);
+
+/* Write the rows of new tokens, k_new / v_new [layers, seqs, tokens, kv_heads, head_dim] (strides in
+ * values), at positions lens[b] + t, t < counts[b] (NULL: tokens); lens_out[b] = lens[b] + that
+ * count, cut to the table's width.  lens_out must not be lens. */
+int ntl_cache_append(const ntl_cache_t* cache, const void* k_new, const void* v_new, int64_t layer_stride,
+                     int64_t seq_stride, int64_t token_stride, int64_t head_stride, const int32_t* table,
+                     int64_t table_stride, int64_t seqs, int64_t max_pages, const int32_t* lens, const int32_t* counts,
+                     int64_t tokens, int32_t* lens_out, ntl_stream_t stream);
+
+/* Keep a verified path of the last drafts_of[b] (NULL: drafts) cached tokens: the row of draft
+ * path[b, i] moves to draft place i, i < counts[b]; lens_out[b] = lens[b] - drafts + counts[b].
+ * path is increasing along i.  lens_out must not be lens. */
+int ntl_cache_accept(const ntl_cache_t* cache, const int32_t* table, int64_t table_stride, int64_t seqs,
+                     int64_t max_pages, const int32_t* lens, const int32_t* drafts_of, int64_t drafts,
+                     const int32_t* path, int64_t path_stride, int64_t path_len, const int32_t* counts,
+                     int32_t* lens_out, ntl_stream_t stream);
+
+/* Copy pages src[i] to dst[i], every layer, K and V.  No page may be both read and written. */
+int ntl_cache_copy_pages(const ntl_cache_t* cache, const int32_t* src, const int32_t* dst, int64_t n,
+                         ntl_stream_t stream);
+
+/* Workspace of fork and reserve (n sequences) and of compact (n = 0). */
+int ntl_cache_workspace_size(int64_t pages, int64_t n, uint64_t* bytes_out);
+
+/* Sequences dst[i] (holding nothing) become copies of src[i]: full pages are shared (refs + 1), the
+ * part of a page at the end is copied into the lowest free page (refs <= 0), children served in
+ * order.  granted[i] = 0, and dst[i] stays empty, where no page is left.  dst and src are disjoint
+ * and dst has no repeats. */
+int ntl_cache_fork(const ntl_cache_t* cache, int32_t* table, int64_t table_stride, int64_t seqs, int64_t max_pages,
+                   int32_t* lens, int32_t* refs, const int32_t* src, const int32_t* dst, int64_t n, int32_t* granted,
+                   void* workspace, uint64_t workspace_bytes, ntl_stream_t stream);
+
+/* Map the lowest free pages to the unmapped entries of sequences seq[i] (no repeats) from the page of
+ * their next token up to lens + extra (extra_of[i] where not NULL) tokens, in order; granted[i] = 0, and
+ * nothing is mapped, where the pages or the table's width run out. */
+int ntl_cache_reserve(int64_t pages, int64_t page_size, int32_t* table, int64_t table_stride, int64_t seqs,
+                      int64_t max_pages, const int32_t* lens, int32_t* refs, const int32_t* seq, int64_t n,
+                      int64_t extra, const int32_t* extra_of, int32_t* granted, void* workspace,
+                      uint64_t workspace_bytes, ntl_stream_t stream);
+
+/* Sequences seq[i] give their pages back (refs - 1 for each entry) and hold nothing. */
+int ntl_cache_free(int64_t pages, int32_t* table, int64_t table_stride, int64_t seqs, int64_t max_pages, int32_t* lens,
+                   int32_t* refs, const int32_t* seq, int64_t n, ntl_stream_t stream);
+
+/* Close up the pool: of n live pages (refs > 0), the k-th at or past n moves into the k-th hole before
+ * n, every layer, K and V; table_out and refs_out (which may be table and refs) follow, and
+ * *live = n. */
+int ntl_cache_compact(const ntl_cache_t* cache, const int32_t* table, int64_t table_stride, int32_t* table_out,
+                      int64_t out_stride, int64_t seqs, int64_t max_pages, const int32_t* refs, int32_t* refs_out,
+                      int32_t* live, void* workspace, uint64_t workspace_bytes, ntl_stream_t stream);
+
 /* Generic elementwise programs (outside the families above): run-time compiled kernels.
  * ntl_rtc_build compiles CUDA C `source` (one extern "C" __global__ function named
  * `kernel_name`) with NVRTC for sm_100a on the host, no GPU needed, and returns a handle;

@@ -26,5 +26,15 @@ __all__ = [
     "jit",
     "language",
     "layout",
+    "paged",
     "patch_tilelang",
 ]
+
+
+def __getattr__(name):
+    """``paged`` (the cache and its attention) needs torch, which nothing else here imports up front."""
+    if name == "paged":
+        import importlib
+
+        return importlib.import_module(".paged", __name__)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -17,6 +17,7 @@ _handle = None
 
 c_f32p = ctypes.c_void_p
 c_i64 = ctypes.c_int64
+_p = ctypes.c_void_p
 
 # name -> (restype, argtypes); must match include/ntl_kernels.h
 SIGNATURES = {
@@ -44,6 +45,24 @@ SIGNATURES = {
                                                 ctypes.c_void_p]),
     "ntl_fa2_fwd_f16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, c_i64,
                                        c_i64, c_i64, c_i64, ctypes.c_float, ctypes.c_int, ctypes.c_void_p]),
+    "ntl_tree_attention": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, _p, c_i64, _p, ctypes.c_uint64, _p]),
+    "ntl_window_attention": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, c_i64, c_i64, _p, ctypes.c_uint64, _p]),
+    "ntl_cache_attention_workspace": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p,
+                                                     ctypes.POINTER(ctypes.c_uint64)]),
+    "ntl_tree_mask": (ctypes.c_int, [_p, c_i64, c_i64, c_i64, _p, _p]),
+    "ntl_cache_append": (ctypes.c_int, [ctypes.c_char_p, _p, _p, c_i64, c_i64, c_i64, c_i64, _p, c_i64, c_i64, c_i64,
+                                        _p, _p, c_i64, _p, _p]),
+    "ntl_cache_accept": (ctypes.c_int, [ctypes.c_char_p, _p, c_i64, c_i64, c_i64, _p, _p, c_i64, _p, c_i64, c_i64, _p,
+                                        _p, _p]),
+    "ntl_cache_copy_pages": (ctypes.c_int, [ctypes.c_char_p, _p, _p, c_i64, _p]),
+    "ntl_cache_workspace_size": (ctypes.c_int, [c_i64, c_i64, ctypes.POINTER(ctypes.c_uint64)]),
+    "ntl_cache_fork": (ctypes.c_int, [ctypes.c_char_p, _p, c_i64, c_i64, c_i64, _p, _p, _p, _p, c_i64, _p, _p,
+                                      ctypes.c_uint64, _p]),
+    "ntl_cache_reserve": (ctypes.c_int, [c_i64, c_i64, _p, c_i64, c_i64, c_i64, _p, _p, _p, c_i64, c_i64, _p, _p, _p,
+                                         ctypes.c_uint64, _p]),
+    "ntl_cache_free": (ctypes.c_int, [c_i64, _p, c_i64, c_i64, c_i64, _p, _p, _p, c_i64, _p]),
+    "ntl_cache_compact": (ctypes.c_int, [ctypes.c_char_p, _p, c_i64, _p, c_i64, c_i64, c_i64, _p, _p, _p, _p,
+                                         ctypes.c_uint64, _p]),
     "ntl_rtc_build": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_uint64)]),
     "ntl_rtc_launch": (ctypes.c_int, [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32,
                                       ctypes.POINTER(ctypes.c_void_p), ctypes.c_void_p]),

@@ -1,0 +1,429 @@
+"""A paged key/value cache and the attention that reads it.
+
+A cache is a pair of 16-bit tensors ``k``, ``v`` [pages, page_size, kv_heads, head_dim] (attention reads
+one layer) or [layers, pages, page_size, kv_heads, head_dim] (the cache operators move all layers at
+once; a 4-D cache is one layer).  A sequence is a row of ``table`` (int32 page numbers, -1 where
+there is no page) and its length in ``lens`` (int32); ``refs`` (int32) counts the sequences that hold
+each page.  ``Cache`` keeps the five together.
+
+Tables, lengths and counts stay on the GPU: no call here waits for the device, every call is
+launched on ``torch.cuda.current_stream()`` and may be captured in a CUDA graph.  What a table or
+list says is checked where it is read: a page, position or sequence out of range is skipped.
+
+    cache = Cache(layers=2, pages=256, page_size=16, kv_heads=8, head_dim=128, seqs=4, max_pages=64)
+    cache.reserve(seqs, 100)
+    cache.append(k_new, v_new)                                # [layers, seqs, tokens, kv_heads, head_dim]
+    o = tree_attention(q, cache.k[0], cache.v[0], cache.table, cache.lens, tree_mask(parents))
+    cache.accept(path, counts, drafts)
+
+Kernels: ``csrc/cache_attn.cu`` and ``csrc/cache_pages.cu``, through the C ABI of ``ntl_kernels.h``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import struct
+from functools import lru_cache
+
+import torch
+
+from . import _lib
+
+_CACHE = struct.Struct("=12q")
+_QUERY = struct.Struct("=13qd")
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(index):
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _call(index, name, *args):
+    """The entry point ``name`` on device ``index``'s current stream."""
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _stream(index))
+
+
+def _ints(name, x, index, *shape):
+    """An int32 CUDA tensor on device ``index`` whose sizes are ``shape`` (None: any), last dim dense."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if x.dtype is not torch.int32:
+        raise ValueError(f"{name}: expected dtype int32, got {x.dtype}")
+    if x.dim() != len(shape) or any(want is not None and want != got for want, got in zip(shape, x.shape)):
+        want = tuple("any" if n is None else n for n in shape)
+        raise ValueError(f"{name}: expected shape {want}, got {tuple(x.shape)}")
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        raise ValueError(f"{name} must be dense along its last dimension")
+    if x.get_device() != index:
+        raise ValueError("All tensor arguments must be on the same CUDA device")
+
+
+def _values(name, x):
+    """A 16-bit CUDA tensor that the kernels can read 16 bytes at a time along its last dimension."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"{name}: expected dtype float16 or bfloat16, got {x.dtype}")
+    if x.numel() and (x.stride(-1) != 1 or any(s % 8 for s in x.stride()[:-1])):
+        raise ValueError(f"{name} must be dense along its last dimension, its other strides multiples of 8")
+    if x.data_ptr() % 16:
+        raise ValueError(f"{name} requires a tensor with an inspectable, 16-byte-aligned data pointer")
+
+
+def _cache(k, v, dims):
+    """(descriptor, device index) of a cache; ``dims``: the ranks it may have."""
+    _values("k", k)
+    _values("v", v)
+    shape, stride = k.shape, k.stride()
+    if len(shape) not in dims:
+        raise ValueError(f"k: expected {' or '.join(map(str, dims))} dimensions, got shape {tuple(shape)}")
+    if v.shape != shape or v.stride() != stride or v.dtype is not k.dtype:
+        raise ValueError("k and v must have the same shape, strides and dtype")
+    index = k.get_device()
+    if v.get_device() != index:
+        raise ValueError("All tensor arguments must be on the same CUDA device")
+    if len(shape) == 4:
+        shape, stride = (1, *shape), (0, *stride)
+    if shape[4] % 8 or not shape[4]:
+        raise ValueError(f"k: head_dim {shape[4]} is not a multiple of 8")
+    if not shape[2]:
+        raise ValueError("k: page_size is 0")
+    return _CACHE.pack(k.data_ptr(), v.data_ptr(), *shape, *stride[:4], _DTYPES[k.dtype]), index
+
+
+def _writable(k):
+    if any(n > 1 and s == 0 for n, s in zip(k.shape, k.stride())):
+        raise ValueError("k and v must not be broadcast: their rows are written")
+
+
+@lru_cache(maxsize=1024)
+def _pool_workspace(pages, n):
+    out = ctypes.c_uint64(0)
+    _lib.call("ntl_cache_workspace_size", pages, n, ctypes.byref(out))
+    return out.value
+
+
+def _bytes(n, index):
+    return torch.empty(n, dtype=torch.uint8, device=f"cuda:{index}")
+
+
+# ------------------------------------------------------------------------------ attention
+
+
+@lru_cache(maxsize=1024)
+def _attention_workspace(index, cache_shape, dtype, q_shape, max_pages):
+    """Workspace bytes of an attention call: it depends on sizes alone."""
+    del index
+    pages, page_size, kv_heads, dim = cache_shape
+    cache = _CACHE.pack(16, 16, 1, pages, page_size, kv_heads, dim, 0, 0, 0, 0, dtype)
+    query = _QUERY.pack(16, 16, *q_shape[:3], 0, 0, 0, 16, 0, max_pages, 16, 0, 1.0)
+    out = ctypes.c_uint64(0)
+    _lib.call("ntl_cache_attention_workspace", cache, query, ctypes.byref(out))
+    return out.value
+
+
+def _attend(entry, q, k, v, table, lens, q_lens, scale, out, *args):
+    cache, index = _cache(k, v, (4,))
+    _values("q", q)
+    shape, kv = q.shape, k.shape
+    if len(shape) != 4:
+        raise ValueError(f"q: expected 4 dimensions [seqs, tokens, heads, head_dim], got shape {tuple(shape)}")
+    seqs, tokens, heads, dim = shape
+    if q.dtype is not k.dtype:
+        raise ValueError(f"q: expected dtype {k.dtype} like the cache, got {q.dtype}")
+    if dim != kv[3] or dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, the same for q ({dim}) and the cache ({kv[3]})")
+    if kv[1] % 8:
+        raise ValueError(f"page_size {kv[1]} is not a multiple of 8")
+    if not kv[2] or heads % kv[2] or heads // kv[2] > 128:
+        raise ValueError(f"{heads} query heads cannot share {kv[2]} key heads (a whole number, up to 128 each)")
+    if q.get_device() != index:
+        raise ValueError("All tensor arguments must be on the same CUDA device")
+    _ints("table", table, index, seqs, None)
+    _ints("lens", lens, index, seqs)
+    if q_lens is not None:
+        _ints("q_lens", q_lens, index, seqs)
+    if scale is None:
+        scale = 1.0 / math.sqrt(dim)
+    elif not 0 < scale < 1e30:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    else:
+        _values("out", out)
+        if out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != index:
+            raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(shape)} on q's device")
+        begin, end = out.data_ptr(), out.data_ptr() + out.numel() * 2
+        for name, x in (("q", q), ("k", k), ("v", v)):
+            if x.numel() and out.numel():
+                reach = sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1
+                if x.data_ptr() < end and begin < x.data_ptr() + 2 * reach:
+                    raise ValueError(f"Tensor arguments {name} and out must have disjoint storage")
+    if not out.numel():
+        return out
+    size = _attention_workspace(index, kv, _DTYPES[q.dtype], shape, table.shape[1])
+    work = _bytes(size, index) if size else None
+    stride = q.stride()
+    query = _QUERY.pack(q.data_ptr(), out.data_ptr(), seqs, tokens, heads, *stride[:3], table.data_ptr(),
+                        table.stride(0), table.shape[1], lens.data_ptr(), q_lens.data_ptr() if q_lens is not None else 0,
+                        scale)
+    _call(index, entry, cache, query, *args, work.data_ptr() if size else None, size)
+    return out
+
+
+def tree_mask(parents):
+    """Visibility words of draft trees: int32 [seqs, tokens, ceil(tokens / 32)], bit s % 32 of word
+    s // 32 set where draft s is draft t itself or an ancestor.  ``parents`` int32 [seqs, tokens] holds
+    each draft's parent; what is not an earlier draft (-1) is a root."""
+    if not isinstance(parents, torch.Tensor) or not parents.is_cuda:
+        raise TypeError("parents must be a CUDA tensor")
+    index = parents.get_device()
+    _ints("parents", parents, index, None, None)
+    seqs, tokens = parents.shape
+    words = torch.empty((seqs, tokens, (tokens + 31) // 32), dtype=torch.int32, device=parents.device)
+    _call(index, "ntl_tree_mask", parents.data_ptr(), parents.stride(0), seqs, tokens, words.data_ptr())
+    return words
+
+
+def tree_attention(q, k, v, table, lens, tree, *, q_lens=None, scale=None, out=None):
+    """Attention of drafted tokens over one layer of a cache that already holds their keys and values.
+
+    ``q`` [seqs, tokens, heads, head_dim] (head_dim 64 or 128, heads a multiple of the cache's): sequence
+    b's tokens are the last ``q_lens[b]`` (default: tokens) of its ``lens[b]`` cached ones.  A token sees
+    every key before the drafts, and draft s where bit s of its words in ``tree`` ([seqs or 1, tokens,
+    ceil(tokens / 32)] int32, see ``tree_mask``) is set; a token that sees nothing, and tokens past
+    ``q_lens``, give 0.  ``scale`` defaults to 1 / sqrt(head_dim).  One token with its own bit set is
+    single-token decode.  Returns [seqs, tokens, heads, head_dim] in q's dtype (``out`` if given).
+
+    Statistics and sums are fp32; the exponentials are rounded to the cache's type for the product
+    with V.  A NaN or infinity in a key row reaches the tokens that see it; in a value row that some token
+    of the call sees, it may reach tokens of the same sequence that do not."""
+    if not isinstance(tree, torch.Tensor) or tree.dim() != 3:
+        raise TypeError("tree must be a CUDA tensor [seqs or 1, tokens, words]")
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise TypeError("q must be a CUDA tensor")
+    if q.dim() != 4:
+        raise ValueError(f"q: expected 4 dimensions [seqs, tokens, heads, head_dim], got shape {tuple(q.shape)}")
+    seqs, tokens = q.shape[:2]
+    words = (tokens + 31) // 32
+    shared = tree.shape[0] == 1
+    _ints("tree", tree, q.get_device(), 1 if shared else seqs, tokens, words)
+    if tokens > 1 and tree.stride(1) != words:
+        raise ValueError("tree must be dense along its last two dimensions")
+    return _attend("ntl_tree_attention", q, k, v, table, lens, q_lens, scale, out, tree.data_ptr(),
+                   0 if shared else tree.stride(0))
+
+
+def window_attention(q, k, v, table, lens, window, sinks=0, *, q_lens=None, scale=None, out=None):
+    """Causal attention with a sliding window over one layer of a cache that already holds the new tokens.
+
+    As ``tree_attention``, but the token at position i sees the keys j <= i with j > i - window, or
+    j < sinks (the first tokens, which stay visible).  ``tokens`` may be one (decode) or a prompt's
+    chunk.  Pages wholly outside what the call sees are not read and may be -1 in ``table``."""
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    return _attend("ntl_window_attention", q, k, v, table, lens, q_lens, scale, out, window, sinks)
+
+
+# ------------------------------------------------------------------------------ cache operators
+
+
+def append_tokens(k, v, k_new, v_new, table, lens, counts=None):
+    """Write new tokens' rows, ``k_new`` / ``v_new`` [layers, seqs, tokens, kv_heads, head_dim] (4-D without
+    layers for a 4-D cache), at positions lens[b] + t, t < counts[b] (default: all); returns the new
+    lengths.  A row whose position has no page is dropped: ``reserve`` first."""
+    cache, index = _cache(k, v, (4, 5))
+    _writable(k)
+    _values("k_new", k_new)
+    _values("v_new", v_new)
+    layered = k.dim() == 5
+    if k_new.dim() != k.dim():
+        raise ValueError(f"k_new: expected {k.dim()} dimensions, got shape {tuple(k_new.shape)}")
+    seqs, tokens = k_new.shape[-4], k_new.shape[-3]
+    want = (*k.shape[:1], seqs, tokens, *k.shape[-2:]) if layered else (seqs, tokens, *k.shape[-2:])
+    if k_new.shape != want or k_new.dtype is not k.dtype:
+        raise ValueError(f"k_new: expected {k.dtype} of shape {tuple(want)}, got {k_new.dtype} {tuple(k_new.shape)}")
+    if v_new.shape != want or v_new.dtype is not k.dtype or v_new.stride() != k_new.stride():
+        raise ValueError("k_new and v_new must have the same shape, strides and dtype")
+    if k_new.get_device() != index or v_new.get_device() != index:
+        raise ValueError("All tensor arguments must be on the same CUDA device")
+    _ints("table", table, index, seqs, None)
+    _ints("lens", lens, index, seqs)
+    if counts is not None:
+        _ints("counts", counts, index, seqs)
+    new = torch.empty_like(lens)
+    stride = k_new.stride() if layered else (0, *k_new.stride())
+    _call(index, "ntl_cache_append", cache, k_new.data_ptr(), v_new.data_ptr(), *stride[:4], table.data_ptr(),
+          table.stride(0), seqs, table.shape[1], lens.data_ptr(), counts.data_ptr() if counts is not None else None,
+          tokens, new.data_ptr())
+    return new
+
+
+def accept_path(k, v, table, lens, path, counts, drafts):
+    """Keep a verified path of each sequence's last ``drafts`` cached tokens (an int, or int32 [seqs]): the
+    row of draft path[b, i] moves to draft place i, i < counts[b]; ``path`` int32 [seqs, most] increases along
+    i.  Returns the new lengths, lens - drafts + counts."""
+    cache, index = _cache(k, v, (4, 5))
+    _writable(k)
+    _ints("lens", lens, index, None)
+    seqs = lens.shape[0]
+    _ints("table", table, index, seqs, None)
+    _ints("path", path, index, seqs, None)
+    _ints("counts", counts, index, seqs)
+    each, common = None, 0
+    if isinstance(drafts, torch.Tensor):
+        _ints("drafts", drafts, index, seqs)
+        each = drafts.data_ptr()
+    elif drafts < 0:
+        raise ValueError(f"drafts must be at least 0, got {drafts}")
+    else:
+        common = int(drafts)
+    new = torch.empty_like(lens)
+    _call(index, "ntl_cache_accept", cache, table.data_ptr(), table.stride(0), seqs, table.shape[1], lens.data_ptr(),
+          each, common, path.data_ptr(), path.stride(0), path.shape[1], counts.data_ptr(), new.data_ptr())
+    return new
+
+
+def copy_pages(k, v, src, dst):
+    """Copy pages ``src[i]`` to ``dst[i]`` (int32), all layers, K and V.  No page may be both read and written."""
+    cache, index = _cache(k, v, (4, 5))
+    _writable(k)
+    _ints("src", src, index, None)
+    _ints("dst", dst, index, src.shape[0])
+    _call(index, "ntl_cache_copy_pages", cache, src.data_ptr(), dst.data_ptr(), src.shape[0])
+
+
+def fork(k, v, table, lens, refs, src, dst):
+    """Make sequences ``dst[i]`` (int32, holding nothing, no repeats) copies of ``src[i]``: full pages are shared,
+    the part of a page at the end is copied into the lowest free page, in order.  ``dst`` and ``src`` have no
+    sequence in common.  Updates table, lens and refs in place; returns int32 [n]: 1, or 0 where no
+    page was left and the child holds nothing."""
+    cache, index = _cache(k, v, (4, 5))
+    _writable(k)
+    pages = k.shape[-4]
+    _ints("table", table, index, None, None)
+    _ints("lens", lens, index, table.shape[0])
+    _ints("refs", refs, index, pages)
+    _ints("src", src, index, None)
+    n = src.shape[0]
+    _ints("dst", dst, index, n)
+    granted = torch.empty_like(src)
+    size = _pool_workspace(pages, n)
+    work = _bytes(size, index)
+    _call(index, "ntl_cache_fork", cache, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
+          lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n, granted.data_ptr(), work.data_ptr(), size)
+    return granted
+
+
+def reserve(table, lens, refs, seqs, extra, page_size):
+    """Map the lowest free pages so that each sequence in ``seqs`` (int32, no repeats) can hold ``extra`` (an int,
+    or int32 [n]) more tokens, in order.  Updates table and refs in place; returns int32 [n]: 1, or 0 where
+    the pages or the table's width ran out and nothing was mapped."""
+    if not isinstance(table, torch.Tensor) or not table.is_cuda:
+        raise TypeError("table must be a CUDA tensor")
+    index = table.get_device()
+    _ints("table", table, index, None, None)
+    _ints("lens", lens, index, table.shape[0])
+    _ints("refs", refs, index, None)
+    _ints("seqs", seqs, index, None)
+    n, pages = seqs.shape[0], refs.shape[0]
+    each, common = None, 0
+    if isinstance(extra, torch.Tensor):
+        _ints("extra", extra, index, n)
+        each = extra.data_ptr()
+    elif extra < 0:
+        raise ValueError(f"extra must be at least 0, got {extra}")
+    else:
+        common = int(extra)
+    granted = torch.empty_like(seqs)
+    size = _pool_workspace(pages, n)
+    work = _bytes(size, index)
+    _call(index, "ntl_cache_reserve", pages, int(page_size), table.data_ptr(), table.stride(0), table.shape[0],
+          table.shape[1], lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), n, common, each, granted.data_ptr(),
+          work.data_ptr(), size)
+    return granted
+
+
+def free(table, lens, refs, seqs):
+    """Sequences ``seqs`` (int32) give their pages back and hold nothing; table, lens and refs in place."""
+    if not isinstance(table, torch.Tensor) or not table.is_cuda:
+        raise TypeError("table must be a CUDA tensor")
+    index = table.get_device()
+    _ints("table", table, index, None, None)
+    _ints("lens", lens, index, table.shape[0])
+    _ints("refs", refs, index, None)
+    _ints("seqs", seqs, index, None)
+    _call(index, "ntl_cache_free", refs.shape[0], table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
+          lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), seqs.shape[0])
+
+
+def compact(k, v, table, refs, *, table_out=None, refs_out=None):
+    """Move the live pages (refs > 0) to the lowest numbers: of n, the k-th at or past n goes into the k-th hole
+    before n.  ``table_out`` and ``refs_out`` (default: in place) follow.  Returns int32 [1]: n."""
+    cache, index = _cache(k, v, (4, 5))
+    _writable(k)
+    pages = k.shape[-4]
+    _ints("table", table, index, None, None)
+    _ints("refs", refs, index, pages)
+    table_out = table if table_out is None else table_out
+    refs_out = refs if refs_out is None else refs_out
+    _ints("table_out", table_out, index, *table.shape)
+    _ints("refs_out", refs_out, index, pages)
+    live = torch.empty(1, dtype=torch.int32, device=k.device)
+    size = _pool_workspace(pages, 0)
+    work = _bytes(size, index)
+    _call(index, "ntl_cache_compact", cache, table.data_ptr(), table.stride(0), table_out.data_ptr(),
+          table_out.stride(0), table.shape[0], table.shape[1], refs.data_ptr(), refs_out.data_ptr(), live.data_ptr(),
+          work.data_ptr(), size)
+    return live
+
+
+class Cache:
+    """The tensors of one paged cache and the operators on them.  Every sequence slot starts empty."""
+
+    def __init__(self, *, layers, pages, page_size, kv_heads, head_dim, seqs, max_pages, dtype=torch.float16,
+                 device="cuda"):
+        shape = (layers, pages, page_size, kv_heads, head_dim)
+        self.k = torch.empty(shape, dtype=dtype, device=device)
+        self.v = torch.empty(shape, dtype=dtype, device=device)
+        self.table = torch.full((seqs, max_pages), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(seqs, dtype=torch.int32, device=device)
+        self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
+
+    def reserve(self, seqs, extra):
+        return reserve(self.table, self.lens, self.refs, seqs, extra, self.k.shape[2])
+
+    def append(self, k_new, v_new, counts=None):
+        self.lens = append_tokens(self.k, self.v, k_new, v_new, self.table, self.lens, counts)
+
+    def accept(self, path, counts, drafts):
+        self.lens = accept_path(self.k, self.v, self.table, self.lens, path, counts, drafts)
+
+    def fork(self, src, dst):
+        return fork(self.k, self.v, self.table, self.lens, self.refs, src, dst)
+
+    def free(self, seqs):
+        free(self.table, self.lens, self.refs, seqs)
+
+    def copy_pages(self, src, dst):
+        copy_pages(self.k, self.v, src, dst)
+
+    def compact(self):
+        return compact(self.k, self.v, self.table, self.refs)
+
+    def tree_attention(self, layer, q, tree, **kwargs):
+        return tree_attention(q, self.k[layer], self.v[layer], self.table, self.lens, tree, **kwargs)
+
+    def window_attention(self, layer, q, window, sinks=0, **kwargs):
+        return window_attention(q, self.k[layer], self.v[layer], self.table, self.lens, window, sinks, **kwargs)
+
+
+__all__ = ["Cache", "accept_path", "append_tokens", "compact", "copy_pages", "fork", "free", "reserve",
+           "tree_attention", "tree_mask", "window_attention"]
