@@ -1,120 +1,979 @@
-// Attention of a few new tokens over a paged key/value cache: a tree of drafted tokens, or causal
-// with a sliding window and a few first tokens that stay visible.
+// Attention of a few new tokens over a paged key/value cache, on sm_100a tensor cores (TMA, tcgen05
+// MMA, TMEM accumulators): a tree of drafted tokens, or causal with a sliding window and a few first
+// tokens that stay visible.
 //
 // For query row (sequence b, token t, head h), over the keys j it sees:
 //   s_j = scale * q . k_j ; m = max s ; o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
-// in 32 bits, rounded once; a row that sees nothing gives 0.
+// scores, m, sums and o in fp32; the exponentials are rounded to the cache's type for the product
+// with V (the tensor core multiplies 16-bit operands), o once at the end.  A row that sees nothing
+// gives 0.
+//
+// Work.  A unit is (sequence, key head, block of tokens): its rows are the block's tokens times the
+// G query heads of the key head, packed token-major into one or two 128-row tiles, so each key and value
+// row is read once for all of them.  A unit's key axis is cut into tiles; all units' tiles form one
+// line (ordered by sequence, token block, key head) that is cut into equal pieces, one per CTA.  A CTA
+// runs its piece as one stream of tiles; a unit inside one piece is finished there, a unit cut between
+// pieces leaves (o, m, l) parts in the workspace that cache_attn_join adds up in order.  So ragged
+// lengths balance by themselves, from lengths that only the device knows.
+//
+// Two shapes of CTA, chosen by the rows a unit has (see launch()):
+//   NT = 1: one 128-row tile, 64-key tiles, two CTAs per SM (one loads and multiplies while the other
+//           is in its softmax or between units).  For up to 128 rows: decode and small trees, bound by
+//           HBM.  S is double-buffered, so Q K^T of the next tile runs during the softmax.
+//   NT = 2: two 128-row tiles that share every K and V tile, 128-key tiles, one CTA per SM.  For wide
+//           trees and prompt chunks, bound by the tensor cores and the exponentials.
+// Warps: 4 per row tile for the softmax (one thread per row = TMEM lane; the same thread rescales
+// and writes out the row), then one each for MMA issue, K/V loads, Q loads, and clearing value rows past
+// the sequence's end (a page's unwritten rows may hold NaN, and 0 * NaN is not 0).
+// Every wait is bounded: one that gives up records a status code, and the CTA drains its copies
+// and MMAs, frees TMEM and returns.
+#include <atomic>
 #include <cuda_bf16.h>
+#include <mutex>
 
 #include "ntl_common.cuh"
 
 namespace {
 
+__device__ uint32_t g_cache_attn_status;
+
+constexpr int BM = 128;                // rows per tile
+constexpr float kRescaleLog2 = 8.0f;   // o is rescaled when the maximum rose by more than 2^8
+
 struct AttnParams {
-  const uint16_t* q;
   uint16_t* o;
-  const uint16_t* k;
-  const uint16_t* v;
   const int32_t* table;
   const int32_t* lens;
-  const int32_t* q_lens;
-  const uint32_t* tree;  // null: window
-  int64_t table_stride, q_seq, q_token, q_head, page_stride, row_stride, head_stride, tree_stride;
+  const int32_t* q_lens;  // null: every sequence has `tokens`
+  const uint32_t* tree;   // null: window
+  float* part;            // workspace: [2 * ctas][rows][D] values, then [2 * ctas][rows] (m, l)
+  float2* part_ml;
+  int4* head;             // [ctas] the unit a CTA begins and does not end: {item, key head, last CTA, -}
+  int64_t table_stride, tree_stride;
   int seqs, tokens, heads, kv_heads, group, pages, page_size, max_pages, words, window, sinks;
-  float scale_log2;
+  int tile_tokens;   // tokens per 128-row tile
+  int blocks;        // token blocks per sequence (units of NT tiles)
+  int tile_keys;     // keys per tile: whole pages, or a divisor of a page
+  int tile_pages;    // pages per tile (1 where a page holds several tiles)
+  int rows;          // rows a workspace slot has
+  int min_tiles;     // least tiles per CTA
+  float c;           // softmax scale in log2 units
+  int64_t wait_limit;
 };
 
-template <bool BF16>
-__device__ __forceinline__ float to_float(uint16_t x) {
-  if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(x) << 16);
-  return __half2float(__ushort_as_half(x));
-}
-template <bool BF16>
-__device__ __forceinline__ uint16_t from_float(float x) {
-  if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
-  return __half_as_ushort(__float2half_rn(x));
+template <int D, int NT>
+struct Shape {
+  static constexpr int BN = NT == 1 ? 64 : 128;  // keys per tile
+  static constexpr int STAGES = D == 64 ? 4 : 2;  // of K and of V
+  static constexpr int SOFTMAX_WARPS = 4 * NT;
+  static constexpr int MMA_WARP = SOFTMAX_WARPS, KV_WARP = MMA_WARP + 1, Q_WARP = MMA_WARP + 2, FIX_WARP = MMA_WARP + 3;
+  static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);
+  static constexpr int CTAS_PER_SM = NT == 1 ? 2 : 1;
+  static constexpr int Q_BYTES = BM * D * 2;
+  static constexpr int KV_BYTES = BN * D * 2;
+  static constexpr int K_OFF = NT * Q_BYTES;
+  static constexpr int V_OFF = K_OFF + STAGES * KV_BYTES;
+  static constexpr int CTL_OFF = V_OFF + STAGES * KV_BYTES;
+  static constexpr uint32_t TMEM_COLS = NT == 1 ? 256 : 512;
+  // S buffer i (NT = 1: of every other key tile; NT = 2: of row tile i), O of row tile i.
+  __host__ __device__ static constexpr uint32_t S_COL(int i) { return static_cast<uint32_t>(i * BN); }
+  __host__ __device__ static constexpr uint32_t O_COL(int i) { return static_cast<uint32_t>(2 * BN + i * D); }
+};
+
+struct __align__(16) Ctl {
+  uint64_t q_full, q_empty;
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t v_raw[4];    // a V tile with rows past the end has landed: v_full follows once they are cleared
+  uint64_t s_full[2];   // S buffer holds scores
+  uint64_t p_ready[2];  // S buffer holds exponentials (4 warps)
+  uint64_t pv_done[2];  // row tile i: P V of one more key tile is complete
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+  int start[5];  // first unit's item, key head, tile; tiles of this CTA; total tiles
+  int sums[32];
+};
+
+template <int D, int NT>
+constexpr int smem_bytes() {
+  const int used = Shape<D, NT>::CTL_OFF + static_cast<int>(sizeof(Ctl)) + 1024;
+  // One CTA per SM needs >= 116 KB, so that its 512-column TMEM allocation never contends.
+  return NT == 2 && used < 118784 ? 118784 : used;
 }
 
-// One warp per query row.
-template <int D, bool BF16>
-__global__ void cache_attn_simple(const AttnParams p) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  if (w >= static_cast<int64_t>(p.seqs) * p.tokens * p.heads) return;
-  const int h = w % p.heads, t = (w / p.heads) % p.tokens, b = w / p.heads / p.tokens;
-  const int len = min(static_cast<int64_t>(max(p.lens[b], 0)), static_cast<int64_t>(p.max_pages) * p.page_size);
-  const int n = min(len, p.q_lens ? min(max(p.q_lens[b], 0), p.tokens) : p.tokens);
-  const int prefix = len - n, pos = prefix + t;
-  float q[E], o[E] = {}, m = -INFINITY, l = 0;
-  for (int e = 0; e < E; ++e)
-    q[e] = to_float<BF16>(p.q[b * p.q_seq + t * p.q_token + h * p.q_head + e * 32 + lane]);
-  const int last = p.tree ? len : pos + 1;
-  for (int j = 0; j < last && t < n; ++j) {
-    if (p.tree) {
-      const int s = j - prefix;
-      if (s >= 0 && !(p.tree[b * p.tree_stride + static_cast<int64_t>(t) * p.words + (s >> 5)] >> (s & 31) & 1))
-        continue;
-    } else if (pos - j >= p.window && j >= p.sinks) {
-      continue;
-    }
-    const int page = p.table[b * p.table_stride + j / p.page_size];
-    if (page < 0 || page >= p.pages) continue;
-    const int64_t at = page * p.page_stride + (j % p.page_size) * p.row_stride + (h / p.group) * p.head_stride + lane;
-    float s = 0;
-    for (int e = 0; e < E; ++e) s += q[e] * to_float<BF16>(p.k[at + e * 32]);
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= p.scale_log2;
-    const float top = fmaxf(m, s), old = m == -INFINITY ? 0.f : exp2f(m - top), x = exp2f(s - top);
-    l = l * old + x;
-    for (int e = 0; e < E; ++e) o[e] = o[e] * old + x * to_float<BF16>(p.v[at + e * 32]);
-    m = top;
+// Register split of the one-CTA-per-SM shape: the softmax threads hold a row's 128 scores.
+constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 200, REGS_OTHER = 104;
+static_assert(8 * REGS_SOFTMAX + 4 * REGS_OTHER == 12 * REGS_LAUNCH, "register split must match the launch");
+
+__device__ __forceinline__ void give_up(Ctl* ctl, uint32_t code) {
+  if (!*reinterpret_cast<volatile int*>(&ctl->abort)) atomicCAS(&g_cache_attn_status, 0u, code);
+  *reinterpret_cast<volatile int*>(&ctl->abort) = 1;
+}
+
+// A wait of a whole warp, which gives up as one: no lane goes on without the others.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int64_t limit, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, limit, abort_flag));
+}
+
+// ------------------------------------------------------------------------------ units
+
+struct Unit {
+  int b, t0;        // sequence, first token
+  int len, live;    // cached tokens; new tokens among them
+  int tiles, sink_tiles, first;  // key tiles; those of the sinks; the window's first
+};
+
+__device__ __forceinline__ Unit unit_of(const AttnParams& p, int item, int block_tokens) {
+  Unit u;
+  u.b = item / p.blocks;
+  u.t0 = (item - u.b * p.blocks) * block_tokens;
+  const int64_t room = static_cast<int64_t>(p.max_pages) * p.page_size;
+  u.len = static_cast<int>(min(static_cast<int64_t>(max(p.lens[u.b], 0)), room));
+  u.live = min(u.len, p.q_lens ? min(max(p.q_lens[u.b], 0), p.tokens) : p.tokens);
+  u.tiles = 1;  // a unit without keys has one tile that nothing sees, and writes zeros
+  u.sink_tiles = u.first = 0;
+  if (u.t0 >= u.live) return u;
+  if (p.tree) {
+    u.tiles = max(1, (u.len + p.tile_keys - 1) / p.tile_keys);
+  } else {
+    const int prefix = u.len - u.live;
+    const int last = prefix + min(u.t0 + block_tokens, u.live) - 1;
+    u.first = max(0, prefix + u.t0 - p.window + 1) / p.tile_keys;
+    u.sink_tiles = min(u.first, static_cast<int>((static_cast<int64_t>(p.sinks) + p.tile_keys - 1) / p.tile_keys));
+    u.tiles = u.sink_tiles + last / p.tile_keys - u.first + 1;
   }
-  for (int e = 0; e < E; ++e) p.o[w * D + e * 32 + lane] = from_float<BF16>(l > 0 ? o[e] / l : (l == l ? 0.f : l));
+  return u;
+}
+
+__device__ __forceinline__ int tile_key(const AttnParams& p, const Unit& u, int a) {
+  return (a < u.sink_tiles ? a : u.first + a - u.sink_tiles) * p.tile_keys;
+}
+
+// Whether the tile holds rows at or past the sequence's end, which V must not multiply as they are.
+__device__ __forceinline__ bool past_end(const AttnParams& p, const Unit& u, int a) {
+  return u.len - tile_key(p, u, a) < p.tile_keys;
+}
+
+// The pieces: `total` tiles over `ctas` CTAs, CTA i from piece_start(i).
+__device__ __forceinline__ int piece_start(int i, int total, int ctas) {
+  return static_cast<int>(static_cast<int64_t>(i) * total / ctas);
+}
+__device__ __forceinline__ int piece_of(int tile, int total, int ctas) {
+  return static_cast<int>(((static_cast<int64_t>(tile) + 1) * ctas - 1) / total);
+}
+
+__device__ __forceinline__ int block_exclusive(int x, int* sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int s = x;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, s, d);
+    if (lane >= d) s += y;
+  }
+  if (lane == 31) sums[warp] = s;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+  for (int w = 0; w < warps; ++w) {
+    const int n = sums[w];
+    if (w < warp) before += n;
+    total += n;
+  }
+  __syncthreads();
+  return before + s - x;
+}
+
+// Finds this CTA's piece (ctl->start); all threads.  Returns the CTAs that have a piece.
+__device__ __forceinline__ int find_piece(const AttnParams& p, Ctl* ctl, int block_tokens) {
+  const int items = p.seqs * p.blocks;
+  int total = 0, mine = 0, at = 0;
+  for (int e0 = 0; e0 < items; e0 += blockDim.x) {
+    const int e = e0 + threadIdx.x;
+    mine = e < items ? unit_of(p, e, block_tokens).tiles * p.kv_heads : 0;
+    int sum;
+    at = total + block_exclusive(mine, ctl->sums, sum);
+    total += sum;
+  }
+  const int ctas = max(1, min(static_cast<int>(gridDim.x), total / p.min_tiles));
+  if (static_cast<int>(blockIdx.x) >= ctas) return ctas;
+  const int begin = piece_start(blockIdx.x, total, ctas), end = piece_start(blockIdx.x + 1, total, ctas);
+  int seen = 0;
+  for (int e0 = 0; e0 < items; e0 += blockDim.x) {
+    const int e = e0 + threadIdx.x;
+    if (items > static_cast<int>(blockDim.x)) {
+      mine = e < items ? unit_of(p, e, block_tokens).tiles * p.kv_heads : 0;
+      int sum;
+      at = seen + block_exclusive(mine, ctl->sums, sum);
+      seen += sum;
+    }
+    if (mine > 0 && at <= begin && begin < at + mine) {
+      const int tiles = mine / p.kv_heads;
+      ctl->start[0] = e;
+      ctl->start[1] = (begin - at) / tiles;
+      ctl->start[2] = (begin - at) % tiles;
+      ctl->start[3] = end - begin;
+      ctl->start[4] = total;
+    }
+  }
+  return ctas;
+}
+
+// The tiles of a CTA in order; every role walks its own copy.
+struct Walk {
+  int item, kv_head, tile, left;
+  Unit u;
+  int a0, a1;  // this unit's tiles in this CTA
+
+  __device__ __forceinline__ void begin(const AttnParams& p, const Ctl* ctl, int block_tokens) {
+    item = ctl->start[0];
+    kv_head = ctl->start[1];
+    tile = ctl->start[2];
+    left = ctl->start[3];
+    u = unit_of(p, item, block_tokens);
+    a0 = tile;
+    a1 = min(u.tiles, a0 + left);
+  }
+  __device__ __forceinline__ bool next(const AttnParams& p, int block_tokens) {
+    left -= a1 - a0;
+    if (left <= 0) return false;
+    if (++kv_head == p.kv_heads) {
+      kv_head = 0;
+      u = unit_of(p, ++item, block_tokens);
+    }
+    a0 = 0;
+    a1 = min(u.tiles, left);
+    return true;
+  }
+};
+
+// ------------------------------------------------------------------------------ PTX
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t x, int32_t y,
+                                            int32_t z, int32_t w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// kind::f16 instruction descriptor (see umma_idesc_f16_f32) with both operands fp16 or both bf16.
+template <bool BF16>
+__host__ __device__ constexpr uint32_t idesc(uint32_t n, uint32_t b_mn_major) {
+  return umma_idesc_f16_f32(BM, n, 0, b_mn_major) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// The x low bits of 64 (none for x <= 0, all for x >= 64).
+__device__ __forceinline__ uint64_t low_bits(int x) {
+  return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1;
+}
+
+// Which of the 64 keys from k0 on the row sees.
+__device__ __forceinline__ uint64_t visible(const AttnParams& p, const Unit& u, int t, int k0) {
+  const int prefix = u.len - u.live;
+  if (!p.tree) {
+    const int pos = prefix + t;
+    return low_bits(pos + 1 - k0) & (~low_bits(pos - p.window + 1 - k0) | low_bits(p.sinks - k0));
+  }
+  uint64_t bits = low_bits(prefix - k0);
+  if (k0 + 64 > prefix) {
+    const uint32_t* row = p.tree + u.b * p.tree_stride + static_cast<int64_t>(t) * p.words;
+    const int s0 = k0 - prefix;  // draft at bit 0
+    const int w0 = s0 >> 5;      // floor
+    uint64_t lo = 0, hi = 0;     // words w0 .. w0 + 2
+    if (w0 >= 0 && w0 < p.words) lo = row[w0];
+    if (w0 + 1 >= 0 && w0 + 1 < p.words) lo |= static_cast<uint64_t>(row[w0 + 1]) << 32;
+    if (w0 + 2 >= 0 && w0 + 2 < p.words) hi = row[w0 + 2];
+    const int sh = s0 & 31;
+    uint64_t drafts = lo >> sh;
+    if (sh) drafts |= hi << (64 - sh);
+    bits |= drafts & ~low_bits(prefix - k0);
+  }
+  return bits & low_bits(u.len - k0);
+}
+
+// ------------------------------------------------------------------------------ kernel
+
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_SM)
+    cache_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                      const __grid_constant__ CUtensorMap tv, const AttnParams p) {
+  using C = Shape<D, NT>;
+  constexpr int BN = C::BN, ST = C::STAGES;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL_OFF);
+  volatile int* abort_flag = &ctl->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int block_tokens = NT * p.tile_tokens;
+
+  pdl_trigger();
+  const int ctas = find_piece(p, ctl, block_tokens);
+  if (static_cast<int>(blockIdx.x) >= ctas) {
+    if (threadIdx.x == 0) p.head[blockIdx.x] = make_int4(0, 0, -1, 0);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(&ctl->q_full, 1);
+    mbar_init(&ctl->q_empty, 1);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&ctl->k_full[s], 1);
+      mbar_init(&ctl->k_empty[s], 1);
+      mbar_init(&ctl->v_full[s], 1);
+      mbar_init(&ctl->v_empty[s], 1);
+      mbar_init(&ctl->v_raw[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->s_full[i], 1);
+      mbar_init(&ctl->p_ready[i], 4);
+      mbar_init(&ctl->pv_done[i], 1);
+    }
+    mbar_init(&ctl->drain, 1);
+    ctl->abort = 0;
+    fence_mbar_init();
+  }
+  if (p.tile_keys < BN) {
+    // Rows of the V stages that no page reaches: zero once, no copy writes them.
+    const int spare = (BN - p.tile_keys) * 8;  // 16-byte units per 64-column half
+    for (int e = threadIdx.x; e < ST * (D / 64) * spare; e += blockDim.x) {
+      const int half = e / spare, at = e % spare;
+      *reinterpret_cast<uint4*>(smem + C::V_OFF + half * (BN * 128) + p.tile_keys * 128 + at * 16) =
+          make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
+  }
+  if (warp == C::MMA_WARP) {
+    tmem_alloc(&ctl->tmem_base, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem_base;
+  Walk w;
+  w.begin(p, ctl, block_tokens);
+
+  if (warp >= C::SOFTMAX_WARPS) {
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS_OTHER) : "memory");
+    if (warp == C::KV_WARP) {
+      // ---------------------------------------------- K and V loads, one lane per page of the tile
+      // Lane 0 waits for the whole warp, so that either every lane issues its boxes or none does.
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const bool ok = lane != 0 || mbar_wait_bounded(bar, parity, p.wait_limit, abort_flag);
+        return __shfl_sync(0xffffffffu, ok, 0);
+      };
+      const int boxes = p.tile_pages;
+      const int box_keys = p.tile_keys / boxes;
+      const int box_bytes = box_keys * 128;  // one page's rows of one 64-column half
+      const uint32_t tile_bytes = static_cast<uint32_t>(boxes * box_bytes * (D / 64));
+      bool ok = true;
+      int k_issued = 0, v_issued = 0;
+      uint32_t raw = 0, cleared = 0;  // bit s: parity of the next v_raw[s]; stage s's last V tile is one to clear
+      do {
+        const int lo = p.tree ? 0 : max(0, w.u.len - w.u.live + w.u.t0 - p.window + 1);  // the window's first key
+        const int32_t* row = p.table + w.u.b * p.table_stride;
+        // A page that the unit sees nothing of, or that is not there, reads as zeros (the tensor
+        // map fills what lies outside it), so a page given back or never written is not touched.
+        auto page_at = [&](int a) -> int {
+          const int k0 = tile_key(p, w.u, a) + lane * box_keys;
+          const int j = k0 / p.page_size;
+          if (lane >= boxes || j >= p.max_pages || k0 >= w.u.len || (k0 + box_keys <= lo && k0 >= p.sinks)) return -1;
+          return row[j];
+        };
+        int next_page = page_at(w.a0);
+        for (int a = w.a0; a < w.a1; ++a) {
+          const int s = k_issued % ST;
+          const uint32_t parity = ((k_issued / ST) & 1) ^ 1;
+          const int y = boxes > 1 ? 0 : tile_key(p, w.u, a) % p.page_size;
+          const int page = next_page;
+          if (a + 1 < w.a1) next_page = page_at(a + 1);
+          if (!(ok = wait(&ctl->k_empty[s], parity))) break;
+          if (lane == 0) mbar_arrive_expect_tx(&ctl->k_full[s], tile_bytes);
+          __syncwarp();
+          uint8_t* to = smem + C::K_OFF + s * C::KV_BYTES + lane * box_bytes;
+          if (lane < boxes) {
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+              tma_load_4d(to + d * (BN * 128), &tk, &ctl->k_full[s], d * 64, w.kv_head, y, page);
+          }
+          ++k_issued;
+          if (!(ok = wait(&ctl->v_empty[s], parity))) break;
+          const bool clear = past_end(p, w.u, a);
+          uint64_t* landed = clear ? &ctl->v_raw[s] : &ctl->v_full[s];
+          if (clear) raw ^= 1u << s;
+          cleared = clear ? cleared | 1u << s : cleared & ~(1u << s);
+          if (lane == 0) mbar_arrive_expect_tx(landed, tile_bytes);
+          __syncwarp();
+          to += C::V_OFF - C::K_OFF;
+          if (lane < boxes) {
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+              tma_load_4d(to + d * (BN * 128), &tv, landed, d * 64, w.kv_head, y, page);
+          }
+          ++v_issued;
+        }
+      } while (ok && w.next(p, block_tokens));
+      if (!ok && lane == 0) {
+        give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
+        // Drain every copy this warp issued before the CTA exits.
+        for (int j = max(0, k_issued - ST); j < k_issued; ++j)
+          if (!mbar_wait_bounded(&ctl->k_full[j % ST], (j / ST) & 1, int64_t(1) << 24, nullptr))
+            atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
+        for (int j = max(0, v_issued - ST); j < v_issued; ++j) {
+          const int s = j % ST;
+          const bool clear = cleared >> s & 1;
+          if (!mbar_wait_bounded(clear ? &ctl->v_raw[s] : &ctl->v_full[s], clear ? ~raw >> s & 1 : (j / ST) & 1,
+                                 int64_t(1) << 24, nullptr))
+            atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
+        }
+      }
+    } else if (warp == C::Q_WARP) {
+      // ---------------------------------------------- Q loads: the next unit's, once the last Q K^T retired
+      if (lane == 0) {
+        const uint32_t bytes = static_cast<uint32_t>(NT * (D / 64) * p.tile_tokens * p.group * 128);
+        bool ok = true;
+        int n = 0;
+        do {
+          if (n > 0 && !(ok = mbar_wait_bounded(&ctl->q_empty, (n - 1) & 1, p.wait_limit, abort_flag))) break;
+          mbar_arrive_expect_tx(&ctl->q_full, bytes);
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+              tma_load_4d(smem + i * C::Q_BYTES + d * (BM * 128), &tq, &ctl->q_full, d * 64, w.kv_head * p.group,
+                          w.u.t0 + i * p.tile_tokens, w.u.b);
+          ++n;
+        } while (w.next(p, block_tokens));
+        if (!ok) give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
+        // The MMA thread waits for each load; if it gave up, this thread does before the CTA exits.
+        if (!mbar_wait_bounded(&ctl->q_full, (n - 1) & 1, int64_t(1) << 24, nullptr))
+          atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
+      }
+    } else if (warp == C::FIX_WARP) {
+      // ---------------------------------------------- value rows past the sequence's end become zeros
+      bool ok = true;
+      int g = 0;
+      uint32_t raw = 0;  // bit s: parity of v_raw[s]
+      do {
+        for (int a = w.a0; a < w.a1 && ok; ++a, ++g) {
+          if (!past_end(p, w.u, a)) continue;
+          const int s = g % ST;
+          if (lane == 0) ok = mbar_wait_bounded(&ctl->v_raw[s], raw >> s & 1, p.wait_limit, abort_flag);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) break;
+          raw ^= 1u << s;
+          const int rows = w.u.len - tile_key(p, w.u, a);  // rows that hold tokens
+          const int first = max(rows, 0);
+          const int units = (p.tile_keys - first) * 8;  // 16-byte units per half
+          for (int e = lane; e < (D / 64) * units; e += 32) {
+            const int half = e / units, at = e - half * units;
+            *reinterpret_cast<uint4*>(smem + C::V_OFF + s * C::KV_BYTES + half * (BN * 128) + first * 128 + at * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->v_full[s]);
+        }
+      } while (ok && w.next(p, block_tokens));
+      if (!ok && lane == 0) give_up(ctl, NTL_STATUS_SOFTMAX_WAIT);
+    } else if (elect_one_lane()) {
+      // ---------------------------------------------- MMA issue
+      constexpr uint32_t idesc_s = idesc<BF16>(BN, 0);  // B = K tile, K-major
+      constexpr uint32_t idesc_o = idesc<BF16>(D, 1);   // B = V tile, N-major
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        if (mbar_wait_bounded(bar, parity, p.wait_limit, abort_flag)) return true;
+        give_up(ctl, NTL_STATUS_MMA_FULL_WAIT);
+        return false;
+      };
+      // Two cursors over the same tiles: Q K^T runs one tile ahead of P V.
+      Walk wq = w;
+      int gq = 0, aq = wq.a0, uq = 0;
+      bool more = true;
+      auto qk_ready = [&]() -> bool {
+        if (aq == wq.a0 && !wait(&ctl->q_full, uq & 1)) return false;
+        return wait(&ctl->k_full[gq % ST], (gq / ST) & 1);
+      };
+      auto qk = [&](int i) {  // S (buffer gq % 2, or row tile i) = Q_i K^T
+        const uint32_t q_addr = smem_u32(smem + (NT == 2 ? i : 0) * C::Q_BYTES);
+        const uint32_t k_addr = smem_u32(smem + C::K_OFF + (gq % ST) * C::KV_BYTES);
+        const int buf = NT == 2 ? i : gq & 1;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t q_off = (kk >> 2) * (BM * 128) + (kk & 3) * 32, k_off = (kk >> 2) * (BN * 128) + (kk & 3) * 32;
+          tc_mma_f16_ss(tmem + C::S_COL(buf), umma_desc_sw128(q_addr + q_off, 16, 1024),
+                        umma_desc_sw128(k_addr + k_off, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&ctl->s_full[buf]);
+      };
+      auto qk_end = [&]() {  // after the last row tile's
+        tc_commit(&ctl->k_empty[gq % ST]);
+        ++gq;
+        if (++aq == wq.a1) {
+          tc_commit(&ctl->q_empty);
+          more = wq.next(p, block_tokens);
+          aq = wq.a0;
+          ++uq;
+        }
+      };
+      if ((ok = qk_ready())) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) qk(i);
+        qk_end();
+      }
+      int g = 0;
+      bool left = ok;
+      while (left) {
+        for (int a = w.a0; a < w.a1 && ok; ++a, ++g) {
+          const int s = g % ST;
+          auto pv = [&](int i) -> bool {  // O_i += P V
+            const int buf = NT == 2 ? i : g & 1;
+            if (!wait(&ctl->p_ready[buf], (NT == 2 ? g : g >> 1) & 1)) return false;
+            tc_fence_after();
+            const uint32_t v_addr = smem_u32(smem + C::V_OFF + s * C::KV_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < BN / 16; ++kk)
+              tc_mma_f16_ts(tmem + C::O_COL(i), tmem + C::S_COL(buf) + kk * 8,
+                            umma_desc_sw128(v_addr + kk * 2048, BN * 128, 1024), idesc_o, (a > w.a0 || kk > 0) ? 1u : 0u);
+            tc_commit(&ctl->pv_done[i]);
+            return true;
+          };
+          if constexpr (NT == 1) {
+            if (more) {
+              if (!(ok = qk_ready())) break;
+              qk(0);
+              qk_end();
+            }
+            if (!(ok = wait(&ctl->v_full[s], (g / ST) & 1) && pv(0))) break;
+          } else {
+            if (!(ok = wait(&ctl->v_full[s], (g / ST) & 1) && pv(0))) break;
+            const bool ahead = more;
+            if (ahead) {
+              if (!(ok = qk_ready())) break;
+              qk(0);
+            }
+            if (!(ok = pv(1))) break;
+            if (ahead) {
+              qk(1);
+              qk_end();
+            }
+          }
+          tc_commit(&ctl->v_empty[s]);
+        }
+        left = ok && w.next(p, block_tokens);
+      }
+      if (!ok) {
+        tc_commit(&ctl->drain);
+        if (!mbar_wait_bounded(&ctl->drain, 0, int64_t(1) << 24, nullptr))
+          atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
+      }
+    }
+  } else {
+    // ---------------------------------------------- softmax: one thread per row
+    if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS_SOFTMAX) : "memory");
+    const int i = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;
+    const int row_token = r / p.group, row_head = r - row_token * p.group;
+    const int t_in_block = i * p.tile_tokens + row_token;
+    const bool in_tile = row_token < p.tile_tokens;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t o_addr = tmem + lane_off + C::O_COL(i);
+    const float c = p.c;
+    int4 cut = make_int4(0, 0, -1, 0);
+    bool ok = true;
+    int g = 0;
+    do {
+      const Unit& u = w.u;
+      const int t = u.t0 + t_in_block;
+      const bool live = in_tile && t < u.live;
+      const bool any = __any_sync(0xffffffffu, live);
+      // Keys that every row of this row tile sees: [0, all_hi), or for the window [all_lo, all_hi)
+      // and the sinks.
+      const int prefix = u.len - u.live;
+      const int t_first = u.t0 + i * p.tile_tokens, t_last = min(t_first + p.tile_tokens, u.live) - 1;
+      const int all_hi = p.tree ? prefix : prefix + t_first + 1;
+      const int all_lo = p.tree ? 0 : prefix + t_last - p.window + 1;
+      float m = -INFINITY, l = 0.0f;
+      for (int a = w.a0; a < w.a1; ++a, ++g) {
+        const int buf = NT == 2 ? i : g & 1;
+        const uint32_t s_addr = tmem + lane_off + C::S_COL(buf);
+        if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g >> 1) & 1, p.wait_limit, abort_flag))) break;
+        if (any) {
+          tc_fence_after();
+          uint32_t sv[BN];
+#pragma unroll
+          for (int ch = 0; ch < BN / 32; ++ch)
+            tmem_ld_32x32b_x32(s_addr + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + ch * 32));
+          tc_wait_ld();
+          const int k0 = tile_key(p, u, a);
+          const bool whole = p.tile_keys == BN && k0 + BN <= all_hi && (k0 >= all_lo || k0 + BN <= p.sinks);
+          if (!whole) {
+#pragma unroll
+            for (int ch = 0; ch < BN / 64; ++ch) {
+              uint64_t see = live ? visible(p, u, t, k0 + ch * 64) & low_bits(p.tile_keys - ch * 64) : 0;
+#pragma unroll
+              for (int e = 0; e < 64; ++e)
+                if (!(see >> e & 1)) sv[ch * 64 + e] = __float_as_uint(-INFINITY);
+            }
+          }
+          float top;
+          {
+            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < BN; e += 8) {
+              x[0] = fmax3(x[0], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+              x[1] = fmax3(x[1], __uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3]));
+              x[2] = fmax3(x[2], __uint_as_float(sv[e + 4]), __uint_as_float(sv[e + 5]));
+              x[3] = fmax3(x[3], __uint_as_float(sv[e + 6]), __uint_as_float(sv[e + 7]));
+            }
+            top = fmax3(fmaxf(x[0], x[1]), x[2], x[3]);
+          }
+          float scale_old = 1.0f;
+          bool moved = false;
+          if (m == -INFINITY) {
+            m = top;  // nothing seen so far: o and l are zero (or not begun)
+          } else if ((top - m) * c > kRescaleLog2) {
+            scale_old = ex2_approx((m - top) * c);
+            m = top;
+            moved = true;
+          }
+          const bool rescale = __any_sync(0xffffffffu, moved);
+          // NT = 1: S of this tile was issued before P V of the tile before, which is waited for here
+          // where o is about to change, and on the unit's last tile: before this warp hands over P,
+          // pv_done is at most one phase behind, so the wait after it is not a phase early.
+          // (NT = 2 issued S after that P V: it is complete.)
+          if (NT == 1 && g > 0 && (rescale || a + 1 == w.a1) &&
+              !(ok = warp_wait(&ctl->pv_done[0], (g - 1) & 1, p.wait_limit, abort_flag)))
+            break;
+          if (rescale) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int ch = 0; ch < D / 32; ++ch) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(o_addr + ch * 32, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale_old);
+              tmem_st_32x32b_x32(o_addr + ch * 32, o);
+            }
+          }
+          const float shift = m == -INFINITY ? 0.0f : -m * c;
+          const uint64_t c2 = f2_make(c, c), shift2 = f2_make(shift, shift);
+          uint64_t acc[2] = {0ull, 0ull};
+#pragma unroll
+          for (int ch = 0; ch < BN / 32; ++ch) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int k = ch * 32 + 2 * e;
+              float x0, x1;
+              f2_split(f2_fma(f2_make(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), c2, shift2), x0, x1);
+              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              acc[e & 1] = f2_add(acc[e & 1], f2_make(p0, p1));
+              packed[e] = pack2<BF16>(p0, p1);
+            }
+            tmem_st_32x32b_x16(s_addr + ch * 16, packed);
+          }
+          float s0, s1;
+          f2_split(f2_add(acc[0], acc[1]), s0, s1);
+          l = __fmaf_rn(l, scale_old, s0 + s1);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&ctl->p_ready[buf]);
+      }
+      if (!ok || (any && !(ok = warp_wait(&ctl->pv_done[i], (g - 1) & 1, p.wait_limit, abort_flag)))) break;
+      tc_fence_after();
+      const bool done = w.a0 == 0 && w.a1 == u.tiles;
+      if (!done && w.a0 == 0) {
+        const int total = ctl->start[4];
+        const int unit_start = piece_start(blockIdx.x + 1, total, ctas) - w.a1;
+        cut = make_int4(w.item, w.kv_head, piece_of(unit_start + u.tiles - 1, total, ctas), 0);
+      }
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (w.a0 == 0 ? 1 : 0);
+      const int64_t slot_row = slot * p.rows + i * BM + r;
+      const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // NaN stays
+      uint16_t* out = p.o + ((static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + w.kv_head * p.group + row_head) * D;
+      if (any) {
+#pragma unroll
+        for (int ch = 0; ch < D / 32; ++ch) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(o_addr + ch * 32, o);
+          tc_wait_ld();
+          if (!live) continue;
+          if (done) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t h[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                h[x] = pack2<BF16>(__uint_as_float(o[8 * e + 2 * x]) * inv, __uint_as_float(o[8 * e + 2 * x + 1]) * inv);
+              reinterpret_cast<uint4*>(out + ch * 32)[e] = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              reinterpret_cast<uint4*>(p.part + slot_row * D + ch * 32)[e] =
+                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        if (live && !done) p.part_ml[slot_row] = make_float2(m == -INFINITY ? m : m * c, l);
+      }
+      if (done && !live && in_tile && t < p.tokens)
+#pragma unroll
+        for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(out)[e] = make_uint4(0, 0, 0, 0);
+      tc_fence_before();
+    } while (w.next(p, block_tokens));
+    if (!ok) give_up(ctl, NTL_STATUS_SOFTMAX_WAIT);
+    if (threadIdx.x == 0) p.head[blockIdx.x] = cut;
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::TMEM_COLS);
+}
+
+// Adds up the parts of the unit that CTA blockIdx.x of the attention kernel began and did not end, in
+// CTA order: weights 2^(m_s - max m), o = sum w_s o_s / sum w_s l_s.  One warp per row, 8 rows per
+// block and round.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) cache_attn_join(const AttnParams p, int row_tiles) {
+  pdl_wait();
+  const int4 cut = p.head[blockIdx.x];
+  if (cut.z < 0) return;
+  const int first = blockIdx.x, last = cut.z;
+  const Unit u = unit_of(p, cut.x, row_tiles * p.tile_tokens);
+  const int lane = threadIdx.x & 31;
+  constexpr int E = D / 32;
+  const int rows = min(p.rows, row_tiles * BM);
+  for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < rows; row += gridDim.y * 8) {
+    const int r = row % BM, token = r / p.group;
+    if (token >= p.tile_tokens) continue;
+    const int t = u.t0 + (row / BM) * p.tile_tokens + token;
+    if (t >= p.tokens) continue;
+    uint16_t* out = p.o + ((static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + cut.y * p.group + r % p.group) * D + lane * E;
+    float o[E] = {};
+    float inv = 0.0f;
+    if (t < u.live) {
+      float m = -INFINITY;
+      for (int s = first + lane; s <= last; s += 32)
+        m = fmaxf(m, p.part_ml[(2ll * s + (s == first)) * p.rows + row].x);
+#pragma unroll
+      for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      float l = 0.0f;
+      for (int s = first; s <= last; ++s) {
+        const int64_t at = (2ll * s + (s == first)) * p.rows + row;
+        const float2 ml = p.part_ml[at];
+        const float wgt = ml.x == -INFINITY ? (ml.y == ml.y ? 0.0f : ml.y) : ex2_approx(ml.x - m);
+        l += wgt * ml.y;
+        float v[E];
+        if constexpr (E == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(p.part + at * D + lane * E);
+          v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(p.part + at * D + lane * E);
+          v[0] = x.x, v[1] = x.y;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += wgt * v[e];
+      }
+      inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
+    }
+    uint32_t h[E / 2];
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) h[e] = pack2<BF16>(o[2 * e] * inv, o[2 * e + 1] * inv);
+    if constexpr (E == 4) {
+      *reinterpret_cast<uint2*>(out) = make_uint2(h[0], h[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(out) = h[0];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------ host side
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+// A 4-D tensor of 16-bit values, strides in values (of dimensions 1 to 3), 128-byte swizzle.
+int make_map(CUtensorMap* map, const char* what, const void* base, bool bf16, const int64_t (&dims)[4],
+             const int64_t (&strides)[3], const int64_t (&box)[4]) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return ntl_fail(NTL_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    b[i] = static_cast<cuuint32_t>(box[i]);
+  }
+  // The stride of a dimension of one is never used; any legal one will do.
+  for (int i = 0; i < 3; ++i) s[i] = dims[i + 1] == 1 ? 16 : static_cast<cuuint64_t>(strides[i]) * 2;
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                  const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return ntl_fail(NTL_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, int(r));
+  return NTL_OK;
+}
+
+// What the sizes decide: the shape of CTA, the grid and the workspace.
+struct Plan {
+  int row_tiles, tile_tokens, blocks, tile_keys, tile_pages, rows, ctas;
+  uint64_t part_bytes, bytes;
+};
+
+int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, Plan* plan) {
+  const int64_t group = q->heads / c->kv_heads;
+  Plan& n = *plan;
+  n.row_tiles = q->tokens * group > BM ? 2 : 1;
+  n.tile_tokens = static_cast<int>(BM / group < q->tokens ? BM / group : q->tokens);
+  const int64_t block_tokens = int64_t(n.row_tiles) * n.tile_tokens;
+  const int64_t blocks = (q->tokens + block_tokens - 1) / block_tokens;
+  const int most = n.row_tiles == 1 ? 64 : 128;
+  if (c->page_size <= most) {
+    n.tile_pages = static_cast<int>(most / c->page_size);
+    n.tile_keys = static_cast<int>(n.tile_pages * c->page_size);
+  } else {
+    n.tile_pages = 1;
+    n.tile_keys = 8;  // page_size is a multiple of 8
+    for (int k = most; k > 8; k -= 8)
+      if (c->page_size % k == 0) {
+        n.tile_keys = k;
+        break;
+      }
+  }
+  n.rows = n.row_tiles == 1 ? static_cast<int>(q->tokens * group) : 2 * BM;
+  const int64_t tiles = q->max_pages * c->page_size / n.tile_keys + 2;  // of one unit, at most
+  NTL_REQUIRE(q->seqs * blocks < (int64_t(1) << 31) / c->kv_heads / tiles, NTL_ERR_UNSUPPORTED,
+              "%s: more than 2^31 tiles of keys", what);
+  n.blocks = static_cast<int>(blocks);
+  int sms = 0;
+  if (int rc = ntl_num_sms(&sms)) return rc;
+  const int64_t work = q->seqs * blocks * c->kv_heads * tiles;
+  const int64_t resident = n.row_tiles == 1 ? 2 * sms : sms;
+  n.ctas = static_cast<int>(work < resident ? work : resident);
+  n.part_bytes = static_cast<uint64_t>(2) * n.ctas * n.rows * c->head_dim * 4;
+  n.bytes = n.part_bytes + static_cast<uint64_t>(2) * n.ctas * n.rows * 8 + static_cast<uint64_t>(n.ctas) * 16;
+  n.bytes = (n.bytes + 15) / 16 * 16;
+  return NTL_OK;
+}
+
+template <int D, int NT, bool BF16>
+int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                 const AttnParams& p, const Plan& n, cudaStream_t s) {
+  static std::atomic<uint64_t> done_mask{0};
+  auto kernel = cache_attn_kernel<D, NT, BF16>;
+  constexpr int smem = smem_bytes<D, NT>();
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "cudaGetDevice failed");
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (!(bit && (done_mask.load(std::memory_order_acquire) & bit))) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+    // The register split must equal what the launch allocates, or the raising warps would wait for
+    // registers forever: refuse a build whose register count differs.
+    cudaFuncAttributes fa;
+    if (NT == 2 && (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.numRegs != REGS_LAUNCH))
+      return ntl_fail(NTL_ERR_UNSUPPORTED, "%s: kernel compiled with %d registers, the split needs %d", what,
+                      fa.numRegs, REGS_LAUNCH);
+    done_mask.fetch_or(bit, std::memory_order_release);
+  }
+  kernel<<<n.ctas, Shape<D, NT>::THREADS, smem, s>>>(mq, mk, mv, p);
+  ntl_note_launch();
+  if (int rc = ntl_check_launch(what)) return rc;
+  if (n.ctas == 1) return NTL_OK;  // one piece: no unit is cut
+  const unsigned chunks = static_cast<unsigned>((n.rows + 31) / 32);
+  cudaError_t e = ntl_launch_pdl(cache_attn_join<D, BF16>, dim3(n.ctas - 1, chunks), dim3(256), 0, s, p, NT);
+  if (e != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  ntl_note_launch();
+  return ntl_check_launch(what);
 }
 
 int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const uint32_t* tree, int64_t tree_stride,
-           int64_t window, int64_t sinks, cudaStream_t s) {
+           int64_t window, int64_t sinks, void* workspace, uint64_t workspace_bytes, cudaStream_t s) {
+  Plan n;
+  if (int rc = make_plan(what, c, q, &n)) return rc;
+  NTL_REQUIRE(workspace && workspace_bytes >= n.bytes && ntl_aligned(workspace, 16), NTL_ERR_INVALID,
+              "%s: workspace of %llu bytes, %llu needed (16-byte aligned)", what, (unsigned long long)workspace_bytes,
+              (unsigned long long)n.bytes);
+  const int64_t group = q->heads / c->kv_heads, dim = c->head_dim;
+  const bool bf16 = c->dtype == NTL_BF16;
+  CUtensorMap mq, mk, mv;
+  if (int rc = make_map(&mq, what, q->q, bf16, {dim, q->heads, q->tokens, q->seqs},
+                        {q->head_stride, q->token_stride, q->seq_stride}, {64, group, n.tile_tokens, 1}))
+    return rc;
+  const int64_t dims[4] = {dim, c->kv_heads, c->page_size, c->pages};
+  const int64_t strides[3] = {c->head_stride, c->row_stride, c->page_stride};
+  const int64_t box[4] = {64, 1, n.tile_keys / n.tile_pages, 1};
+  if (int rc = make_map(&mk, what, c->k, bf16, dims, strides, box)) return rc;
+  if (int rc = make_map(&mv, what, c->v, bf16, dims, strides, box)) return rc;
   AttnParams p = {};
-  p.q = static_cast<const uint16_t*>(q->q);
   p.o = static_cast<uint16_t*>(q->o);
-  p.k = static_cast<const uint16_t*>(c->k);
-  p.v = static_cast<const uint16_t*>(c->v);
   p.table = q->table;
   p.lens = q->lens;
   p.q_lens = q->q_lens;
   p.tree = tree;
-  p.tree_stride = tree_stride;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.part = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + n.part_bytes);
+  p.head = reinterpret_cast<int4*>(ws + n.part_bytes + static_cast<uint64_t>(2) * n.ctas * n.rows * 8);
   p.table_stride = q->table_stride;
-  p.q_seq = q->seq_stride;
-  p.q_token = q->token_stride;
-  p.q_head = q->head_stride;
-  p.page_stride = c->page_stride;
-  p.row_stride = c->row_stride;
-  p.head_stride = c->head_stride;
-  p.seqs = q->seqs;
-  p.tokens = q->tokens;
-  p.heads = q->heads;
-  p.kv_heads = c->kv_heads;
-  p.group = q->heads / c->kv_heads;
-  p.pages = c->pages;
-  p.page_size = c->page_size;
-  p.max_pages = q->max_pages;
-  p.words = (q->tokens + 31) / 32;
-  p.window = window;
-  p.sinks = sinks;
-  p.scale_log2 = static_cast<float>(q->scale * 1.4426950408889634);
-  const unsigned grid = (q->seqs * q->tokens * q->heads + 3) / 4;
-  const bool bf = c->dtype == NTL_BF16;
-  if (c->head_dim == 128) {
-    if (bf) cache_attn_simple<128, true><<<grid, 128, 0, s>>>(p);
-    else cache_attn_simple<128, false><<<grid, 128, 0, s>>>(p);
-  } else {
-    if (bf) cache_attn_simple<64, true><<<grid, 128, 0, s>>>(p);
-    else cache_attn_simple<64, false><<<grid, 128, 0, s>>>(p);
+  p.tree_stride = tree_stride;
+  p.seqs = static_cast<int>(q->seqs);
+  p.tokens = static_cast<int>(q->tokens);
+  p.heads = static_cast<int>(q->heads);
+  p.kv_heads = static_cast<int>(c->kv_heads);
+  p.group = static_cast<int>(group);
+  p.pages = static_cast<int>(c->pages);
+  p.page_size = static_cast<int>(c->page_size);
+  p.max_pages = static_cast<int>(q->max_pages);
+  p.words = static_cast<int>((q->tokens + 31) / 32);
+  p.window = static_cast<int>(window);
+  p.sinks = static_cast<int>(sinks);
+  p.tile_tokens = n.tile_tokens;
+  p.blocks = n.blocks;
+  p.tile_keys = n.tile_keys;
+  p.tile_pages = n.tile_pages;
+  p.rows = n.rows;
+  p.min_tiles = 1;
+  p.c = static_cast<float>(q->scale * 1.4426950408889634);
+  p.wait_limit = ntl_wait_limit();
+#define NTL_CACHE_ATTN(D, NT) \
+  return bf16 ? launch_shape<D, NT, true>(what, mq, mk, mv, p, n, s) : launch_shape<D, NT, false>(what, mq, mk, mv, p, n, s)
+  if (dim == 64) {
+    if (n.row_tiles == 1) NTL_CACHE_ATTN(64, 1);
+    NTL_CACHE_ATTN(64, 2);
   }
-  ntl_note_launch();
-  return ntl_check_launch(what);
+  if (n.row_tiles == 1) NTL_CACHE_ATTN(128, 1);
+  NTL_CACHE_ATTN(128, 2);
+#undef NTL_CACHE_ATTN
 }
 
 int check(const char* what, const ntl_cache_t* c, const ntl_query_t* q) {
@@ -147,9 +1006,24 @@ int check(const char* what, const ntl_cache_t* c, const ntl_query_t* q) {
 
 }  // namespace
 
+uint32_t ntl_cache_attn_status_read(int clear) {
+  uint32_t v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_cache_attn_status, sizeof(v)) != cudaSuccess) return 0;
+  if (clear) {
+    uint32_t z = 0;
+    cudaMemcpyToSymbol(g_cache_attn_status, &z, sizeof(z));
+  }
+  return v;
+}
+
 extern "C" int ntl_cache_attention_workspace(const ntl_cache_t* cache, const ntl_query_t* query, uint64_t* bytes_out) {
   if (int rc = check("cache attention", cache, query)) return rc;
+  NTL_REQUIRE(bytes_out, NTL_ERR_INVALID, "cache attention: NULL result");
   *bytes_out = 0;
+  if (query->seqs == 0 || query->tokens == 0 || query->heads == 0) return NTL_OK;
+  Plan n;
+  if (int rc = make_plan("cache attention", cache, query, &n)) return rc;
+  *bytes_out = n.bytes;
   return NTL_OK;
 }
 
@@ -160,7 +1034,8 @@ extern "C" int ntl_tree_attention(const ntl_cache_t* cache, const ntl_query_t* q
   NTL_REQUIRE(tree_stride >= 0, NTL_ERR_INVALID, "tree attention: negative mask stride");
   if (query->seqs == 0 || query->tokens == 0 || query->heads == 0) return NTL_OK;
   NTL_REQUIRE(tree, NTL_ERR_INVALID, "tree attention: NULL mask");
-  return launch("tree attention", cache, query, tree, tree_stride, 0, 0, static_cast<cudaStream_t>(stream));
+  return launch("tree attention", cache, query, tree, tree_stride, 0, 0, workspace, workspace_bytes,
+                static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ntl_window_attention(const ntl_cache_t* cache, const ntl_query_t* query, int64_t window, int64_t sinks,
@@ -171,5 +1046,5 @@ extern "C" int ntl_window_attention(const ntl_cache_t* cache, const ntl_query_t*
   if (query->seqs == 0 || query->tokens == 0 || query->heads == 0) return NTL_OK;
   const int64_t most = int64_t(1) << 30;
   return launch("window attention", cache, query, nullptr, 0, window < most ? window : most, sinks < most ? sinks : most,
-                static_cast<cudaStream_t>(stream));
+                workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }

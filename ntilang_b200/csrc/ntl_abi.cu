@@ -72,6 +72,7 @@ int ntl_device_status(uint32_t* status_out) {
   if (status_out == nullptr) return ntl_fail(NTL_ERR_INVALID, "status_out is NULL");
   uint32_t s = ntl_gemm_status_read(0);
   if (s == 0) s = ntl_fa2_status_read(0);
+  if (s == 0) s = ntl_cache_attn_status_read(0);
   *status_out = s;
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "reading device status: %s", cudaGetErrorString(err));
@@ -81,6 +82,7 @@ int ntl_device_status(uint32_t* status_out) {
 int ntl_clear_device_status(void) {
   ntl_gemm_status_read(1);
   ntl_fa2_status_read(1);
+  ntl_cache_attn_status_read(1);
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "clearing device status: %s", cudaGetErrorString(err));
   return NTL_OK;

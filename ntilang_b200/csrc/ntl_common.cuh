@@ -43,6 +43,7 @@ enum : uint32_t {
 // Per-translation-unit status readers (each .cu with bounded waits defines one pair).
 uint32_t ntl_gemm_status_read(int clear);
 uint32_t ntl_fa2_status_read(int clear);
+uint32_t ntl_cache_attn_status_read(int clear);
 
 // ----------------------------------------------------------------------------- device
 

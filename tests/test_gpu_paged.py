@@ -131,6 +131,61 @@ def test_tree_shapes(torch_cuda, dtype, dim, heads, kv_heads, page, tokens):
     assert not out[0, ::3].any()
 
 
+# Several units, whole and cut, run back to back on one CTA: more units than CTAs, units of one key
+# tile and of many, lengths that end inside pages.
+@pytest.mark.parametrize("dtype,dim,seqs,kv_heads,group,tokens,longest", [
+    ("float16", 128, 4, 296, 1, 1, 128), ("bfloat16", 64, 3, 592, 1, 2, 640), ("float16", 64, 40, 30, 4, 8, 700),
+    ("bfloat16", 128, 70, 9, 3, 5, 900), ("float16", 128, 60, 6, 4, 40, 500), ("bfloat16", 64, 33, 8, 2, 100, 700),
+    ("float16", 64, 300, 3, 8, 30, 130),
+])
+@pytest.mark.parametrize("kind", ["tree", "window"])
+def test_many_units(torch_cuda, kind, dtype, dim, seqs, kv_heads, group, tokens, longest):
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    rng = np.random.default_rng(seqs)
+    lens = rng.integers(tokens, longest + 1, seqs)
+    lens[0] = longest
+    q, k, v, table, n = make(torch, dtype=dtype, dim=dim, heads=kv_heads * group, kv_heads=kv_heads, lens=lens,
+                             tokens=tokens, seed=seqs)
+    bits = np.tril(rng.random((1, tokens, tokens)) < 0.5)
+    for again in range(3):
+        if kind == "tree":
+            out = paged.tree_attention(q, k, v, table, n, pack(torch, bits))
+            masks = [tree_mask_of(bits[0], x, tokens) for x in lens.tolist()]
+        else:
+            out = paged.window_attention(q, k, v, table, n, 200, 10)
+            masks = [window_mask(x, tokens, 200, 10) for x in lens.tolist()]
+        if again == 0:
+            check(torch, out, q, k, v, table, n, masks)
+            first = out
+        assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("tokens", [1, 60])
+def test_a_wait_that_gives_up_is_reported(torch_cuda, tokens):
+    """With a limit of one poll the kernel's waits give up: it returns, says so, and the next call is right."""
+    from ntilang_b200 import _lib, paged
+
+    torch = torch_cuda
+    lens = [3000, 2000, 900]
+    q, k, v, table, n = make(torch, lens=lens, tokens=tokens, seed=2)
+    want = paged.window_attention(q, k, v, table, n, 1 << 20)
+    torch.cuda.synchronize()
+    _lib.clear_device_status()
+    _lib.set_wait_limit(1)
+    try:
+        paged.window_attention(q, k, v, table, n, 1 << 20)
+        torch.cuda.synchronize()
+        assert _lib.device_status() != 0
+    finally:
+        _lib.set_wait_limit(1 << 26)
+        _lib.clear_device_status()
+    assert _lib.device_status() == 0
+    assert torch.equal(paged.window_attention(q, k, v, table, n, 1 << 20), want)
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("tokens", [1, 5, 64, 200])
 def test_tree_of_parents(torch_cuda, tokens):
     """tree_mask, one tree shared by every sequence, and a chain's equality with causal attention."""
