@@ -23,13 +23,14 @@
 //   NT = 2: two 128-row tiles that share every K and V tile, 128-key tiles, one CTA per SM.  For wide
 //           trees and prompt chunks, bound by the tensor cores and the exponentials.
 // Warps: 4 per row tile for the softmax (one thread per row = TMEM lane; the same thread rescales
-// and writes out the row), then one each for MMA issue, K/V loads, Q loads, and clearing value rows past
-// the sequence's end (a page's unwritten rows may hold NaN, and 0 * NaN is not 0).
+// and writes out the row), then one each for MMA issue, K loads, V loads, and for Q loads and clearing value
+// rows past the sequence's end (a page's unwritten rows may hold NaN, and 0 * NaN is not 0).
 // Every wait is bounded: one that gives up records a status code, and the CTA drains its copies
 // and MMAs, frees TMEM and returns.
 #include <atomic>
 #include <cuda_bf16.h>
 #include <mutex>
+#include <type_traits>
 
 #include "ntl_common.cuh"
 
@@ -38,6 +39,7 @@ namespace {
 __device__ uint32_t g_cache_attn_status;
 
 constexpr int BM = 128;                // rows per tile
+constexpr int kOutRow = 80;            // bytes from one staged output row to the next: 64 and a gap against bank conflicts
 constexpr float kRescaleLog2 = 8.0f;   // o is rescaled when the maximum rose by more than 2^8
 
 struct AttnParams {
@@ -55,6 +57,7 @@ struct AttnParams {
   int blocks;        // token blocks per sequence (units of NT tiles)
   int tile_keys;     // keys per tile: whole pages, or a divisor of a page
   int tile_pages;    // pages per tile (1 where a page holds several tiles)
+  int tile_shift;    // log2 of tile_keys, -1 if it is no power of two
   int rows;          // rows a workspace slot has
   int min_tiles;     // least tiles per CTA
   float c;           // softmax scale in log2 units
@@ -66,14 +69,15 @@ struct Shape {
   static constexpr int BN = NT == 1 ? 64 : 128;  // keys per tile
   static constexpr int STAGES = D == 64 ? 4 : 2;  // of K and of V
   static constexpr int SOFTMAX_WARPS = 4 * NT;
-  static constexpr int MMA_WARP = SOFTMAX_WARPS, KV_WARP = MMA_WARP + 1, Q_WARP = MMA_WARP + 2, FIX_WARP = MMA_WARP + 3;
+  static constexpr int MMA_WARP = SOFTMAX_WARPS, K_WARP = MMA_WARP + 1, V_WARP = MMA_WARP + 2, AUX_WARP = MMA_WARP + 3;
   static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);
   static constexpr int CTAS_PER_SM = NT == 1 ? 2 : 1;
   static constexpr int Q_BYTES = BM * D * 2;
   static constexpr int KV_BYTES = BN * D * 2;
   static constexpr int K_OFF = NT * Q_BYTES;
   static constexpr int V_OFF = K_OFF + STAGES * KV_BYTES;
-  static constexpr int CTL_OFF = V_OFF + STAGES * KV_BYTES;
+  static constexpr int OUT_OFF = V_OFF + STAGES * KV_BYTES;  // staging of the outputs, kOutRow * 32 bytes a warp
+  static constexpr int CTL_OFF = OUT_OFF + SOFTMAX_WARPS * 32 * kOutRow;
   static constexpr uint32_t TMEM_COLS = NT == 1 ? 256 : 512;
   // S buffer i (NT = 1: of every other key tile; NT = 2: of row tile i), O of row tile i.
   __host__ __device__ static constexpr uint32_t S_COL(int i) { return static_cast<uint32_t>(i * BN); }
@@ -110,9 +114,26 @@ __device__ __forceinline__ void give_up(Ctl* ctl, uint32_t code) {
   *reinterpret_cast<volatile int*>(&ctl->abort) = 1;
 }
 
+// mbar_wait_bounded with the clock read only once the wait is long (reading it first costs more than
+// most of the waits here take).
+__device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, int64_t limit, volatile int* abort_flag) {
+  if (mbar_test_wait(bar, parity)) return true;
+  uint64_t t0 = 0;
+  for (int64_t i = 1; i < limit; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63) == 63) {
+      if (abort_flag != nullptr && *abort_flag) return false;
+      const uint64_t now = global_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kWaitCapNs) return false;
+    }
+  }
+  return false;
+}
+
 // A wait of a whole warp, which gives up as one: no lane goes on without the others.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int64_t limit, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, limit, abort_flag));
+  return __all_sync(0xffffffffu, wait_bounded(bar, parity, limit, abort_flag));
 }
 
 // ------------------------------------------------------------------------------ units
@@ -123,24 +144,27 @@ struct Unit {
   int tiles, sink_tiles, first;  // key tiles; those of the sinks; the window's first
 };
 
+__device__ __forceinline__ int tile_index(const AttnParams& p, int key) {
+  return p.tile_shift >= 0 ? key >> p.tile_shift : key / p.tile_keys;
+}
+
 __device__ __forceinline__ Unit unit_of(const AttnParams& p, int item, int block_tokens) {
   Unit u;
-  u.b = item / p.blocks;
+  u.b = p.blocks == 1 ? item : item / p.blocks;
   u.t0 = (item - u.b * p.blocks) * block_tokens;
-  const int64_t room = static_cast<int64_t>(p.max_pages) * p.page_size;
-  u.len = static_cast<int>(min(static_cast<int64_t>(max(p.lens[u.b], 0)), room));
+  u.len = min(max(p.lens[u.b], 0), p.max_pages * p.page_size);
   u.live = min(u.len, p.q_lens ? min(max(p.q_lens[u.b], 0), p.tokens) : p.tokens);
   u.tiles = 1;  // a unit without keys has one tile that nothing sees, and writes zeros
   u.sink_tiles = u.first = 0;
   if (u.t0 >= u.live) return u;
   if (p.tree) {
-    u.tiles = max(1, (u.len + p.tile_keys - 1) / p.tile_keys);
+    u.tiles = max(1, tile_index(p, u.len + p.tile_keys - 1));
   } else {
     const int prefix = u.len - u.live;
     const int last = prefix + min(u.t0 + block_tokens, u.live) - 1;
-    u.first = max(0, prefix + u.t0 - p.window + 1) / p.tile_keys;
-    u.sink_tiles = min(u.first, static_cast<int>((static_cast<int64_t>(p.sinks) + p.tile_keys - 1) / p.tile_keys));
-    u.tiles = u.sink_tiles + last / p.tile_keys - u.first + 1;
+    u.first = tile_index(p, max(0, prefix + u.t0 - p.window + 1));
+    u.sink_tiles = min(u.first, tile_index(p, p.sinks + p.tile_keys - 1));
+    u.tiles = u.sink_tiles + tile_index(p, last) - u.first + 1;
   }
   return u;
 }
@@ -155,8 +179,9 @@ __device__ __forceinline__ bool past_end(const AttnParams& p, const Unit& u, int
 }
 
 // The pieces: `total` tiles over `ctas` CTAs, CTA i from piece_start(i).
-__device__ __forceinline__ int piece_start(int i, int total, int ctas) {
-  return static_cast<int>(static_cast<int64_t>(i) * total / ctas);
+__device__ __forceinline__ int piece_start(int i, int total, int ctas) {  // floor(i * total / ctas)
+  const int each = total / ctas;
+  return i * each + i * (total - each * ctas) / ctas;
 }
 __device__ __forceinline__ int piece_of(int tile, int total, int ctas) {
   return static_cast<int>(((static_cast<int64_t>(tile) + 1) * ctas - 1) / total);
@@ -319,12 +344,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
   const int block_tokens = NT * p.tile_tokens;
 
   pdl_trigger();
-  const int ctas = find_piece(p, ctl, block_tokens);
-  if (static_cast<int>(blockIdx.x) >= ctas) {
-    if (threadIdx.x == 0) p.head[blockIdx.x] = make_int4(0, 0, -1, 0);
-    return;
-  }
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 3) prefetch_tensormap(threadIdx.x == 0 ? &tq : threadIdx.x == 1 ? &tk : &tv);
+  if (warp == C::MMA_WARP) {
+    tmem_alloc(&ctl->tmem_base, C::TMEM_COLS);
+    tmem_relinquish();
+  } else if (threadIdx.x == 0) {
     mbar_init(&ctl->q_full, 1);
     mbar_init(&ctl->q_empty, 1);
     for (int s = 0; s < ST; ++s) {
@@ -353,33 +377,37 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
     }
     fence_proxy_async_smem();
   }
-  if (warp == C::MMA_WARP) {
-    tmem_alloc(&ctl->tmem_base, C::TMEM_COLS);
-    tmem_relinquish();
-  }
+  const int ctas = find_piece(p, ctl, block_tokens);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (static_cast<int>(blockIdx.x) >= ctas) {
+    if (threadIdx.x == 0) p.head[blockIdx.x] = make_int4(0, 0, -1, 0);
+    if (warp == C::MMA_WARP) tmem_dealloc(ctl->tmem_base, C::TMEM_COLS);
+    return;
+  }
   const uint32_t tmem = ctl->tmem_base;
   Walk w;
   w.begin(p, ctl, block_tokens);
 
   if (warp >= C::SOFTMAX_WARPS) {
     if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS_OTHER) : "memory");
-    if (warp == C::KV_WARP) {
-      // ---------------------------------------------- K and V loads, one lane per page of the tile
+    if (warp == C::K_WARP || warp == C::V_WARP) {
+      // ---------------------------------------------- K loads, V loads: one warp each, a lane per page
+      // K frees its stages a softmax earlier than V does; one warp for both would hold K back.
       // Lane 0 waits for the whole warp, so that either every lane issues its boxes or none does.
-      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        const bool ok = lane != 0 || mbar_wait_bounded(bar, parity, p.wait_limit, abort_flag);
-        return __shfl_sync(0xffffffffu, ok, 0);
-      };
+      const bool is_v = warp == C::V_WARP;
+      uint64_t* full = is_v ? ctl->v_full : ctl->k_full;
+      uint64_t* empty = is_v ? ctl->v_empty : ctl->k_empty;
+      const CUtensorMap* map = is_v ? &tv : &tk;
+      uint8_t* stages = smem + (is_v ? C::V_OFF : C::K_OFF);
       const int boxes = p.tile_pages;
       const int box_keys = p.tile_keys / boxes;
       const int box_bytes = box_keys * 128;  // one page's rows of one 64-column half
       const uint32_t tile_bytes = static_cast<uint32_t>(boxes * box_bytes * (D / 64));
       bool ok = true;
-      int k_issued = 0, v_issued = 0;
-      uint32_t raw = 0, cleared = 0;  // bit s: parity of the next v_raw[s]; stage s's last V tile is one to clear
+      int issued = 0;
+      uint32_t raw = 0, cleared = 0;  // bit s: parity of the next v_raw[s]; stage s's last tile is one to clear
       do {
         const int lo = p.tree ? 0 : max(0, w.u.len - w.u.live + w.u.t0 - p.window + 1);  // the window's first key
         const int32_t* row = p.table + w.u.b * p.table_stride;
@@ -393,89 +421,70 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
         };
         int next_page = page_at(w.a0);
         for (int a = w.a0; a < w.a1; ++a) {
-          const int s = k_issued % ST;
-          const uint32_t parity = ((k_issued / ST) & 1) ^ 1;
+          const int s = issued % ST;
           const int y = boxes > 1 ? 0 : tile_key(p, w.u, a) % p.page_size;
           const int page = next_page;
           if (a + 1 < w.a1) next_page = page_at(a + 1);
-          if (!(ok = wait(&ctl->k_empty[s], parity))) break;
-          if (lane == 0) mbar_arrive_expect_tx(&ctl->k_full[s], tile_bytes);
-          __syncwarp();
-          uint8_t* to = smem + C::K_OFF + s * C::KV_BYTES + lane * box_bytes;
-          if (lane < boxes) {
-#pragma unroll
-            for (int d = 0; d < D / 64; ++d)
-              tma_load_4d(to + d * (BN * 128), &tk, &ctl->k_full[s], d * 64, w.kv_head, y, page);
-          }
-          ++k_issued;
-          if (!(ok = wait(&ctl->v_empty[s], parity))) break;
-          const bool clear = past_end(p, w.u, a);
-          uint64_t* landed = clear ? &ctl->v_raw[s] : &ctl->v_full[s];
+          ok = lane != 0 || wait_bounded(&empty[s], ((issued / ST) & 1) ^ 1, p.wait_limit, abort_flag);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) break;
+          const bool clear = is_v && past_end(p, w.u, a);
+          uint64_t* landed = clear ? &ctl->v_raw[s] : &full[s];
           if (clear) raw ^= 1u << s;
           cleared = clear ? cleared | 1u << s : cleared & ~(1u << s);
           if (lane == 0) mbar_arrive_expect_tx(landed, tile_bytes);
           __syncwarp();
-          to += C::V_OFF - C::K_OFF;
+          uint8_t* to = stages + s * C::KV_BYTES + lane * box_bytes;
           if (lane < boxes) {
 #pragma unroll
-            for (int d = 0; d < D / 64; ++d)
-              tma_load_4d(to + d * (BN * 128), &tv, landed, d * 64, w.kv_head, y, page);
+            for (int d = 0; d < D / 64; ++d) tma_load_4d(to + d * (BN * 128), map, landed, d * 64, w.kv_head, y, page);
           }
-          ++v_issued;
+          ++issued;
         }
       } while (ok && w.next(p, block_tokens));
       if (!ok && lane == 0) {
         give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
         // Drain every copy this warp issued before the CTA exits.
-        for (int j = max(0, k_issued - ST); j < k_issued; ++j)
-          if (!mbar_wait_bounded(&ctl->k_full[j % ST], (j / ST) & 1, int64_t(1) << 24, nullptr))
-            atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
-        for (int j = max(0, v_issued - ST); j < v_issued; ++j) {
+        for (int j = max(0, issued - ST); j < issued; ++j) {
           const int s = j % ST;
           const bool clear = cleared >> s & 1;
-          if (!mbar_wait_bounded(clear ? &ctl->v_raw[s] : &ctl->v_full[s], clear ? ~raw >> s & 1 : (j / ST) & 1,
+          if (!wait_bounded(clear ? &ctl->v_raw[s] : &full[s], clear ? ~raw >> s & 1 : (j / ST) & 1,
                                  int64_t(1) << 24, nullptr))
             atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
         }
       }
-    } else if (warp == C::Q_WARP) {
-      // ---------------------------------------------- Q loads: the next unit's, once the last Q K^T retired
-      if (lane == 0) {
-        const uint32_t bytes = static_cast<uint32_t>(NT * (D / 64) * p.tile_tokens * p.group * 128);
-        bool ok = true;
-        int n = 0;
-        do {
-          if (n > 0 && !(ok = mbar_wait_bounded(&ctl->q_empty, (n - 1) & 1, p.wait_limit, abort_flag))) break;
-          mbar_arrive_expect_tx(&ctl->q_full, bytes);
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int d = 0; d < D / 64; ++d)
-              tma_load_4d(smem + i * C::Q_BYTES + d * (BM * 128), &tq, &ctl->q_full, d * 64, w.kv_head * p.group,
-                          w.u.t0 + i * p.tile_tokens, w.u.b);
-          ++n;
-        } while (w.next(p, block_tokens));
-        if (!ok) give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
-        // The MMA thread waits for each load; if it gave up, this thread does before the CTA exits.
-        if (!mbar_wait_bounded(&ctl->q_full, (n - 1) & 1, int64_t(1) << 24, nullptr))
-          atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
-      }
-    } else if (warp == C::FIX_WARP) {
-      // ---------------------------------------------- value rows past the sequence's end become zeros
+    } else if (warp == C::AUX_WARP) {
+      // ---------------------------------------------- Q loads, and value rows past the end become zeros
+      const uint32_t q_bytes = static_cast<uint32_t>(NT * (D / 64) * p.tile_tokens * p.group * 128);
       bool ok = true;
-      int g = 0;
+      int n = 0, g = 0;
       uint32_t raw = 0;  // bit s: parity of v_raw[s]
       do {
+        // The next unit's Q once the last Q K^T of the unit before retired.
+        if (lane == 0) {
+          ok = n == 0 || wait_bounded(&ctl->q_empty, (n - 1) & 1, p.wait_limit, abort_flag);
+          if (ok) {
+            mbar_arrive_expect_tx(&ctl->q_full, q_bytes);
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+              for (int d = 0; d < D / 64; ++d)
+                tma_load_4d(smem + i * C::Q_BYTES + d * (BM * 128), &tq, &ctl->q_full, d * 64, w.kv_head * p.group,
+                            w.u.t0 + i * p.tile_tokens, w.u.b);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        ++n;
         for (int a = w.a0; a < w.a1 && ok; ++a, ++g) {
           if (!past_end(p, w.u, a)) continue;
           const int s = g % ST;
-          if (lane == 0) ok = mbar_wait_bounded(&ctl->v_raw[s], raw >> s & 1, p.wait_limit, abort_flag);
+          if (lane == 0) ok = wait_bounded(&ctl->v_raw[s], raw >> s & 1, p.wait_limit, abort_flag);
           ok = __shfl_sync(0xffffffffu, ok, 0);
           if (!ok) break;
           raw ^= 1u << s;
-          const int rows = w.u.len - tile_key(p, w.u, a);  // rows that hold tokens
-          const int first = max(rows, 0);
-          const int units = (p.tile_keys - first) * 8;  // 16-byte units per half
+          const int first = max(w.u.len - tile_key(p, w.u, a), 0);  // rows that hold tokens
+          const int units = (p.tile_keys - first) * 8;              // 16-byte units per half
           for (int e = lane; e < (D / 64) * units; e += 32) {
             const int half = e / units, at = e - half * units;
             *reinterpret_cast<uint4*>(smem + C::V_OFF + s * C::KV_BYTES + half * (BN * 128) + first * 128 + at * 16) =
@@ -486,14 +495,19 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           if (lane == 0) mbar_arrive(&ctl->v_full[s]);
         }
       } while (ok && w.next(p, block_tokens));
-      if (!ok && lane == 0) give_up(ctl, NTL_STATUS_SOFTMAX_WAIT);
+      if (lane == 0) {
+        if (!ok) give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
+        // The MMA thread waits for each Q load; if it gave up, this thread does before the CTA exits.
+        if (n > 0 && !wait_bounded(&ctl->q_full, (n - 1) & 1, int64_t(1) << 24, nullptr))
+          atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
+      }
     } else if (elect_one_lane()) {
       // ---------------------------------------------- MMA issue
       constexpr uint32_t idesc_s = idesc<BF16>(BN, 0);  // B = K tile, K-major
       constexpr uint32_t idesc_o = idesc<BF16>(D, 1);   // B = V tile, N-major
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        if (mbar_wait_bounded(bar, parity, p.wait_limit, abort_flag)) return true;
+        if (wait_bounded(bar, parity, p.wait_limit, abort_flag)) return true;
         give_up(ctl, NTL_STATUS_MMA_FULL_WAIT);
         return false;
       };
@@ -551,12 +565,22 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
             return true;
           };
           if constexpr (NT == 1) {
-            if (more) {
+            // The next tile's Q K^T goes first, to run during the softmax; a new unit's waits for loads
+            // that the end of this unit must not wait for, and goes second.
+            const bool ahead = more, other = aq == wq.a0;
+            if (ahead && !other) {
               if (!(ok = qk_ready())) break;
               qk(0);
               qk_end();
             }
             if (!(ok = wait(&ctl->v_full[s], (g / ST) & 1) && pv(0))) break;
+            if (ahead && other) {
+              tc_commit(&ctl->v_empty[s]);
+              if (!(ok = qk_ready())) break;
+              qk(0);
+              qk_end();
+              continue;
+            }
           } else {
             if (!(ok = wait(&ctl->v_full[s], (g / ST) & 1) && pv(0))) break;
             const bool ahead = more;
@@ -576,7 +600,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       }
       if (!ok) {
         tc_commit(&ctl->drain);
-        if (!mbar_wait_bounded(&ctl->drain, 0, int64_t(1) << 24, nullptr))
+        if (!wait_bounded(&ctl->drain, 0, int64_t(1) << 24, nullptr))
           atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
       }
     }
@@ -599,6 +623,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       const int t = u.t0 + t_in_block;
       const bool live = in_tile && t < u.live;
       const bool any = __any_sync(0xffffffffu, live);
+      const bool here = in_tile && t < p.tokens;  // the output has this row
+      const int64_t out_row =
+          (static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + w.kv_head * p.group + row_head;
       // Keys that every row of this row tile sees: [0, all_hi), or for the window [all_lo, all_hi)
       // and the sinks.
       const int prefix = u.len - u.live;
@@ -644,7 +671,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           bool moved = false;
           if (m == -INFINITY) {
             m = top;  // nothing seen so far: o and l are zero (or not begun)
-          } else if ((top - m) * c > kRescaleLog2) {
+          } else if (live && (top - m) * c > kRescaleLog2) {
             scale_old = ex2_approx((m - top) * c);
             m = top;
             moved = true;
@@ -698,43 +725,64 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       if (!ok || (any && !(ok = warp_wait(&ctl->pv_done[i], (g - 1) & 1, p.wait_limit, abort_flag)))) break;
       tc_fence_after();
       const bool done = w.a0 == 0 && w.a1 == u.tiles;
-      if (!done && w.a0 == 0) {
+      if (!done && w.a0 == 0 && threadIdx.x == 0) {
         const int total = ctl->start[4];
         const int unit_start = piece_start(blockIdx.x + 1, total, ctas) - w.a1;
         cut = make_int4(w.item, w.kv_head, piece_of(unit_start + u.tiles - 1, total, ctas), 0);
       }
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (w.a0 == 0 ? 1 : 0);
-      const int64_t slot_row = slot * p.rows + i * BM + r;
-      const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // NaN stays
-      uint16_t* out = p.o + ((static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + w.kv_head * p.group + row_head) * D;
       if (any) {
+        // Rows leave through shared memory, 64 bytes of each at a time, so that a store instruction
+        // writes whole sectors: quad n of a warp writes 64 bytes of row 8 i + n (a thread writing its own
+        // row 16 bytes at a time took 5 to 9 us per 108 rows).
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (w.a0 == 0 ? 1 : 0);
+        const int64_t slot_row = slot * p.rows + i * BM + (warp & 3) * 32;  // of the warp's first row
+        const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // NaN stays
+        uint8_t* stage = smem + C::OUT_OFF + warp * 32 * kOutRow;
+        // Where this thread's quad writes: row 8 e + lane / 4 of the warp, or nowhere.
+        uint8_t* to[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = 8 * e + (lane >> 2);
+          const int64_t at = __shfl_sync(0xffffffffu, out_row, row);
+          const bool row_live = __shfl_sync(0xffffffffu, static_cast<int>(live), row);
+          const bool row_here = __shfl_sync(0xffffffffu, static_cast<int>(here), row);
+          to[e] = done ? (row_here ? reinterpret_cast<uint8_t*>(p.o + at * D) : nullptr)
+                       : (row_live ? reinterpret_cast<uint8_t*>(p.part + (slot_row + row) * D) : nullptr);
+          if (to[e]) to[e] += (lane & 3) * 16;
+        }
 #pragma unroll
         for (int ch = 0; ch < D / 32; ++ch) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(o_addr + ch * 32, o);
           tc_wait_ld();
-          if (!live) continue;
           if (done) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t h[4];
+            for (int e = 0; e < 16; ++e)
+              o[e] = live ? pack2<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv) : 0u;
+          }
 #pragma unroll
-              for (int x = 0; x < 4; ++x)
-                h[x] = pack2<BF16>(__uint_as_float(o[8 * e + 2 * x]) * inv, __uint_as_float(o[8 * e + 2 * x + 1]) * inv);
-              reinterpret_cast<uint4*>(out + ch * 32)[e] = make_uint4(h[0], h[1], h[2], h[3]);
-            }
-          } else {
+          for (int half = 0; half < 2; ++half) {  // 16-bit: one half of 64 bytes; fp32: two
+            if (half == 1 && done) break;
+            __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              reinterpret_cast<uint4*>(p.part + slot_row * D + ch * 32)[e] =
-                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(stage + lane * kOutRow + e * 16) =
+                  make_uint4(o[half * 16 + 4 * e], o[half * 16 + 4 * e + 1], o[half * 16 + 4 * e + 2], o[half * 16 + 4 * e + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (to[e]) {
+                *reinterpret_cast<uint4*>(to[e]) =
+                    *reinterpret_cast<const uint4*>(stage + (8 * e + (lane >> 2)) * kOutRow + (lane & 3) * 16);
+                to[e] += 64;
+              }
           }
         }
-        if (live && !done) p.part_ml[slot_row] = make_float2(m == -INFINITY ? m : m * c, l);
-      }
-      if (done && !live && in_tile && t < p.tokens)
+        if (live && !done) p.part_ml[slot_row + lane] = make_float2(m == -INFINITY ? m : m * c, l);
+      } else if (done && here) {
 #pragma unroll
-        for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(out)[e] = make_uint4(0, 0, 0, 0);
+        for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(p.o + out_row * D)[e] = make_uint4(0, 0, 0, 0);
+      }
       tc_fence_before();
     } while (w.next(p, block_tokens));
     if (!ok) give_up(ctl, NTL_STATUS_SOFTMAX_WAIT);
@@ -748,59 +796,71 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
 }
 
 // Adds up the parts of the unit that CTA blockIdx.x of the attention kernel began and did not end, in
-// CTA order: weights 2^(m_s - max m), o = sum w_s o_s / sum w_s l_s.  One warp per row, 8 rows per
-// block and round.
+// CTA order: weights 2^(m_s - max m), o = sum w_s o_s / sum w_s l_s.  One warp per row; the lanes
+// hold 32 parts' (m, l) at a time and the parts' values are read kJoinUnroll at a time, so a row costs
+// a few memory latencies and not one per part (one part after another: 10 to 24 us per call for 16 to 37
+// parts, against 4 to 7 us).
+constexpr int kJoinWarps = 4, kJoinUnroll = 8;
+
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) cache_attn_join(const AttnParams p, int row_tiles) {
+__global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const AttnParams p, int row_tiles) {
   pdl_wait();
   const int4 cut = p.head[blockIdx.x];
   if (cut.z < 0) return;
   const int first = blockIdx.x, last = cut.z;
+  const int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int r = row % BM, token = r / p.group;
+  if (row >= p.rows || token >= p.tile_tokens) return;
   const Unit u = unit_of(p, cut.x, row_tiles * p.tile_tokens);
-  const int lane = threadIdx.x & 31;
+  const int t = u.t0 + (row / BM) * p.tile_tokens + token;
+  if (t >= p.tokens) return;
   constexpr int E = D / 32;
-  const int rows = min(p.rows, row_tiles * BM);
-  for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < rows; row += gridDim.y * 8) {
-    const int r = row % BM, token = r / p.group;
-    if (token >= p.tile_tokens) continue;
-    const int t = u.t0 + (row / BM) * p.tile_tokens + token;
-    if (t >= p.tokens) continue;
-    uint16_t* out = p.o + ((static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + cut.y * p.group + r % p.group) * D + lane * E;
-    float o[E] = {};
-    float inv = 0.0f;
-    if (t < u.live) {
-      float m = -INFINITY;
-      for (int s = first + lane; s <= last; s += 32)
-        m = fmaxf(m, p.part_ml[(2ll * s + (s == first)) * p.rows + row].x);
+  using Vec = typename std::conditional<E == 4, float4, float2>::type;
+  // Part s of the unit: CTA first's second slot, then the first slots of those after it.
+  auto at = [&](int s) { return (2ll * s + (s == first)) * p.rows + row; };
+  float o[E] = {}, m = -INFINITY, l = 0.0f;
+  if (t < u.live) {
+    for (int s0 = first; s0 <= last; s0 += 32) {
+      const float2 ml = s0 + lane <= last ? p.part_ml[at(s0 + lane)] : make_float2(-INFINITY, 0.0f);
+      float top = fmaxf(m, ml.x);
 #pragma unroll
-      for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      float l = 0.0f;
-      for (int s = first; s <= last; ++s) {
-        const int64_t at = (2ll * s + (s == first)) * p.rows + row;
-        const float2 ml = p.part_ml[at];
-        const float wgt = ml.x == -INFINITY ? (ml.y == ml.y ? 0.0f : ml.y) : ex2_approx(ml.x - m);
-        l += wgt * ml.y;
-        float v[E];
-        if constexpr (E == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(p.part + at * D + lane * E);
-          v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-        } else {
-          const float2 x = *reinterpret_cast<const float2*>(p.part + at * D + lane * E);
-          v[0] = x.x, v[1] = x.y;
+      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float old = m == -INFINITY ? 0.0f : ex2_approx(m - top);
+      // A part that saw nothing has m = -inf and l = 0 (or NaN scores: l NaN).
+      const float weight = ml.x == -INFINITY ? (ml.y == ml.y ? 0.0f : ml.y) : ex2_approx(ml.x - top);
+      float sum = weight * ml.y;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      l = l * old + sum;
+      m = top;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= old;
+      const int n = min(32, last - s0 + 1);
+      for (int j0 = 0; j0 < n; j0 += kJoinUnroll) {
+        float v[kJoinUnroll][E];
+#pragma unroll
+        for (int j = 0; j < kJoinUnroll; ++j)
+          if (j0 + j < n)
+            *reinterpret_cast<Vec*>(v[j]) = *reinterpret_cast<const Vec*>(p.part + at(s0 + j0 + j) * D + lane * E);
+#pragma unroll
+        for (int j = 0; j < kJoinUnroll; ++j) {
+          const float wgt = __shfl_sync(0xffffffffu, weight, (j0 + j) & 31);
+          if (j0 + j < n)
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += wgt * v[j][e];
         }
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += wgt * v[e];
       }
-      inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
     }
-    uint32_t h[E / 2];
+  }
+  const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
+  uint32_t h[E / 2];
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) h[e] = pack2<BF16>(o[2 * e] * inv, o[2 * e + 1] * inv);
-    if constexpr (E == 4) {
-      *reinterpret_cast<uint2*>(out) = make_uint2(h[0], h[1]);
-    } else {
-      *reinterpret_cast<uint32_t*>(out) = h[0];
-    }
+  for (int e = 0; e < E / 2; ++e) h[e] = pack2<BF16>(o[2 * e] * inv, o[2 * e + 1] * inv);
+  uint16_t* out = p.o + ((static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + cut.y * p.group + r % p.group) * D + lane * E;
+  if constexpr (E == 4) {
+    *reinterpret_cast<uint2*>(out) = make_uint2(h[0], h[1]);
+  } else {
+    *reinterpret_cast<uint32_t*>(out) = h[0];
   }
 }
 
@@ -909,8 +969,9 @@ int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk,
   ntl_note_launch();
   if (int rc = ntl_check_launch(what)) return rc;
   if (n.ctas == 1) return NTL_OK;  // one piece: no unit is cut
-  const unsigned chunks = static_cast<unsigned>((n.rows + 31) / 32);
-  cudaError_t e = ntl_launch_pdl(cache_attn_join<D, BF16>, dim3(n.ctas - 1, chunks), dim3(256), 0, s, p, NT);
+  const unsigned chunks = static_cast<unsigned>((n.rows + kJoinWarps - 1) / kJoinWarps);
+  cudaError_t e =
+      ntl_launch_pdl(cache_attn_join<D, BF16>, dim3(n.ctas - 1, chunks), dim3(kJoinWarps * 32), 0, s, p, NT);
   if (e != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   ntl_note_launch();
   return ntl_check_launch(what);
@@ -961,6 +1022,9 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   p.blocks = n.blocks;
   p.tile_keys = n.tile_keys;
   p.tile_pages = n.tile_pages;
+  p.tile_shift = -1;
+  for (int i = 3; i < 8; ++i)
+    if (n.tile_keys == 1 << i) p.tile_shift = i;
   p.rows = n.rows;
   p.min_tiles = 1;
   p.c = static_cast<float>(q->scale * 1.4426950408889634);
