@@ -186,12 +186,12 @@ typedef struct {
 typedef struct {
   const void* q;
   void* o;
-  int64_t seqs, tokens, heads;
-  int64_t seq_stride, token_stride, head_stride; /* of q, in values */
   const int32_t* table;
-  int64_t table_stride, max_pages;
   const int32_t* lens;
   const int32_t* q_lens;
+  int64_t seqs, tokens, heads;
+  int64_t seq_stride, token_stride, head_stride; /* of q, in values */
+  int64_t table_stride, max_pages;
   double scale; /* of q . k, > 0 */
 } ntl_query_t;
 

@@ -24,16 +24,21 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
-from functools import lru_cache
 
 import torch
 
 from . import _lib
 
+# ntl_cache_t and ntl_query_t: pointers first, then what the shapes decide.
 _CACHE = struct.Struct("=12q")
 _QUERY = struct.Struct("=13qd")
+_CACHE_TAIL = struct.Struct("=10q")
+_QUERY_TAIL = struct.Struct("=8qd")
+_TWO = struct.Struct("=2q")
+_FIVE = struct.Struct("=5q")
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_empty, _empty_like, _uint8 = torch.empty, torch.empty_like, torch.uint8
 
 
 def _stream(index):
@@ -47,6 +52,34 @@ def _call(index, name, *args):
     else:
         with torch.cuda.device(index):
             _lib.call(name, *args, _stream(index))
+
+
+# ------------------------------------------------------------------------------ argument checks
+#
+# Checks look at shapes, strides, dtypes and devices alone, so a call whose arguments have been seen in
+# that form before skips them (about 10 us of a call): ``_plan`` keeps what a check returned by that
+# form, never by a tensor's address or identity.  Addresses are only checked for alignment, every time.
+
+_plans: dict = {}
+
+
+def _form(x):
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
+
+
+def _plan(check, tensors, *values):
+    """``check(*tensors, *values)``, or what it returned for arguments of the same form."""
+    try:
+        key = (check, *map(_form, tensors), *values)
+        plan = _plans.get(key)
+    except (AttributeError, TypeError, RuntimeError):  # not tensors, or not hashable: the check says so
+        return check(*tensors, *values)
+    if plan is None:
+        plan = check(*tensors, *values)
+        if len(_plans) >= 4096:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
 
 
 def _ints(name, x, index, *shape):
@@ -72,12 +105,16 @@ def _values(name, x):
         raise ValueError(f"{name}: expected dtype float16 or bfloat16, got {x.dtype}")
     if x.numel() and (x.stride(-1) != 1 or any(s % 8 for s in x.stride()[:-1])):
         raise ValueError(f"{name} must be dense along its last dimension, its other strides multiples of 8")
-    if x.data_ptr() % 16:
-        raise ValueError(f"{name} requires a tensor with an inspectable, 16-byte-aligned data pointer")
 
 
-def _cache(k, v, dims):
-    """(descriptor, device index) of a cache; ``dims``: the ranks it may have."""
+def _aligned(**tensors):
+    for name, x in tensors.items():
+        if x.data_ptr() % 16:
+            raise ValueError(f"{name} requires a tensor with an inspectable, 16-byte-aligned data pointer")
+
+
+def _check_cache(k, v, dims, written):
+    """(descriptor without its pointers, device index) of a cache; ``dims``: the ranks it may have."""
     _values("k", k)
     _values("v", v)
     shape, stride = k.shape, k.stride()
@@ -88,48 +125,35 @@ def _cache(k, v, dims):
     index = k.get_device()
     if v.get_device() != index:
         raise ValueError("All tensor arguments must be on the same CUDA device")
+    if written and any(n > 1 and s == 0 for n, s in zip(shape, stride)):
+        raise ValueError("k and v must not be broadcast: their rows are written")
     if len(shape) == 4:
         shape, stride = (1, *shape), (0, *stride)
     if shape[4] % 8 or not shape[4]:
         raise ValueError(f"k: head_dim {shape[4]} is not a multiple of 8")
     if not shape[2]:
         raise ValueError("k: page_size is 0")
-    return _CACHE.pack(k.data_ptr(), v.data_ptr(), *shape, *stride[:4], _DTYPES[k.dtype]), index
+    return _CACHE_TAIL.pack(*shape, *stride[:4], _DTYPES[k.dtype]), index
 
 
-def _writable(k):
-    if any(n > 1 and s == 0 for n, s in zip(k.shape, k.stride())):
-        raise ValueError("k and v must not be broadcast: their rows are written")
+def _cache(k, v, tail):
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if (kp | vp) & 15:
+        _aligned(k=k, v=v)
+    return _TWO.pack(kp, vp) + tail
 
 
-@lru_cache(maxsize=1024)
 def _pool_workspace(pages, n):
     out = ctypes.c_uint64(0)
     _lib.call("ntl_cache_workspace_size", pages, n, ctypes.byref(out))
     return out.value
 
 
-def _bytes(n, index):
-    return torch.empty(n, dtype=torch.uint8, device=f"cuda:{index}")
-
-
 # ------------------------------------------------------------------------------ attention
 
 
-@lru_cache(maxsize=1024)
-def _attention_workspace(index, cache_shape, dtype, q_shape, max_pages):
-    """Workspace bytes of an attention call: it depends on sizes alone."""
-    del index
-    pages, page_size, kv_heads, dim = cache_shape
-    cache = _CACHE.pack(16, 16, 1, pages, page_size, kv_heads, dim, 0, 0, 0, 0, dtype)
-    query = _QUERY.pack(16, 16, *q_shape[:3], 0, 0, 0, 16, 0, max_pages, 16, 0, 1.0)
-    out = ctypes.c_uint64(0)
-    _lib.call("ntl_cache_attention_workspace", cache, query, ctypes.byref(out))
-    return out.value
-
-
-def _attend(entry, q, k, v, table, lens, q_lens, scale, out, *args):
-    cache, index = _cache(k, v, (4,))
+def _check_attention(q, k, v, table, lens, q_lens, scale):
+    cache, index = _check_cache(k, v, (4,), False)
     _values("q", q)
     shape, kv = q.shape, k.shape
     if len(shape) != 4:
@@ -153,41 +177,79 @@ def _attend(entry, q, k, v, table, lens, q_lens, scale, out, *args):
         scale = 1.0 / math.sqrt(dim)
     elif not 0 < scale < 1e30:
         raise ValueError(f"scale must be positive and finite, got {scale}")
+    size = 0
+    query = _QUERY_TAIL.pack(seqs, tokens, heads, *q.stride()[:3], table.stride(0), table.shape[1], scale)
+    if q.numel():
+        out = ctypes.c_uint64(0)
+        with torch.cuda.device(index):
+            _lib.call("ntl_cache_attention_workspace", _TWO.pack(16, 16) + cache, _FIVE.pack(16, 16, 16, 16, 0) + query,
+                      ctypes.byref(out))
+        size = out.value
+    return cache, query, index, size, q.is_contiguous(), q.device
+
+
+def _check_out(out, q, k, v):
+    _values("out", out)
+    if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous() or out.device != q.device:
+        raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} on q's device")
+    _aligned(out=out)
+    begin, end = out.data_ptr(), out.data_ptr() + out.numel() * 2
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        if x.numel() and out.numel():
+            reach = sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1
+            if x.data_ptr() < end and begin < x.data_ptr() + 2 * reach:
+                raise ValueError(f"Tensor arguments {name} and out must have disjoint storage")
+
+
+def _attend(entry, q, k, v, table, lens, q_lens, scale, out, *args):
+    cache, query, index, size, dense, device = _plan(_check_attention, (q, k, v, table, lens, q_lens), scale)
+    qp = q.data_ptr()
+    if qp & 15:
+        _aligned(q=q)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = _empty_like(q) if dense else _empty(q.shape, dtype=q.dtype, device=device)
     else:
-        _values("out", out)
-        if out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != index:
-            raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(shape)} on q's device")
-        begin, end = out.data_ptr(), out.data_ptr() + out.numel() * 2
-        for name, x in (("q", q), ("k", k), ("v", v)):
-            if x.numel() and out.numel():
-                reach = sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1
-                if x.data_ptr() < end and begin < x.data_ptr() + 2 * reach:
-                    raise ValueError(f"Tensor arguments {name} and out must have disjoint storage")
-    if not out.numel():
+        _check_out(out, q, k, v)
+    if not size:
         return out
-    size = _attention_workspace(index, kv, _DTYPES[q.dtype], shape, table.shape[1])
-    work = _bytes(size, index) if size else None
-    stride = q.stride()
-    query = _QUERY.pack(q.data_ptr(), out.data_ptr(), seqs, tokens, heads, *stride[:3], table.data_ptr(),
-                        table.stride(0), table.shape[1], lens.data_ptr(), q_lens.data_ptr() if q_lens is not None else 0,
-                        scale)
-    _call(index, entry, cache, query, *args, work.data_ptr() if size else None, size)
+    work = _empty(size, dtype=_uint8, device=device)
+    query = _FIVE.pack(qp, out.data_ptr(), table.data_ptr(), lens.data_ptr(),
+                       0 if q_lens is None else q_lens.data_ptr()) + query
+    _call(index, entry, _cache(k, v, cache), query, *args, work.data_ptr(), size)
     return out
+
+
+def _check_parents(parents):
+    if not isinstance(parents, torch.Tensor) or not parents.is_cuda:
+        raise TypeError("parents must be a CUDA tensor")
+    index = parents.get_device()
+    _ints("parents", parents, index, None, None)
+    return index, (parents.shape[0], parents.shape[1], (parents.shape[1] + 31) // 32), parents.device
+
+
+def _check_tree(tree, q):
+    if not isinstance(tree, torch.Tensor) or tree.dim() != 3:
+        raise TypeError("tree must be a CUDA tensor [seqs or 1, tokens, words]")
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise TypeError("q must be a CUDA tensor")
+    if q.dim() != 4:
+        raise ValueError(f"q: expected 4 dimensions [seqs, tokens, heads, head_dim], got shape {tuple(q.shape)}")
+    seqs, tokens = q.shape[:2]
+    words = (tokens + 31) // 32
+    shared = tree.shape[0] == 1
+    _ints("tree", tree, q.get_device(), 1 if shared else seqs, tokens, words)
+    if tokens > 1 and tree.stride(1) != words:
+        raise ValueError("tree must be dense along its last two dimensions")
+    return 0 if shared else tree.stride(0)
 
 
 def tree_mask(parents):
     """Visibility words of draft trees: int32 [seqs, tokens, ceil(tokens / 32)], bit s % 32 of word
     s // 32 set where draft s is draft t itself or an ancestor.  ``parents`` int32 [seqs, tokens] holds
     each draft's parent; what is not an earlier draft (-1) is a root."""
-    if not isinstance(parents, torch.Tensor) or not parents.is_cuda:
-        raise TypeError("parents must be a CUDA tensor")
-    index = parents.get_device()
-    _ints("parents", parents, index, None, None)
-    seqs, tokens = parents.shape
-    words = torch.empty((seqs, tokens, (tokens + 31) // 32), dtype=torch.int32, device=parents.device)
-    _call(index, "ntl_tree_mask", parents.data_ptr(), parents.stride(0), seqs, tokens, words.data_ptr())
+    index, shape, device = _plan(_check_parents, (parents,))
+    words = _empty(shape, dtype=torch.int32, device=device)
+    _call(index, "ntl_tree_mask", parents.data_ptr(), parents.stride(0), shape[0], shape[1], words.data_ptr())
     return words
 
 
@@ -204,20 +266,8 @@ def tree_attention(q, k, v, table, lens, tree, *, q_lens=None, scale=None, out=N
     Statistics and sums are fp32; the exponentials are rounded to the cache's type for the product
     with V.  A NaN or infinity in a key row reaches the tokens that see it; in a value row that some token
     of the call sees, it may reach tokens of the same sequence that do not."""
-    if not isinstance(tree, torch.Tensor) or tree.dim() != 3:
-        raise TypeError("tree must be a CUDA tensor [seqs or 1, tokens, words]")
-    if not isinstance(q, torch.Tensor) or not q.is_cuda:
-        raise TypeError("q must be a CUDA tensor")
-    if q.dim() != 4:
-        raise ValueError(f"q: expected 4 dimensions [seqs, tokens, heads, head_dim], got shape {tuple(q.shape)}")
-    seqs, tokens = q.shape[:2]
-    words = (tokens + 31) // 32
-    shared = tree.shape[0] == 1
-    _ints("tree", tree, q.get_device(), 1 if shared else seqs, tokens, words)
-    if tokens > 1 and tree.stride(1) != words:
-        raise ValueError("tree must be dense along its last two dimensions")
-    return _attend("ntl_tree_attention", q, k, v, table, lens, q_lens, scale, out, tree.data_ptr(),
-                   0 if shared else tree.stride(0))
+    stride = _plan(_check_tree, (tree, q))
+    return _attend("ntl_tree_attention", q, k, v, table, lens, q_lens, scale, out, tree.data_ptr(), stride)
 
 
 def window_attention(q, k, v, table, lens, window, sinks=0, *, q_lens=None, scale=None, out=None):
@@ -235,12 +285,8 @@ def window_attention(q, k, v, table, lens, window, sinks=0, *, q_lens=None, scal
 # ------------------------------------------------------------------------------ cache operators
 
 
-def append_tokens(k, v, k_new, v_new, table, lens, counts=None):
-    """Write new tokens' rows, ``k_new`` / ``v_new`` [layers, seqs, tokens, kv_heads, head_dim] (4-D without
-    layers for a 4-D cache), at positions lens[b] + t, t < counts[b] (default: all); returns the new
-    lengths.  A row whose position has no page is dropped: ``reserve`` first."""
-    cache, index = _cache(k, v, (4, 5))
-    _writable(k)
+def _check_append(k, v, k_new, v_new, table, lens, counts):
+    cache, index = _check_cache(k, v, (4, 5), True)
     _values("k_new", k_new)
     _values("v_new", v_new)
     layered = k.dim() == 5
@@ -258,46 +304,82 @@ def append_tokens(k, v, k_new, v_new, table, lens, counts=None):
     _ints("lens", lens, index, seqs)
     if counts is not None:
         _ints("counts", counts, index, seqs)
-    new = torch.empty_like(lens)
     stride = k_new.stride() if layered else (0, *k_new.stride())
-    _call(index, "ntl_cache_append", cache, k_new.data_ptr(), v_new.data_ptr(), *stride[:4], table.data_ptr(),
-          table.stride(0), seqs, table.shape[1], lens.data_ptr(), counts.data_ptr() if counts is not None else None,
-          tokens, new.data_ptr())
+    return cache, index, stride[:4], (table.stride(0), seqs, table.shape[1]), tokens
+
+
+def append_tokens(k, v, k_new, v_new, table, lens, counts=None):
+    """Write new tokens' rows, ``k_new`` / ``v_new`` [layers, seqs, tokens, kv_heads, head_dim] (4-D without
+    layers for a 4-D cache), at positions lens[b] + t, t < counts[b] (default: all); returns the new
+    lengths.  A row whose position has no page is dropped: ``reserve`` first."""
+    cache, index, strides, sizes, tokens = _plan(_check_append, (k, v, k_new, v_new, table, lens, counts))
+    kp, vp = k_new.data_ptr(), v_new.data_ptr()
+    if (kp | vp) & 15:
+        _aligned(k_new=k_new, v_new=v_new)
+    new = _empty_like(lens)
+    _call(index, "ntl_cache_append", _cache(k, v, cache), kp, vp, *strides, table.data_ptr(), *sizes, lens.data_ptr(),
+          None if counts is None else counts.data_ptr(), tokens, new.data_ptr())
     return new
+
+
+def _check_accept(k, v, table, lens, path, counts, each, common):
+    cache, index = _check_cache(k, v, (4, 5), True)
+    _ints("lens", lens, index, None)
+    seqs = lens.shape[0]
+    _ints("table", table, index, seqs, None)
+    _ints("path", path, index, seqs, None)
+    _ints("counts", counts, index, seqs)
+    if each is not None:
+        _ints("drafts", each, index, seqs)
+    elif common < 0:
+        raise ValueError(f"drafts must be at least 0, got {common}")
+    return cache, index, (table.stride(0), seqs, table.shape[1]), (path.stride(0), path.shape[1])
 
 
 def accept_path(k, v, table, lens, path, counts, drafts):
     """Keep a verified path of each sequence's last ``drafts`` cached tokens (an int, or int32 [seqs]): the
     row of draft path[b, i] moves to draft place i, i < counts[b]; ``path`` int32 [seqs, most] increases along
     i.  Returns the new lengths, lens - drafts + counts."""
-    cache, index = _cache(k, v, (4, 5))
-    _writable(k)
-    _ints("lens", lens, index, None)
-    seqs = lens.shape[0]
-    _ints("table", table, index, seqs, None)
-    _ints("path", path, index, seqs, None)
-    _ints("counts", counts, index, seqs)
-    each, common = None, 0
-    if isinstance(drafts, torch.Tensor):
-        _ints("drafts", drafts, index, seqs)
-        each = drafts.data_ptr()
-    elif drafts < 0:
-        raise ValueError(f"drafts must be at least 0, got {drafts}")
-    else:
-        common = int(drafts)
-    new = torch.empty_like(lens)
-    _call(index, "ntl_cache_accept", cache, table.data_ptr(), table.stride(0), seqs, table.shape[1], lens.data_ptr(),
-          each, common, path.data_ptr(), path.stride(0), path.shape[1], counts.data_ptr(), new.data_ptr())
+    each, common = (drafts, 0) if isinstance(drafts, torch.Tensor) else (None, int(drafts))
+    cache, index, sizes, steps = _plan(_check_accept, (k, v, table, lens, path, counts, each), common)
+    new = _empty_like(lens)
+    _call(index, "ntl_cache_accept", _cache(k, v, cache), table.data_ptr(), *sizes, lens.data_ptr(),
+          None if each is None else each.data_ptr(), common, path.data_ptr(), *steps, counts.data_ptr(), new.data_ptr())
     return new
+
+
+def _check_copy(k, v, src, dst):
+    cache, index = _check_cache(k, v, (4, 5), True)
+    _ints("src", src, index, None)
+    _ints("dst", dst, index, src.shape[0])
+    return cache, index, src.shape[0]
 
 
 def copy_pages(k, v, src, dst):
     """Copy pages ``src[i]`` to ``dst[i]`` (int32), all layers, K and V.  No page may be both read and written."""
-    cache, index = _cache(k, v, (4, 5))
-    _writable(k)
+    cache, index, n = _plan(_check_copy, (k, v, src, dst))
+    _call(index, "ntl_cache_copy_pages", _cache(k, v, cache), src.data_ptr(), dst.data_ptr(), n)
+
+
+def _check_sequences(table, lens, refs, pages, index):
+    if index is None:
+        if not isinstance(table, torch.Tensor) or not table.is_cuda:
+            raise TypeError("table must be a CUDA tensor")
+        index = table.get_device()
+    _ints("table", table, index, None, None)
+    _ints("lens", lens, index, table.shape[0])
+    _ints("refs", refs, index, pages)
+    return index, (table.stride(0), *table.shape)
+
+
+def _check_fork(k, v, table, lens, refs, src, dst):
+    cache, index = _check_cache(k, v, (4, 5), True)
+    pages = k.shape[-4]
+    _, sizes = _check_sequences(table, lens, refs, pages, index)
     _ints("src", src, index, None)
-    _ints("dst", dst, index, src.shape[0])
-    _call(index, "ntl_cache_copy_pages", cache, src.data_ptr(), dst.data_ptr(), src.shape[0])
+    n = src.shape[0]
+    _ints("dst", dst, index, n)
+    return cache, index, sizes, n, _pool_workspace(pages, n), k.device
 
 
 def fork(k, v, table, lens, refs, src, dst):
@@ -305,83 +387,73 @@ def fork(k, v, table, lens, refs, src, dst):
     the part of a page at the end is copied into the lowest free page, in order.  ``dst`` and ``src`` have no
     sequence in common.  Updates table, lens and refs in place; returns int32 [n]: 1, or 0 where no
     page was left and the child holds nothing."""
-    cache, index = _cache(k, v, (4, 5))
-    _writable(k)
-    pages = k.shape[-4]
-    _ints("table", table, index, None, None)
-    _ints("lens", lens, index, table.shape[0])
-    _ints("refs", refs, index, pages)
-    _ints("src", src, index, None)
-    n = src.shape[0]
-    _ints("dst", dst, index, n)
-    granted = torch.empty_like(src)
-    size = _pool_workspace(pages, n)
-    work = _bytes(size, index)
-    _call(index, "ntl_cache_fork", cache, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
-          lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n, granted.data_ptr(), work.data_ptr(), size)
+    cache, index, sizes, n, size, device = _plan(_check_fork, (k, v, table, lens, refs, src, dst))
+    granted = _empty(n, dtype=torch.int32, device=device)
+    work = _empty(size, dtype=_uint8, device=device)
+    _call(index, "ntl_cache_fork", _cache(k, v, cache), table.data_ptr(), *sizes, lens.data_ptr(), refs.data_ptr(),
+          src.data_ptr(), dst.data_ptr(), n, granted.data_ptr(), work.data_ptr(), size)
     return granted
+
+
+def _check_reserve(table, lens, refs, seqs, each, common, page_size):
+    index, sizes = _check_sequences(table, lens, refs, None, None)
+    _ints("seqs", seqs, index, None)
+    n, pages = seqs.shape[0], refs.shape[0]
+    if each is not None:
+        _ints("extra", each, index, n)
+    elif common < 0:
+        raise ValueError(f"extra must be at least 0, got {common}")
+    if page_size < 1:
+        raise ValueError(f"page_size must be at least 1, got {page_size}")
+    return index, sizes, n, pages, _pool_workspace(pages, n), table.device
 
 
 def reserve(table, lens, refs, seqs, extra, page_size):
     """Map the lowest free pages so that each sequence in ``seqs`` (int32, no repeats) can hold ``extra`` (an int,
     or int32 [n]) more tokens, in order.  Updates table and refs in place; returns int32 [n]: 1, or 0 where
     the pages or the table's width ran out and nothing was mapped."""
-    if not isinstance(table, torch.Tensor) or not table.is_cuda:
-        raise TypeError("table must be a CUDA tensor")
-    index = table.get_device()
-    _ints("table", table, index, None, None)
-    _ints("lens", lens, index, table.shape[0])
-    _ints("refs", refs, index, None)
-    _ints("seqs", seqs, index, None)
-    n, pages = seqs.shape[0], refs.shape[0]
-    each, common = None, 0
-    if isinstance(extra, torch.Tensor):
-        _ints("extra", extra, index, n)
-        each = extra.data_ptr()
-    elif extra < 0:
-        raise ValueError(f"extra must be at least 0, got {extra}")
-    else:
-        common = int(extra)
-    granted = torch.empty_like(seqs)
-    size = _pool_workspace(pages, n)
-    work = _bytes(size, index)
-    _call(index, "ntl_cache_reserve", pages, int(page_size), table.data_ptr(), table.stride(0), table.shape[0],
-          table.shape[1], lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), n, common, each, granted.data_ptr(),
-          work.data_ptr(), size)
+    each, common = (extra, 0) if isinstance(extra, torch.Tensor) else (None, int(extra))
+    index, sizes, n, pages, size, device = _plan(_check_reserve, (table, lens, refs, seqs, each), common, int(page_size))
+    granted = _empty(n, dtype=torch.int32, device=device)
+    work = _empty(size, dtype=_uint8, device=device)
+    _call(index, "ntl_cache_reserve", pages, int(page_size), table.data_ptr(), *sizes, lens.data_ptr(), refs.data_ptr(),
+          seqs.data_ptr(), n, common, None if each is None else each.data_ptr(), granted.data_ptr(), work.data_ptr(),
+          size)
     return granted
+
+
+def _check_free(table, lens, refs, seqs):
+    index, sizes = _check_sequences(table, lens, refs, None, None)
+    _ints("seqs", seqs, index, None)
+    return index, sizes, refs.shape[0], seqs.shape[0]
 
 
 def free(table, lens, refs, seqs):
     """Sequences ``seqs`` (int32) give their pages back and hold nothing; table, lens and refs in place."""
-    if not isinstance(table, torch.Tensor) or not table.is_cuda:
-        raise TypeError("table must be a CUDA tensor")
-    index = table.get_device()
+    index, sizes, pages, n = _plan(_check_free, (table, lens, refs, seqs))
+    _call(index, "ntl_cache_free", pages, table.data_ptr(), *sizes, lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), n)
+
+
+def _check_compact(k, v, table, refs, table_out, refs_out):
+    cache, index = _check_cache(k, v, (4, 5), True)
+    pages = k.shape[-4]
     _ints("table", table, index, None, None)
-    _ints("lens", lens, index, table.shape[0])
-    _ints("refs", refs, index, None)
-    _ints("seqs", seqs, index, None)
-    _call(index, "ntl_cache_free", refs.shape[0], table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
-          lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), seqs.shape[0])
+    _ints("refs", refs, index, pages)
+    _ints("table_out", table_out, index, *table.shape)
+    _ints("refs_out", refs_out, index, pages)
+    return cache, index, table.shape, _pool_workspace(pages, 0), k.device
 
 
 def compact(k, v, table, refs, *, table_out=None, refs_out=None):
     """Move the live pages (refs > 0) to the lowest numbers: of n, the k-th at or past n goes into the k-th hole
     before n.  ``table_out`` and ``refs_out`` (default: in place) follow.  Returns int32 [1]: n."""
-    cache, index = _cache(k, v, (4, 5))
-    _writable(k)
-    pages = k.shape[-4]
-    _ints("table", table, index, None, None)
-    _ints("refs", refs, index, pages)
     table_out = table if table_out is None else table_out
     refs_out = refs if refs_out is None else refs_out
-    _ints("table_out", table_out, index, *table.shape)
-    _ints("refs_out", refs_out, index, pages)
-    live = torch.empty(1, dtype=torch.int32, device=k.device)
-    size = _pool_workspace(pages, 0)
-    work = _bytes(size, index)
-    _call(index, "ntl_cache_compact", cache, table.data_ptr(), table.stride(0), table_out.data_ptr(),
-          table_out.stride(0), table.shape[0], table.shape[1], refs.data_ptr(), refs_out.data_ptr(), live.data_ptr(),
-          work.data_ptr(), size)
+    cache, index, shape, size, device = _plan(_check_compact, (k, v, table, refs, table_out, refs_out))
+    live = _empty(1, dtype=torch.int32, device=device)
+    work = _empty(size, dtype=_uint8, device=device)
+    _call(index, "ntl_cache_compact", _cache(k, v, cache), table.data_ptr(), table.stride(0), table_out.data_ptr(),
+          table_out.stride(0), *shape, refs.data_ptr(), refs_out.data_ptr(), live.data_ptr(), work.data_ptr(), size)
     return live
 
 

@@ -22,9 +22,9 @@ def cache(**change):
 def query(**change):
     from ntilang_b200 import paged
 
-    names = ["q", "o", "seqs", "tokens", "heads", "seq_stride", "token_stride", "head_stride", "table", "table_stride",
-             "max_pages", "lens", "q_lens", "scale"]
-    values = dict(zip(names, [PTR, PTR, 2, 3, 4, 768, 256, 64, PTR, 8, 8, PTR, 0, 0.125]))
+    names = ["q", "o", "table", "lens", "q_lens", "seqs", "tokens", "heads", "seq_stride", "token_stride", "head_stride",
+             "table_stride", "max_pages", "scale"]
+    values = dict(zip(names, [PTR, PTR, PTR, PTR, 0, 2, 3, 4, 768, 256, 64, 8, 8, 0.125]))
     assert set(change) <= set(names)
     return paged._QUERY.pack(*{**values, **change}.values())
 
