@@ -59,7 +59,6 @@ struct AttnParams {
   int tile_pages;    // pages per tile (1 where a page holds several tiles)
   int tile_shift;    // log2 of tile_keys, -1 if it is no power of two
   int rows;          // rows a workspace slot has
-  int min_tiles;     // least tiles per CTA
   float c;           // softmax scale in log2 units
   int64_t wait_limit;
 };
@@ -84,6 +83,12 @@ struct Shape {
   __host__ __device__ static constexpr uint32_t O_COL(int i) { return static_cast<uint32_t>(2 * BN + i * D); }
 };
 
+struct Unit {
+  int b, t0;        // sequence, first token
+  int len, live;    // cached tokens; new tokens among them
+  int tiles, sink_tiles, first;  // key tiles; those of the sinks; the window's first
+};
+
 struct __align__(16) Ctl {
   uint64_t q_full, q_empty;
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
@@ -94,8 +99,11 @@ struct __align__(16) Ctl {
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
+  uint64_t merge;  // the key groups of a row: hand-offs among the four softmax warps
   int start[5];  // first unit's item, key head, tile; tiles of this CTA; total tiles
+  Unit unit;     // the first unit
   int sums[32];
+  float2 ml[BM];  // (m, l) of every row and key group
 };
 
 template <int D, int NT>
@@ -138,12 +146,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int64_
 
 // ------------------------------------------------------------------------------ units
 
-struct Unit {
-  int b, t0;        // sequence, first token
-  int len, live;    // cached tokens; new tokens among them
-  int tiles, sink_tiles, first;  // key tiles; those of the sinks; the window's first
-};
-
 __device__ __forceinline__ int tile_index(const AttnParams& p, int key) {
   return p.tile_shift >= 0 ? key >> p.tile_shift : key / p.tile_keys;
 }
@@ -178,10 +180,18 @@ __device__ __forceinline__ bool past_end(const AttnParams& p, const Unit& u, int
   return u.len - tile_key(p, u, a) < p.tile_keys;
 }
 
+// a / b for a >= 0, b > 0: the fast divide is within one of it below 2^22.
+__device__ __forceinline__ int quotient(int a, int b) {
+  if (a >> 22) return a / b;
+  int q = static_cast<int>(__fdividef(static_cast<float>(a), static_cast<float>(b)));
+  const int r = a - q * b;
+  return r < 0 ? q - 1 : r >= b ? q + 1 : q;
+}
+
 // The pieces: `total` tiles over `ctas` CTAs, CTA i from piece_start(i).
 __device__ __forceinline__ int piece_start(int i, int total, int ctas) {  // floor(i * total / ctas)
-  const int each = total / ctas;
-  return i * each + i * (total - each * ctas) / ctas;
+  const int each = quotient(total, ctas);
+  return i * each + quotient(i * (total - each * ctas), ctas);
 }
 __device__ __forceinline__ int piece_of(int tile, int total, int ctas) {
   return static_cast<int>(((static_cast<int64_t>(tile) + 1) * ctas - 1) / total);
@@ -208,35 +218,40 @@ __device__ __forceinline__ int block_exclusive(int x, int* sums, int& total) {
   return before + s - x;
 }
 
-// Finds this CTA's piece (ctl->start); all threads.  Returns the CTAs that have a piece.
+// Finds this CTA's piece (ctl->start and its first unit); all threads.  Returns the CTAs that have one.
 __device__ __forceinline__ int find_piece(const AttnParams& p, Ctl* ctl, int block_tokens) {
   const int items = p.seqs * p.blocks;
-  int total = 0, mine = 0, at = 0;
+  int total = 0, at = 0;
+  Unit u;
+  u.tiles = 0;
   for (int e0 = 0; e0 < items; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
-    mine = e < items ? unit_of(p, e, block_tokens).tiles * p.kv_heads : 0;
+    u.tiles = 0;
+    if (e < items) u = unit_of(p, e, block_tokens);
     int sum;
-    at = total + block_exclusive(mine, ctl->sums, sum);
+    at = total + block_exclusive(u.tiles * p.kv_heads, ctl->sums, sum);
     total += sum;
   }
-  const int ctas = max(1, min(static_cast<int>(gridDim.x), total / p.min_tiles));
+  const int ctas = min(static_cast<int>(gridDim.x), total);
   if (static_cast<int>(blockIdx.x) >= ctas) return ctas;
-  const int begin = piece_start(blockIdx.x, total, ctas), end = piece_start(blockIdx.x + 1, total, ctas);
+  const int begin = piece_start(blockIdx.x, total, ctas);
   int seen = 0;
   for (int e0 = 0; e0 < items; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
     if (items > static_cast<int>(blockDim.x)) {
-      mine = e < items ? unit_of(p, e, block_tokens).tiles * p.kv_heads : 0;
+      u.tiles = 0;
+      if (e < items) u = unit_of(p, e, block_tokens);
       int sum;
-      at = seen + block_exclusive(mine, ctl->sums, sum);
+      at = seen + block_exclusive(u.tiles * p.kv_heads, ctl->sums, sum);
       seen += sum;
     }
-    if (mine > 0 && at <= begin && begin < at + mine) {
-      const int tiles = mine / p.kv_heads;
+    if (at <= begin && begin < at + u.tiles * p.kv_heads) {
+      const int head = quotient(begin - at, u.tiles);
+      ctl->unit = u;
       ctl->start[0] = e;
-      ctl->start[1] = (begin - at) / tiles;
-      ctl->start[2] = (begin - at) % tiles;
-      ctl->start[3] = end - begin;
+      ctl->start[1] = head;
+      ctl->start[2] = begin - at - head * u.tiles;
+      ctl->start[3] = piece_start(blockIdx.x + 1, total, ctas) - begin;
       ctl->start[4] = total;
     }
   }
@@ -249,12 +264,12 @@ struct Walk {
   Unit u;
   int a0, a1;  // this unit's tiles in this CTA
 
-  __device__ __forceinline__ void begin(const AttnParams& p, const Ctl* ctl, int block_tokens) {
+  __device__ __forceinline__ void begin(const Ctl* ctl) {
     item = ctl->start[0];
     kv_head = ctl->start[1];
     tile = ctl->start[2];
     left = ctl->start[3];
-    u = unit_of(p, item, block_tokens);
+    u = ctl->unit;
     a0 = tile;
     a1 = min(u.tiles, a0 + left);
   }
@@ -282,10 +297,27 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 // kind::f16 instruction descriptor (see umma_idesc_f16_f32) with both operands fp16 or both bf16.
 template <bool BF16>
 __host__ __device__ constexpr uint32_t idesc(uint32_t n, uint32_t b_mn_major) {
   return umma_idesc_f16_f32(BM, n, 0, b_mn_major) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+}
+
+// umma_desc_sw128 as its low word and a constant high word: the descriptor of an operand `bytes` further on
+// is one 32-bit add away (shared memory ends below 2^18 bytes, so the 14-bit address field does not
+// overflow), which keeps the issuing thread ahead of the softmax.
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr, uint32_t lbo_bytes) {
+  return (smem_addr >> 4) | (lbo_bytes >> 4) << 16;
+}
+__device__ __forceinline__ uint64_t desc_at(uint32_t low, uint32_t bytes) {
+  constexpr uint32_t high = (1024u >> 4) | 1u << 14 | 2u << 29;  // stride 1024 bytes, version 1, 128-byte swizzle
+  return static_cast<uint64_t>(high) << 32 | (low + (bytes >> 4));
 }
 
 template <bool BF16>
@@ -330,12 +362,14 @@ __device__ __forceinline__ uint64_t visible(const AttnParams& p, const Unit& u, 
 
 // ------------------------------------------------------------------------------ kernel
 
-template <int D, int NT, bool BF16>
+template <int D, int NT, int KS, bool BF16>
 __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_SM)
     cache_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv, const AttnParams p) {
   using C = Shape<D, NT>;
   constexpr int BN = C::BN, ST = C::STAGES;
+  constexpr int KC = BN / KS;          // keys of a tile per key group
+  constexpr int GROUP_ROWS = BM / KS;  // rows of the tile per key group
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL_OFF);
@@ -363,6 +397,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       mbar_init(&ctl->p_ready[i], 4);
       mbar_init(&ctl->pv_done[i], 1);
     }
+    mbar_init(&ctl->merge, 4);
     mbar_init(&ctl->drain, 1);
     ctl->abort = 0;
     fence_mbar_init();
@@ -388,7 +423,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
   }
   const uint32_t tmem = ctl->tmem_base;
   Walk w;
-  w.begin(p, ctl, block_tokens);
+  w.begin(ctl);
 
   if (warp >= C::SOFTMAX_WARPS) {
     if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS_OTHER) : "memory");
@@ -455,7 +490,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       }
     } else if (warp == C::AUX_WARP) {
       // ---------------------------------------------- Q loads, and value rows past the end become zeros
-      const uint32_t q_bytes = static_cast<uint32_t>(NT * (D / 64) * p.tile_tokens * p.group * 128);
+      const uint32_t q_bytes = static_cast<uint32_t>(NT * KS * (D / 64) * p.tile_tokens * p.group * 128);
       bool ok = true;
       int n = 0, g = 0;
       uint32_t raw = 0;  // bit s: parity of v_raw[s]
@@ -466,11 +501,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           if (ok) {
             mbar_arrive_expect_tx(&ctl->q_full, q_bytes);
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+            for (int i = 0; i < NT * KS; ++i)  // row tiles, or copies for the key groups
 #pragma unroll
               for (int d = 0; d < D / 64; ++d)
-                tma_load_4d(smem + i * C::Q_BYTES + d * (BM * 128), &tq, &ctl->q_full, d * 64, w.kv_head * p.group,
-                            w.u.t0 + i * p.tile_tokens, w.u.b);
+                tma_load_4d(smem + (NT == 2 ? i * C::Q_BYTES : i * GROUP_ROWS * 128) + d * (BM * 128), &tq, &ctl->q_full,
+                            d * 64, w.kv_head * p.group, w.u.t0 + (NT == 2 ? i * p.tile_tokens : 0), w.u.b);
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -519,17 +554,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
         if (aq == wq.a0 && !wait(&ctl->q_full, uq & 1)) return false;
         return wait(&ctl->k_full[gq % ST], (gq / ST) & 1);
       };
+      const uint32_t q_low = desc_low(smem_u32(smem), 16);
+      const uint32_t k_low = desc_low(smem_u32(smem + C::K_OFF), 16);
+      const uint32_t v_low = desc_low(smem_u32(smem + C::V_OFF), BN * 128);
       auto qk = [&](int i) {  // S (buffer gq % 2, or row tile i) = Q_i K^T
-        const uint32_t q_addr = smem_u32(smem + (NT == 2 ? i : 0) * C::Q_BYTES);
-        const uint32_t k_addr = smem_u32(smem + C::K_OFF + (gq % ST) * C::KV_BYTES);
+        const uint32_t q = q_low + (NT == 2 ? i : 0) * (C::Q_BYTES >> 4), k = k_low + (gq % ST) * (C::KV_BYTES >> 4);
         const int buf = NT == 2 ? i : gq & 1;
         tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t q_off = (kk >> 2) * (BM * 128) + (kk & 3) * 32, k_off = (kk >> 2) * (BN * 128) + (kk & 3) * 32;
-          tc_mma_f16_ss(tmem + C::S_COL(buf), umma_desc_sw128(q_addr + q_off, 16, 1024),
-                        umma_desc_sw128(k_addr + k_off, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
-        }
+        for (int kk = 0; kk < D / 16; ++kk)
+          tc_mma_f16_ss(tmem + C::S_COL(buf), desc_at(q, (kk >> 2) * (BM * 128) + (kk & 3) * 32),
+                        desc_at(k, (kk >> 2) * (BN * 128) + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
         tc_commit(&ctl->s_full[buf]);
       };
       auto qk_end = [&]() {  // after the last row tile's
@@ -556,11 +591,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
             const int buf = NT == 2 ? i : g & 1;
             if (!wait(&ctl->p_ready[buf], (NT == 2 ? g : g >> 1) & 1)) return false;
             tc_fence_after();
-            const uint32_t v_addr = smem_u32(smem + C::V_OFF + s * C::KV_BYTES);
+            const uint32_t v = v_low + s * (C::KV_BYTES >> 4);
 #pragma unroll
             for (int kk = 0; kk < BN / 16; ++kk)
-              tc_mma_f16_ts(tmem + C::O_COL(i), tmem + C::S_COL(buf) + kk * 8,
-                            umma_desc_sw128(v_addr + kk * 2048, BN * 128, 1024), idesc_o, (a > w.a0 || kk > 0) ? 1u : 0u);
+              tc_mma_f16_ts(tmem + C::O_COL(i), tmem + C::S_COL(buf) + kk * 8, desc_at(v, kk * 2048), idesc_o,
+                            (a > w.a0 || kk > 0) ? 1u : 0u);
             tc_commit(&ctl->pv_done[i]);
             return true;
           };
@@ -605,11 +640,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       }
     }
   } else {
-    // ---------------------------------------------- softmax: one thread per row
+    // ---------------------------------------------- softmax: one thread per row (and key group)
     if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS_SOFTMAX) : "memory");
     const int i = warp >> 2;
-    const int r = (warp & 3) * 32 + lane;
-    const int row_token = r / p.group, row_head = r - row_token * p.group;
+    const int group = KS == 1 ? 0 : (warp & 3) / (4 / KS);
+    const int r = (warp & 3) * 32 + lane - group * GROUP_ROWS;
+    const int row_token = quotient(r, p.group), row_head = r - row_token * p.group;
     const int t_in_block = i * p.tile_tokens + row_token;
     const bool in_tile = row_token < p.tile_tokens;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -618,11 +654,18 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
     int4 cut = make_int4(0, 0, -1, 0);
     bool ok = true;
     int g = 0;
+    uint32_t merges = 0;
+    // The four warps meet (key groups only): false when one of them gave up.
+    auto meet = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->merge);
+      return warp_wait(&ctl->merge, merges++ & 1, p.wait_limit, abort_flag);
+    };
     do {
       const Unit& u = w.u;
       const int t = u.t0 + t_in_block;
       const bool live = in_tile && t < u.live;
-      const bool any = __any_sync(0xffffffffu, live);
+      const bool any = KS > 1 ? u.t0 < u.live : __any_sync(0xffffffffu, live);
       const bool here = in_tile && t < p.tokens;  // the output has this row
       const int64_t out_row =
           (static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + w.kv_head * p.group + row_head;
@@ -639,19 +682,24 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
         if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g >> 1) & 1, p.wait_limit, abort_flag))) break;
         if (any) {
           tc_fence_after();
-          uint32_t sv[BN];
+          uint32_t sv[KC];
+          if constexpr (KC == 16) {
+            tmem_ld_32x32b_x16(s_addr + group * KC, sv);
+          } else {
 #pragma unroll
-          for (int ch = 0; ch < BN / 32; ++ch)
-            tmem_ld_32x32b_x32(s_addr + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + ch * 32));
+            for (int ch = 0; ch < KC / 32; ++ch)
+              tmem_ld_32x32b_x32(s_addr + group * KC + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + ch * 32));
+          }
           tc_wait_ld();
           const int k0 = tile_key(p, u, a);
           const bool whole = p.tile_keys == BN && k0 + BN <= all_hi && (k0 >= all_lo || k0 + BN <= p.sinks);
           if (!whole) {
 #pragma unroll
-            for (int ch = 0; ch < BN / 64; ++ch) {
+            for (int ch = 0; ch < (KC + 63) / 64; ++ch) {
               uint64_t see = live ? visible(p, u, t, k0 + ch * 64) & low_bits(p.tile_keys - ch * 64) : 0;
+              if constexpr (KS > 1) see >>= group * KC;
 #pragma unroll
-              for (int e = 0; e < 64; ++e)
+              for (int e = 0; e < (KC < 64 ? KC : 64); ++e)
                 if (!(see >> e & 1)) sv[ch * 64 + e] = __float_as_uint(-INFINITY);
             }
           }
@@ -659,7 +707,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           {
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < BN; e += 8) {
+            for (int e = 0; e < KC; e += 8) {
               x[0] = fmax3(x[0], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
               x[1] = fmax3(x[1], __uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3]));
               x[2] = fmax3(x[2], __uint_as_float(sv[e + 4]), __uint_as_float(sv[e + 5]));
@@ -699,19 +747,40 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           const float shift = m == -INFINITY ? 0.0f : -m * c;
           const uint64_t c2 = f2_make(c, c), shift2 = f2_make(shift, shift);
           uint64_t acc[2] = {0ull, 0ull};
+          // This group's exponentials over its own 16-bit columns of the tile; the others' are zero
+          // in these lanes, so that P V adds up this group's keys alone.
+          constexpr int PC = KC < 32 ? KC / 2 : 16;  // packed columns per store
 #pragma unroll
-          for (int ch = 0; ch < BN / 32; ++ch) {
-            uint32_t packed[16];
+          for (int ch = 0; ch < KC / (2 * PC); ++ch) {
+            uint32_t packed[PC];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int k = ch * 32 + 2 * e;
+            for (int e = 0; e < PC; ++e) {
+              const int k = ch * 2 * PC + 2 * e;
               float x0, x1;
               f2_split(f2_fma(f2_make(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), c2, shift2), x0, x1);
               const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
               acc[e & 1] = f2_add(acc[e & 1], f2_make(p0, p1));
               packed[e] = pack2<BF16>(p0, p1);
             }
-            tmem_st_32x32b_x16(s_addr + ch * 16, packed);
+            if constexpr (PC == 8) {
+              tmem_st_32x32b_x8(s_addr + group * (KC / 2) + ch * PC, packed);
+            } else {
+              tmem_st_32x32b_x16(s_addr + group * (KC / 2) + ch * PC, packed);
+            }
+          }
+          if constexpr (KS > 1) {
+            uint32_t zero[PC];
+#pragma unroll
+            for (int e = 0; e < PC; ++e) zero[e] = 0;
+#pragma unroll
+            for (int j = 1; j < KS; ++j) {
+              const uint32_t at = s_addr + ((group + j) % KS) * (KC / 2);
+              if constexpr (PC == 8) {
+                tmem_st_32x32b_x8(at, zero);
+              } else {
+                tmem_st_32x32b_x16(at, zero);
+              }
+            }
           }
           float s0, s1;
           f2_split(f2_add(acc[0], acc[1]), s0, s1);
@@ -730,27 +799,87 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
         const int unit_start = piece_start(blockIdx.x + 1, total, ctas) - w.a1;
         cut = make_int4(w.item, w.kv_head, piece_of(unit_start + u.tiles - 1, total, ctas), 0);
       }
-      if (any) {
-        // Rows leave through shared memory, 64 bytes of each at a time, so that a store instruction
-        // writes whole sectors: quad n of a warp writes 64 bytes of row 8 i + n (a thread writing its own
-        // row 16 bytes at a time took 5 to 9 us per 108 rows).
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (w.a0 == 0 ? 1 : 0);
-        const int64_t slot_row = slot * p.rows + i * BM + (warp & 3) * 32;  // of the warp's first row
+      // Rows leave through shared memory, so that store instructions write whole sectors (a thread writing
+      // its own row 16 bytes at a time took 5 to 9 us per 108 rows).
+      const int64_t slot_row = (2 * static_cast<int64_t>(blockIdx.x) + (w.a0 == 0 ? 1 : 0)) * p.rows + i * BM;
+      if constexpr (KS > 1) {
+        if (any) {
+          // Each row's key groups add up: weights 2^(m_k - max m).
+          const float mc = m == -INFINITY ? m : m * c;
+          ctl->ml[group * GROUP_ROWS + r] = make_float2(mc, l);
+          if (!(ok = meet())) break;
+          float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) top = fmaxf(top, ctl->ml[k * GROUP_ROWS + r].x);
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            const float2 x = ctl->ml[k * GROUP_ROWS + r];
+            sum += x.x == -INFINITY ? (x.y == x.y ? 0.0f : x.y) : ex2_approx(x.x - top) * x.y;
+          }
+          const float inv = !done ? 1.0f : sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
+          const float weight = mc == -INFINITY ? (l == l ? 0.0f : l) : ex2_approx(mc - top) * inv;
+          if (!done && live && group == 0) p.part_ml[slot_row + r] = make_float2(top, sum);
+          // 16 columns of every live row and group are staged at a time, or more where few rows leave room.
+          const int rows = min(p.tile_tokens, u.live - u.t0) * p.group;
+          const int at_once = min(D / 16, (4 * 32) / (KS * rows));
+          const int tid = (warp & 3) * 32 + lane;
+#pragma unroll 1
+          for (int c0 = 0; c0 < D / 16 && ok; c0 += at_once) {
+            const int n = min(at_once, D / 16 - c0);
+#pragma unroll 1
+            for (int ch = 0; ch < n; ++ch) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(o_addr + (c0 + ch) * 16, o);
+              tc_wait_ld();
+              float4* to = reinterpret_cast<float4*>(smem + C::OUT_OFF + ((ch * KS + group) * rows + r) * kOutRow);
+              if (r < rows)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  to[e] = make_float4(__uint_as_float(o[4 * e]) * weight, __uint_as_float(o[4 * e + 1]) * weight,
+                                      __uint_as_float(o[4 * e + 2]) * weight, __uint_as_float(o[4 * e + 3]) * weight);
+            }
+            if (!(ok = meet())) break;
+            // 4 columns of a row per thread and round
+#pragma unroll 1
+            for (int e = tid; e < n * rows * 4; e += 128) {
+              const int line = e >> 2, ch = quotient(line, rows), row = line - ch * rows;
+              float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+              for (int k = 0; k < KS; ++k) {
+                const float4 y = *reinterpret_cast<const float4*>(smem + C::OUT_OFF + ((ch * KS + k) * rows + row) * kOutRow +
+                                                                  (e & 3) * 16);
+                x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+              }
+              const int column = (c0 + ch) * 16 + (e & 3) * 4;
+              if (done) {
+                const int token = quotient(row, p.group);
+                const int64_t to = (static_cast<int64_t>(u.b) * p.tokens + u.t0 + token) * p.heads +
+                                   w.kv_head * p.group + row - token * p.group;
+                *reinterpret_cast<uint2*>(p.o + to * D + column) = make_uint2(pack2<BF16>(x.x, x.y), pack2<BF16>(x.z, x.w));
+              } else {
+                *reinterpret_cast<float4*>(p.part + (slot_row + row) * D + column) = x;
+              }
+            }
+            ok = meet();
+          }
+          if (!ok) break;
+        }
+      } else if (any) {
+        // Quad n of a warp writes 64 bytes of row 8 e + n.
         const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // NaN stays
         uint8_t* stage = smem + C::OUT_OFF + warp * 32 * kOutRow;
-        // Where this thread's quad writes: row 8 e + lane / 4 of the warp, or nowhere.
         uint8_t* to[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = 8 * e + (lane >> 2);
           const int64_t at = __shfl_sync(0xffffffffu, out_row, row);
           const bool row_live = __shfl_sync(0xffffffffu, static_cast<int>(live), row);
-          const bool row_here = __shfl_sync(0xffffffffu, static_cast<int>(here), row);
-          to[e] = done ? (row_here ? reinterpret_cast<uint8_t*>(p.o + at * D) : nullptr)
-                       : (row_live ? reinterpret_cast<uint8_t*>(p.part + (slot_row + row) * D) : nullptr);
+          to[e] = !row_live ? nullptr
+                  : done    ? reinterpret_cast<uint8_t*>(p.o + at * D)
+                            : reinterpret_cast<uint8_t*>(p.part + (slot_row + (warp & 3) * 32 + row) * D);
           if (to[e]) to[e] += (lane & 3) * 16;
         }
-#pragma unroll
+#pragma unroll 1
         for (int ch = 0; ch < D / 32; ++ch) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(o_addr + ch * 32, o);
@@ -758,7 +887,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           if (done) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              o[e] = live ? pack2<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv) : 0u;
+              o[e] = pack2<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
           }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {  // 16-bit: one half of 64 bytes; fp32: two
@@ -778,11 +907,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
               }
           }
         }
-        if (live && !done) p.part_ml[slot_row + lane] = make_float2(m == -INFINITY ? m : m * c, l);
-      } else if (done && here) {
-#pragma unroll
-        for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(p.o + out_row * D)[e] = make_uint4(0, 0, 0, 0);
+        if (live && !done) p.part_ml[slot_row + r] = make_float2(m == -INFINITY ? m : m * c, l);
       }
+      if (done && here && !live && group == 0)
+#pragma unroll 1
+        for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(p.o + out_row * D)[e] = make_uint4(0, 0, 0, 0);
       tc_fence_before();
     } while (w.next(p, block_tokens));
     if (!ok) give_up(ctl, NTL_STATUS_SOFTMAX_WAIT);
@@ -898,7 +1027,8 @@ int make_map(CUtensorMap* map, const char* what, const void* base, bool bf16, co
   for (int i = 0; i < 3; ++i) s[i] = dims[i + 1] == 1 ? 16 : static_cast<cuuint64_t>(strides[i]) * 2;
   CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                   const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  dims[0] == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return ntl_fail(NTL_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, int(r));
   return NTL_OK;
 }
@@ -945,11 +1075,11 @@ int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, Plan
   return NTL_OK;
 }
 
-template <int D, int NT, bool BF16>
+template <int D, int NT, int KS, bool BF16>
 int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                  const AttnParams& p, const Plan& n, cudaStream_t s) {
   static std::atomic<uint64_t> done_mask{0};
-  auto kernel = cache_attn_kernel<D, NT, BF16>;
+  auto kernel = cache_attn_kernel<D, NT, KS, BF16>;
   constexpr int smem = smem_bytes<D, NT>();
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "cudaGetDevice failed");
@@ -1026,17 +1156,22 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   for (int i = 3; i < 8; ++i)
     if (n.tile_keys == 1 << i) p.tile_shift = i;
   p.rows = n.rows;
-  p.min_tiles = 1;
   p.c = static_cast<float>(q->scale * 1.4426950408889634);
   p.wait_limit = ntl_wait_limit();
-#define NTL_CACHE_ATTN(D, NT) \
-  return bf16 ? launch_shape<D, NT, true>(what, mq, mk, mv, p, n, s) : launch_shape<D, NT, false>(what, mq, mk, mv, p, n, s)
+#define NTL_CACHE_ATTN(D, NT, KS)                                          \
+  return bf16 ? launch_shape<D, NT, KS, true>(what, mq, mk, mv, p, n, s) \
+              : launch_shape<D, NT, KS, false>(what, mq, mk, mv, p, n, s)
+  const int groups = n.row_tiles == 2 ? 0 : n.rows <= 32 ? 4 : n.rows <= 64 ? 2 : 1;
   if (dim == 64) {
-    if (n.row_tiles == 1) NTL_CACHE_ATTN(64, 1);
-    NTL_CACHE_ATTN(64, 2);
+    if (groups == 4) NTL_CACHE_ATTN(64, 1, 4);
+    if (groups == 2) NTL_CACHE_ATTN(64, 1, 2);
+    if (groups == 1) NTL_CACHE_ATTN(64, 1, 1);
+    NTL_CACHE_ATTN(64, 2, 1);
   }
-  if (n.row_tiles == 1) NTL_CACHE_ATTN(128, 1);
-  NTL_CACHE_ATTN(128, 2);
+  if (groups == 4) NTL_CACHE_ATTN(128, 1, 4);
+  if (groups == 2) NTL_CACHE_ATTN(128, 1, 2);
+  if (groups == 1) NTL_CACHE_ATTN(128, 1, 1);
+  NTL_CACHE_ATTN(128, 2, 1);
 #undef NTL_CACHE_ATTN
 }
 
