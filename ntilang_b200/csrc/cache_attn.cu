@@ -94,6 +94,7 @@ struct __align__(16) Ctl {
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t v_raw[4];    // a V tile with rows past the end has landed: v_full follows once they are cleared
   uint64_t s_full[2];   // S buffer holds scores
+  uint64_t p_half[2];   // NT = 2: row tile i's exponentials of the first 64 keys (4 warps)
   uint64_t p_ready[2];  // S buffer holds exponentials (4 warps)
   uint64_t pv_done[2];  // row tile i: P V of one more key tile is complete
   uint64_t drain;
@@ -331,6 +332,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+// Three-operand max that returns NaN when an operand is NaN.
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // The x low bits of 64 (none for x <= 0, all for x >= 64).
 __device__ __forceinline__ uint64_t low_bits(int x) {
   return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1;
@@ -394,6 +402,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->s_full[i], 1);
+      mbar_init(&ctl->p_half[i], 4);
       mbar_init(&ctl->p_ready[i], 4);
       mbar_init(&ctl->pv_done[i], 1);
     }
@@ -422,8 +431,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
     return;
   }
   const uint32_t tmem = ctl->tmem_base;
-  Walk w;
-  w.begin(ctl);
 
   if (warp >= C::SOFTMAX_WARPS) {
     if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS_OTHER) : "memory");
@@ -441,6 +448,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       const int box_bytes = box_keys * 128;  // one page's rows of one 64-column half
       const uint32_t tile_bytes = static_cast<uint32_t>(boxes * box_bytes * (D / 64));
       bool ok = true;
+      Walk w;
+      w.begin(ctl);
       int issued = 0;
       uint32_t raw = 0, cleared = 0;  // bit s: parity of the next v_raw[s]; stage s's last tile is one to clear
       do {
@@ -492,6 +501,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       // ---------------------------------------------- Q loads, and value rows past the end become zeros
       const uint32_t q_bytes = static_cast<uint32_t>(NT * KS * (D / 64) * p.tile_tokens * p.group * 128);
       bool ok = true;
+      Walk w;
+      w.begin(ctl);
       int n = 0, g = 0;
       uint32_t raw = 0;  // bit s: parity of v_raw[s]
       do {
@@ -547,7 +558,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
         return false;
       };
       // Two cursors over the same tiles: Q K^T runs one tile ahead of P V.
-      Walk wq = w;
+      Walk w, wq;
+      w.begin(ctl);
+      wq.begin(ctl);
       int gq = 0, aq = wq.a0, uq = 0;
       bool more = true;
       auto qk_ready = [&]() -> bool {
@@ -587,42 +600,40 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       while (left) {
         for (int a = w.a0; a < w.a1 && ok; ++a, ++g) {
           const int s = g % ST;
-          auto pv = [&](int i) -> bool {  // O_i += P V
+          auto pv = [&](int i) -> bool {  // O_i += P V; NT = 2 starts on the first half of the keys
             const int buf = NT == 2 ? i : g & 1;
-            if (!wait(&ctl->p_ready[buf], (NT == 2 ? g : g >> 1) & 1)) return false;
-            tc_fence_after();
             const uint32_t v = v_low + s * (C::KV_BYTES >> 4);
+            constexpr int HALVES = NT;
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)
-              tc_mma_f16_ts(tmem + C::O_COL(i), tmem + C::S_COL(buf) + kk * 8, desc_at(v, kk * 2048), idesc_o,
-                            (a > w.a0 || kk > 0) ? 1u : 0u);
+            for (int half = 0; half < HALVES; ++half) {
+              if (!wait(half + 1 < HALVES ? &ctl->p_half[buf] : &ctl->p_ready[buf], (NT == 2 ? g : g >> 1) & 1)) return false;
+              tc_fence_after();
+#pragma unroll
+              for (int kk = half * (BN / 16 / HALVES); kk < (half + 1) * (BN / 16 / HALVES); ++kk)
+                tc_mma_f16_ts(tmem + C::O_COL(i), tmem + C::S_COL(buf) + kk * 8, desc_at(v, kk * 2048), idesc_o,
+                              (a > w.a0 || kk > 0) ? 1u : 0u);
+            }
             tc_commit(&ctl->pv_done[i]);
             return true;
           };
+          // The next tile's Q K^T goes out before this tile's P V is done, to run during the softmax; a new
+          // unit's waits for loads that the end of this unit must not wait for, and goes last.
+          bool late = false;
           if constexpr (NT == 1) {
-            // The next tile's Q K^T goes first, to run during the softmax; a new unit's waits for loads
-            // that the end of this unit must not wait for, and goes second.
-            const bool ahead = more, other = aq == wq.a0;
-            if (ahead && !other) {
+            if (more && aq != wq.a0) {
               if (!(ok = qk_ready())) break;
               qk(0);
               qk_end();
+            } else {
+              late = more;
             }
             if (!(ok = wait(&ctl->v_full[s], (g / ST) & 1) && pv(0))) break;
-            if (ahead && other) {
-              tc_commit(&ctl->v_empty[s]);
-              if (!(ok = qk_ready())) break;
-              qk(0);
-              qk_end();
-              continue;
-            }
           } else {
-            if (!(ok = wait(&ctl->v_full[s], (g / ST) & 1) && pv(0))) break;
-            const bool ahead = more;
-            if (ahead) {
-              if (!(ok = qk_ready())) break;
-              qk(0);
-            }
+            const bool ahead = more && aq != wq.a0;
+            late = more && !ahead;
+            // K of the next tile has landed long before P is ready: only P is on the critical path.
+            if (!(ok = wait(&ctl->v_full[s], (g / ST) & 1) && (!ahead || qk_ready()) && pv(0))) break;
+            if (ahead) qk(0);
             if (!(ok = pv(1))) break;
             if (ahead) {
               qk(1);
@@ -630,6 +641,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
             }
           }
           tc_commit(&ctl->v_empty[s]);
+          if (late) {
+            if (!(ok = qk_ready())) break;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) qk(i);
+            qk_end();
+          }
         }
         left = ok && w.next(p, block_tokens);
       }
@@ -653,6 +670,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
     const float c = p.c;
     int4 cut = make_int4(0, 0, -1, 0);
     bool ok = true;
+    Walk w;
+    w.begin(ctl);
     int g = 0;
     uint32_t merges = 0;
     // The four warps meet (key groups only): false when one of them gave up.
@@ -666,9 +685,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       const int t = u.t0 + t_in_block;
       const bool live = in_tile && t < u.live;
       const bool any = KS > 1 ? u.t0 < u.live : __any_sync(0xffffffffu, live);
-      const bool here = in_tile && t < p.tokens;  // the output has this row
-      const int64_t out_row =
-          (static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + w.kv_head * p.group + row_head;
       // Keys that every row of this row tile sees: [0, all_hi), or for the window [all_lo, all_hi)
       // and the sinks.
       const int prefix = u.len - u.live;
@@ -679,6 +695,18 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       for (int a = w.a0; a < w.a1; ++a, ++g) {
         const int buf = NT == 2 ? i : g & 1;
         const uint32_t s_addr = tmem + lane_off + C::S_COL(buf);
+        // What the row sees of this tile, worked out while S is on its way.
+        const int k0 = tile_key(p, u, a);
+        const bool whole = p.tile_keys == BN && k0 + BN <= all_hi && (k0 >= all_lo || k0 + BN <= p.sinks);
+        constexpr int WORDS = (KC + 63) / 64;
+        uint64_t see[WORDS];
+        if (any && !whole) {
+#pragma unroll
+          for (int ch = 0; ch < WORDS; ++ch) {
+            see[ch] = live ? visible(p, u, t, k0 + ch * 64) & low_bits(p.tile_keys - ch * 64) : 0;
+            if constexpr (KS > 1) see[ch] >>= group * KC;
+          }
+        }
         if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g >> 1) & 1, p.wait_limit, abort_flag))) break;
         if (any) {
           tc_fence_after();
@@ -691,33 +719,30 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
               tmem_ld_32x32b_x32(s_addr + group * KC + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + ch * 32));
           }
           tc_wait_ld();
-          const int k0 = tile_key(p, u, a);
-          const bool whole = p.tile_keys == BN && k0 + BN <= all_hi && (k0 >= all_lo || k0 + BN <= p.sinks);
           if (!whole) {
 #pragma unroll
-            for (int ch = 0; ch < (KC + 63) / 64; ++ch) {
-              uint64_t see = live ? visible(p, u, t, k0 + ch * 64) & low_bits(p.tile_keys - ch * 64) : 0;
-              if constexpr (KS > 1) see >>= group * KC;
+            for (int ch = 0; ch < WORDS; ++ch)
 #pragma unroll
               for (int e = 0; e < (KC < 64 ? KC : 64); ++e)
-                if (!(see >> e & 1)) sv[ch * 64 + e] = __float_as_uint(-INFINITY);
-            }
+                if (!(see[ch] >> e & 1)) sv[ch * 64 + e] = __float_as_uint(-INFINITY);
           }
           float top;
           {
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int e = 0; e < KC; e += 8) {
-              x[0] = fmax3(x[0], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
-              x[1] = fmax3(x[1], __uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3]));
-              x[2] = fmax3(x[2], __uint_as_float(sv[e + 4]), __uint_as_float(sv[e + 5]));
-              x[3] = fmax3(x[3], __uint_as_float(sv[e + 6]), __uint_as_float(sv[e + 7]));
+              x[0] = fmax3_nan(x[0], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+              x[1] = fmax3_nan(x[1], __uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3]));
+              x[2] = fmax3_nan(x[2], __uint_as_float(sv[e + 4]), __uint_as_float(sv[e + 5]));
+              x[3] = fmax3_nan(x[3], __uint_as_float(sv[e + 6]), __uint_as_float(sv[e + 7]));
             }
-            top = fmax3(fmaxf(x[0], x[1]), x[2], x[3]);
+            top = fmax3_nan(fmax3_nan(x[0], x[1], x[2]), x[3], x[3]);
           }
           float scale_old = 1.0f;
           bool moved = false;
-          if (m == -INFINITY) {
+          if (!(top < INFINITY)) {  // a NaN or +inf score: the row's softmax is NaN
+            l = __uint_as_float(0x7fffffffu);
+          } else if (m == -INFINITY) {
             m = top;  // nothing seen so far: o and l are zero (or not begun)
           } else if (live && (top - m) * c > kRescaleLog2) {
             scale_old = ex2_approx((m - top) * c);
@@ -756,9 +781,16 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
 #pragma unroll
             for (int e = 0; e < PC; ++e) {
               const int k = ch * 2 * PC + 2 * e;
-              float x0, x1;
-              f2_split(f2_fma(f2_make(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), c2, shift2), x0, x1);
-              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              const uint64_t x2 = f2_fma(f2_make(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), c2, shift2);
+              float p0, p1;
+              if (KS == 1 && (e & 3) == 3) {  // one pair in four on the FMA pipe
+                exp2_fma2(x2, p0, p1);
+              } else {
+                float x0, x1;
+                f2_split(x2, x0, x1);
+                p0 = ex2_approx(x0);
+                p1 = ex2_approx(x1);
+              }
               acc[e & 1] = f2_add(acc[e & 1], f2_make(p0, p1));
               packed[e] = pack2<BF16>(p0, p1);
             }
@@ -766,6 +798,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
               tmem_st_32x32b_x8(s_addr + group * (KC / 2) + ch * PC, packed);
             } else {
               tmem_st_32x32b_x16(s_addr + group * (KC / 2) + ch * PC, packed);
+            }
+            if (NT == 2 && ch == KC / (4 * PC) - 1) {  // the first half of the keys may be multiplied
+              tc_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&ctl->p_half[buf]);
             }
           }
           if constexpr (KS > 1) {
@@ -789,11 +827,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           tc_fence_before();
           __syncwarp();
         }
+        if (NT == 2 && !any && lane == 0) mbar_arrive(&ctl->p_half[buf]);
         if (lane == 0) mbar_arrive(&ctl->p_ready[buf]);
       }
+      // A row that saw nothing: hidden scores may have left ~1e-38 each (exp2_fma2).
+      if (m == -INFINITY && l == l) l = 0.0f;
       if (!ok || (any && !(ok = warp_wait(&ctl->pv_done[i], (g - 1) & 1, p.wait_limit, abort_flag)))) break;
       tc_fence_after();
       const bool done = w.a0 == 0 && w.a1 == u.tiles;
+      const bool here = in_tile && t < p.tokens;  // the output has this row
+      const int64_t out_row =
+          (static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + w.kv_head * p.group + row_head;
       if (!done && w.a0 == 0 && threadIdx.x == 0) {
         const int total = ctl->start[4];
         const int unit_start = piece_start(blockIdx.x + 1, total, ctas) - w.a1;
