@@ -685,30 +685,32 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       const int t = u.t0 + t_in_block;
       const bool live = in_tile && t < u.live;
       const bool any = KS > 1 ? u.t0 < u.live : __any_sync(0xffffffffu, live);
-      // Keys that every row of this row tile sees: [0, all_hi), or for the window [all_lo, all_hi)
-      // and the sinks.
-      const int prefix = u.len - u.live;
-      const int t_first = u.t0 + i * p.tile_tokens, t_last = min(t_first + p.tile_tokens, u.live) - 1;
-      const int all_hi = p.tree ? prefix : prefix + t_first + 1;
-      const int all_lo = p.tree ? 0 : prefix + t_last - p.window + 1;
+      // Tiles that every row of this row tile sees whole: [whole_from, whole_to).  (Tiles of sinks alone
+      // are left to the masked path.)
+      int whole_from = 0, whole_to = 0;
+      if (p.tile_keys == BN) {
+        const int prefix = u.len - u.live;
+        const int t_first = u.t0 + i * p.tile_tokens, t_last = min(t_first + p.tile_tokens, u.live) - 1;
+        const int all_lo = p.tree ? 0 : max(prefix + t_last - p.window + 1, 0);
+        const int all_hi = p.tree ? prefix : prefix + t_first + 1;
+        whole_from = u.sink_tiles + max((all_lo + BN - 1) / BN - u.first, 0);
+        whole_to = u.sink_tiles + all_hi / BN - u.first;
+      }
       float m = -INFINITY, l = 0.0f;
-      for (int a = w.a0; a < w.a1; ++a, ++g) {
-        const int buf = NT == 2 ? i : g & 1;
-        const uint32_t s_addr = tmem + lane_off + C::S_COL(buf);
-        // What the row sees of this tile, worked out while S is on its way.
-        const int k0 = tile_key(p, u, a);
-        const bool whole = p.tile_keys == BN && k0 + BN <= all_hi && (k0 >= all_lo || k0 + BN <= p.sinks);
-        constexpr int WORDS = (KC + 63) / 64;
-        uint64_t see[WORDS];
-        if (any && !whole) {
-#pragma unroll
-          for (int ch = 0; ch < WORDS; ++ch) {
-            see[ch] = live ? visible(p, u, t, k0 + ch * 64) & low_bits(p.tile_keys - ch * 64) : 0;
-            if constexpr (KS > 1) see[ch] >>= group * KC;
+      if (!any) {  // rows past the end: this warp only keeps step
+        for (int a = w.a0; a < w.a1; ++a, ++g) {
+          const int buf = NT == 2 ? i : g & 1;
+          if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g >> 1) & 1, p.wait_limit, abort_flag))) break;
+          if (lane == 0) {
+            if (NT == 2) mbar_arrive(&ctl->p_half[buf]);
+            mbar_arrive(&ctl->p_ready[buf]);
           }
         }
-        if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g >> 1) & 1, p.wait_limit, abort_flag))) break;
-        if (any) {
+      } else {
+        for (int a = w.a0; a < w.a1; ++a, ++g) {
+          const int buf = NT == 2 ? i : g & 1;
+          const uint32_t s_addr = tmem + lane_off + C::S_COL(buf);
+          if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g >> 1) & 1, p.wait_limit, abort_flag))) break;
           tc_fence_after();
           uint32_t sv[KC];
           if constexpr (KC == 16) {
@@ -719,12 +721,16 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
               tmem_ld_32x32b_x32(s_addr + group * KC + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + ch * 32));
           }
           tc_wait_ld();
-          if (!whole) {
+          if (__builtin_expect(a < whole_from || a >= whole_to, 0)) {
+            const int k0 = tile_key(p, u, a);
 #pragma unroll
-            for (int ch = 0; ch < WORDS; ++ch)
+            for (int ch = 0; ch < (KC + 63) / 64; ++ch) {
+              uint64_t see = live ? visible(p, u, t, k0 + ch * 64) & low_bits(p.tile_keys - ch * 64) : 0;
+              if constexpr (KS > 1) see >>= group * KC;
 #pragma unroll
               for (int e = 0; e < (KC < 64 ? KC : 64); ++e)
-                if (!(see[ch] >> e & 1)) sv[ch * 64 + e] = __float_as_uint(-INFINITY);
+                if (!(see >> e & 1)) sv[ch * 64 + e] = __float_as_uint(-INFINITY);
+            }
           }
           float top;
           {
@@ -742,7 +748,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           bool moved = false;
           if (!(top < INFINITY)) {  // a NaN or +inf score: the row's softmax is NaN
             l = __uint_as_float(0x7fffffffu);
-          } else if (m == -INFINITY) {
+            top = m;
+          }
+          if (m == -INFINITY) {
             m = top;  // nothing seen so far: o and l are zero (or not begun)
           } else if (live && (top - m) * c > kRescaleLog2) {
             scale_old = ex2_approx((m - top) * c);
@@ -754,10 +762,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           // where o is about to change, and on the unit's last tile: before this warp hands over P,
           // pv_done is at most one phase behind, so the wait after it is not a phase early.
           // (NT = 2 issued S after that P V: it is complete.)
-          if (NT == 1 && g > 0 && (rescale || a + 1 == w.a1) &&
+          if (NT == 1 && g > 0 && __builtin_expect(rescale || a + 1 == w.a1, 0) &&
               !(ok = warp_wait(&ctl->pv_done[0], (g - 1) & 1, p.wait_limit, abort_flag)))
             break;
-          if (rescale) {
+          if (__builtin_expect(rescale, 0)) {
             tc_fence_after();
 #pragma unroll 1
             for (int ch = 0; ch < D / 32; ++ch) {
@@ -826,9 +834,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->p_ready[buf]);
         }
-        if (NT == 2 && !any && lane == 0) mbar_arrive(&ctl->p_half[buf]);
-        if (lane == 0) mbar_arrive(&ctl->p_ready[buf]);
       }
       // A row that saw nothing: hidden scores may have left ~1e-38 each (exp2_fma2).
       if (m == -INFINITY && l == l) l = 0.0f;
