@@ -50,7 +50,7 @@ struct AttnParams {
   const uint32_t* tree;   // null: window
   float* part;            // workspace: [2 * ctas][rows][D] values, then [2 * ctas][rows] (m, l)
   float2* part_ml;
-  int4* head;             // [ctas] the unit a CTA begins and does not end: {item, key head, last CTA, -}
+  int4* head;             // [ctas] the unit a CTA begins and does not end: {item, key head, last CTA, new tokens}
   int64_t table_stride, tree_stride;
   int seqs, tokens, heads, kv_heads, group, pages, page_size, max_pages, words, window, sinks;
   int tile_tokens;   // tokens per 128-row tile
@@ -421,6 +421,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
     }
     fence_proxy_async_smem();
   }
+  pdl_wait();
   const int ctas = find_piece(p, ctl, block_tokens);
   tc_fence_before();
   __syncthreads();
@@ -789,16 +790,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
 #pragma unroll
             for (int e = 0; e < PC; ++e) {
               const int k = ch * 2 * PC + 2 * e;
-              const uint64_t x2 = f2_fma(f2_make(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), c2, shift2);
-              float p0, p1;
-              if (KS == 1 && (e & 3) == 3) {  // one pair in four on the FMA pipe
-                exp2_fma2(x2, p0, p1);
-              } else {
-                float x0, x1;
-                f2_split(x2, x0, x1);
-                p0 = ex2_approx(x0);
-                p1 = ex2_approx(x1);
-              }
+              float x0, x1;
+              f2_split(f2_fma(f2_make(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), c2, shift2), x0, x1);
+              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
               acc[e & 1] = f2_add(acc[e & 1], f2_make(p0, p1));
               packed[e] = pack2<BF16>(p0, p1);
             }
@@ -837,8 +831,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           if (lane == 0) mbar_arrive(&ctl->p_ready[buf]);
         }
       }
-      // A row that saw nothing: hidden scores may have left ~1e-38 each (exp2_fma2).
-      if (m == -INFINITY && l == l) l = 0.0f;
       if (!ok || (any && !(ok = warp_wait(&ctl->pv_done[i], (g - 1) & 1, p.wait_limit, abort_flag)))) break;
       tc_fence_after();
       const bool done = w.a0 == 0 && w.a1 == u.tiles;
@@ -848,7 +840,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       if (!done && w.a0 == 0 && threadIdx.x == 0) {
         const int total = ctl->start[4];
         const int unit_start = piece_start(blockIdx.x + 1, total, ctas) - w.a1;
-        cut = make_int4(w.item, w.kv_head, piece_of(unit_start + u.tiles - 1, total, ctas), 0);
+        cut = make_int4(w.item, w.kv_head, piece_of(unit_start + u.tiles - 1, total, ctas), u.live);
       }
       // Rows leave through shared memory, so that store instructions write whole sectors (a thread writing
       // its own row 16 bytes at a time took 5 to 9 us per 108 rows).
@@ -976,71 +968,96 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
 }
 
 // Adds up the parts of the unit that CTA blockIdx.x of the attention kernel began and did not end, in
-// CTA order: weights 2^(m_s - max m), o = sum w_s o_s / sum w_s l_s.  One warp per row; the lanes
-// hold 32 parts' (m, l) at a time and the parts' values are read kJoinUnroll at a time, so a row costs
-// a few memory latencies and not one per part (one part after another: 10 to 24 us per call for 16 to 37
-// parts, against 4 to 7 us).
-constexpr int kJoinWarps = 4, kJoinUnroll = 8;
+// CTA order: weights 2^(m_s - max m), o = sum w_s o_s / sum w_s l_s.  A warp takes R rows: its lanes hold
+// (m, l) of R rows x 32 / R parts, and 16 rows and parts of values are in flight at a time, so a warp
+// costs a few memory latencies and not one per part and row.  R = 4 for units of over 64 rows (which
+// few CTAs share: 27 -> 11 us for 147 cuts of 256 rows), 1 for the others (few rows, many parts).
+constexpr int kJoinWarps = 4;
 
-template <int D, bool BF16>
+template <int D, int R, bool BF16>
 __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const AttnParams p, int row_tiles) {
+  constexpr int kJoinRows = R, kJoinParts = 32 / R, kJoinAhead = 16 / R;
+  constexpr int E = D / 32;
+  using Vec = typename std::conditional<E == 4, float4, float2>::type;
   pdl_wait();
   const int4 cut = p.head[blockIdx.x];
   if (cut.z < 0) return;
-  const int first = blockIdx.x, last = cut.z;
-  const int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int r = row % BM, token = r / p.group;
-  if (row >= p.rows || token >= p.tile_tokens) return;
-  const Unit u = unit_of(p, cut.x, row_tiles * p.tile_tokens);
-  const int t = u.t0 + (row / BM) * p.tile_tokens + token;
-  if (t >= p.tokens) return;
-  constexpr int E = D / 32;
-  using Vec = typename std::conditional<E == 4, float4, float2>::type;
-  // Part s of the unit: CTA first's second slot, then the first slots of those after it.
-  auto at = [&](int s) { return (2ll * s + (s == first)) * p.rows + row; };
-  float o[E] = {}, m = -INFINITY, l = 0.0f;
-  if (t < u.live) {
-    for (int s0 = first; s0 <= last; s0 += 32) {
-      const float2 ml = s0 + lane <= last ? p.part_ml[at(s0 + lane)] : make_float2(-INFINITY, 0.0f);
-      float top = fmaxf(m, ml.x);
+  const int first = blockIdx.x, parts = cut.z - first + 1;
+  const int row0 = (blockIdx.y * kJoinWarps + (threadIdx.x >> 5)) * kJoinRows, lane = threadIdx.x & 31;
+  if (row0 >= p.rows) return;
+  const int b = cut.x / p.blocks, t0 = (cut.x - b * p.blocks) * row_tiles * p.tile_tokens, live = cut.w;
+  // Part s of the unit: CTA first's second slot, then the first slots of the CTAs after it.
+  auto at = [&](int s, int row) { return (2ll * (first + s) + (s == 0)) * p.rows + row; };
+  // Token of a row within the sequence, past every token if the tile has no such row.
+  auto token_of = [&](int row) {
+    const int r = row % BM, t = r / p.group;
+    return t < p.tile_tokens && row < p.rows ? t0 + (row / BM) * p.tile_tokens + t : p.tokens;
+  };
+  int t[kJoinRows];
 #pragma unroll
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const float old = m == -INFINITY ? 0.0f : ex2_approx(m - top);
-      // A part that saw nothing has m = -inf and l = 0 (or NaN scores: l NaN).
-      const float weight = ml.x == -INFINITY ? (ml.y == ml.y ? 0.0f : ml.y) : ex2_approx(ml.x - top);
-      float sum = weight * ml.y;
+  for (int i = 0; i < kJoinRows; ++i) t[i] = token_of(row0 + i);
+  float o[kJoinRows][E] = {}, m = -INFINITY, l = 0.0f;  // (m, l) of row lane / 8
+  const int mine = row0 + lane / kJoinParts;
+  for (int s0 = 0; s0 < parts; s0 += kJoinParts) {
+    const int s = s0 + lane % kJoinParts;
+    const float2 ml = s < parts && token_of(mine) < live ? p.part_ml[at(s, mine)] : make_float2(-INFINITY, 0.0f);
+    float v[kJoinAhead][kJoinRows][E];
+    auto fetch = [&](int j0) {
 #pragma unroll
-      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      l = l * old + sum;
-      m = top;
+      for (int j = 0; j < kJoinAhead; ++j)
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] *= old;
-      const int n = min(32, last - s0 + 1);
-      for (int j0 = 0; j0 < n; j0 += kJoinUnroll) {
-        float v[kJoinUnroll][E];
+        for (int i = 0; i < kJoinRows; ++i)
+          if (s0 + j0 + j < parts && t[i] < live)
+            *reinterpret_cast<Vec*>(v[j][i]) =
+                *reinterpret_cast<const Vec*>(p.part + at(s0 + j0 + j, row0 + i) * D + lane * E);
+    };
+    fetch(0);
+    float top = fmaxf(m, ml.x);
 #pragma unroll
-        for (int j = 0; j < kJoinUnroll; ++j)
-          if (j0 + j < n)
-            *reinterpret_cast<Vec*>(v[j]) = *reinterpret_cast<const Vec*>(p.part + at(s0 + j0 + j) * D + lane * E);
+    for (int d = kJoinParts / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float old = m == -INFINITY ? 0.0f : ex2_approx(m - top);
+    // A part that saw nothing has m = -inf and l = 0 (or NaN scores: l NaN).
+    const float weight = ml.x == -INFINITY ? (ml.y == ml.y ? 0.0f : ml.y) : ex2_approx(ml.x - top);
+    float sum = weight * ml.y;
 #pragma unroll
-        for (int j = 0; j < kJoinUnroll; ++j) {
-          const float wgt = __shfl_sync(0xffffffffu, weight, (j0 + j) & 31);
-          if (j0 + j < n)
+    for (int d = kJoinParts / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    l = l * old + sum;
+    m = top;
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += wgt * v[j][e];
+    for (int i = 0; i < kJoinRows; ++i) {
+      const float scale = __shfl_sync(0xffffffffu, old, i * kJoinParts);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[i][e] *= scale;
+    }
+    const int n = min(kJoinParts, parts - s0);
+    for (int j0 = 0; j0 < n; j0 += kJoinAhead) {
+      if (j0 > 0) fetch(j0);
+#pragma unroll
+      for (int j = 0; j < kJoinAhead; ++j)
+#pragma unroll
+        for (int i = 0; i < kJoinRows; ++i) {
+          const float w = __shfl_sync(0xffffffffu, weight, i * kJoinParts + ((j0 + j) & (kJoinParts - 1)));
+          if (j0 + j < n && t[i] < live)
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[i][e] += w * v[j][i][e];
         }
-      }
     }
   }
   const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
-  uint32_t h[E / 2];
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) h[e] = pack2<BF16>(o[2 * e] * inv, o[2 * e + 1] * inv);
-  uint16_t* out = p.o + ((static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + cut.y * p.group + r % p.group) * D + lane * E;
-  if constexpr (E == 4) {
-    *reinterpret_cast<uint2*>(out) = make_uint2(h[0], h[1]);
-  } else {
-    *reinterpret_cast<uint32_t*>(out) = h[0];
+  for (int i = 0; i < kJoinRows; ++i) {
+    const float scale = __shfl_sync(0xffffffffu, inv, i * kJoinParts);
+    if (t[i] >= p.tokens) continue;
+    uint32_t h[E / 2];
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) h[e] = pack2<BF16>(o[i][2 * e] * scale, o[i][2 * e + 1] * scale);
+    const int head = cut.y * p.group + (row0 + i) % BM % p.group;
+    uint16_t* out = p.o + ((static_cast<int64_t>(b) * p.tokens + t[i]) * p.heads + head) * D + lane * E;
+    if constexpr (E == 4) {
+      *reinterpret_cast<uint2*>(out) = make_uint2(h[0], h[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(out) = h[0];
+    }
   }
 }
 
@@ -1146,13 +1163,15 @@ int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk,
                       fa.numRegs, REGS_LAUNCH);
     done_mask.fetch_or(bit, std::memory_order_release);
   }
-  kernel<<<n.ctas, Shape<D, NT>::THREADS, smem, s>>>(mq, mk, mv, p);
+  cudaError_t e = ntl_launch_pdl(kernel, dim3(n.ctas), dim3(Shape<D, NT>::THREADS), smem, s, mq, mk, mv, p);
+  if (e != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   ntl_note_launch();
   if (int rc = ntl_check_launch(what)) return rc;
   if (n.ctas == 1) return NTL_OK;  // one piece: no unit is cut
-  const unsigned chunks = static_cast<unsigned>((n.rows + kJoinWarps - 1) / kJoinWarps);
-  cudaError_t e =
-      ntl_launch_pdl(cache_attn_join<D, BF16>, dim3(n.ctas - 1, chunks), dim3(kJoinWarps * 32), 0, s, p, NT);
+  const int join_rows = n.rows > 64 ? 4 : 1;
+  const unsigned chunks = static_cast<unsigned>((n.rows + kJoinWarps * join_rows - 1) / (kJoinWarps * join_rows));
+  e = ntl_launch_pdl(join_rows == 4 ? cache_attn_join<D, 4, BF16> : cache_attn_join<D, 1, BF16>,
+                     dim3(n.ctas - 1, chunks), dim3(kJoinWarps * 32), 0, s, p, NT);
   if (e != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   ntl_note_launch();
   return ntl_check_launch(what);
@@ -1212,15 +1231,13 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
 #define NTL_CACHE_ATTN(D, NT, KS)                                          \
   return bf16 ? launch_shape<D, NT, KS, true>(what, mq, mk, mv, p, n, s) \
               : launch_shape<D, NT, KS, false>(what, mq, mk, mv, p, n, s)
-  const int groups = n.row_tiles == 2 ? 0 : n.rows <= 32 ? 4 : n.rows <= 64 ? 2 : 1;
+  const int groups = n.row_tiles == 2 ? 0 : n.rows <= 32 ? 4 : 1;
   if (dim == 64) {
     if (groups == 4) NTL_CACHE_ATTN(64, 1, 4);
-    if (groups == 2) NTL_CACHE_ATTN(64, 1, 2);
     if (groups == 1) NTL_CACHE_ATTN(64, 1, 1);
     NTL_CACHE_ATTN(64, 2, 1);
   }
   if (groups == 4) NTL_CACHE_ATTN(128, 1, 4);
-  if (groups == 2) NTL_CACHE_ATTN(128, 1, 2);
   if (groups == 1) NTL_CACHE_ATTN(128, 1, 1);
   NTL_CACHE_ATTN(128, 2, 1);
 #undef NTL_CACHE_ATTN

@@ -105,6 +105,36 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// 2^x on the FMA pipe, for x <= ~8 (softmax exponents): x = n + f with n = round(x) via
+// the 1.5*2^23 rounding constant, 2^f on [-1/2, 1/2] by a cubic fitted here for minimum
+// relative error (max 7.6e-5, below fp16's half-ulp 2.4e-4 that P is rounded to), and
+// 2^n added to the exponent bits.  x is clamped at -126 so the exponent never underflows;
+// such terms (masked or tiny scores) become ~1e-38, i.e. 0 in fp16 P.  Used for a fixed
+// quarter of the exponentials so the MUFU ex2 unit and the FMA pipe share the load.
+// Two values per call, with f32x2 arithmetic.  The method is additive range reduction
+// (W. J. Cody and W. Waite, "Software Manual for the Elementary Functions", 1980) with the
+// result's exponent written straight into the float's bits (N. N. Schraudolph, "A Fast,
+// Compact Approximation of the Exponential Function", Neural Computation 11(4), 1999); the
+// cubic's coefficients were fitted for this kernel.
+__device__ __forceinline__ void exp2_fma2(uint64_t x2, float& p0, float& p1) {
+  constexpr float kRound = 12582912.0f;
+  float x0, x1;
+  f2_split(x2, x0, x1);
+  x2 = f2_make(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+  const uint64_t round2 = f2_make(kRound, kRound);
+  const uint64_t t2 = f2_add(x2, round2);
+  const uint64_t f2 = f2_sub(x2, f2_sub(t2, round2));
+  uint64_t q2 = f2_fma(f2_make(0.055170975625514984f, 0.055170975625514984f), f2,
+                       f2_make(0.24260970950126648f, 0.24260970950126648f));
+  q2 = f2_fma(q2, f2, f2_make(0.6932609677314758f, 0.6932609677314758f));
+  q2 = f2_fma(q2, f2, f2_make(0.9999281764030457f, 0.9999281764030457f));
+  float q0, q1, t0, t1;
+  f2_split(q2, q0, q1);
+  f2_split(t2, t0, t1);
+  p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
+  p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
+}
+
 // Number of KV tiles query tile i of block qb needs (0 when the tile is past S).
 __device__ __forceinline__ int kv_tiles(const Fa2Params& p, int q0_tile) {
   if (q0_tile >= p.S) return 0;
