@@ -16,15 +16,21 @@
 // pieces leaves (o, m, l) parts in the workspace that cache_attn_join adds up in order.  So ragged
 // lengths balance by themselves, from lengths that only the device knows.
 //
-// Two shapes of CTA, chosen by the rows a unit has (see launch()):
-//   NT = 1: one 128-row tile, 64-key tiles, two CTAs per SM (one loads and multiplies while the other
-//           is in its softmax or between units).  For up to 128 rows: decode and small trees, bound by
-//           HBM.  S is double-buffered, so Q K^T of the next tile runs during the softmax.
-//   NT = 2: two 128-row tiles that share every K and V tile, 128-key tiles, one CTA per SM.  For wide
-//           trees and prompt chunks, bound by the tensor cores and the exponentials.
-// Warps: 4 per row tile for the softmax (one thread per row = TMEM lane; the same thread rescales
-// and writes out the row), then one each for MMA issue, K loads, V loads, and for Q loads and clearing value
-// rows past the sequence's end (a page's unwritten rows may hold NaN, and 0 * NaN is not 0).
+// Two shapes of CTA (one per SM), chosen by the rows a unit has (see launch()).  Both run two softmax
+// streams of four warps, so that one stream's tensor work overlaps the other's exponentials:
+//   NT = 1: one 128-row tile; the streams take alternate key tiles of the same rows, each with its own
+//           (o, m, l), and merge at the unit's end.  For up to 128 rows: decode and small trees, bound by
+//           HBM.  Up to 32 rows are copied to four lane groups that take a quarter of each key tile each.
+//           Tiles are 64 keys with four S buffers at head_dim 128 (3 to 6% faster than 128 keys, whose ring is
+//           only 2 + 3 tiles deep) and 128 keys with three at head_dim 64 (64 keys: 13% slower, each
+//           Q K^T reads all of Q from shared memory, however few keys it covers).
+//   NT = 2: two 128-row tiles that share every K and V tile of 128 keys; a stream is a row tile.  For
+//           wide trees and prompt chunks, bound by the tensor cores and the exponentials.
+// Warps: 8 softmax (one thread per row = TMEM lane; the same thread rescales and writes out the row),
+// one for K loads, one for V loads, and two that issue MMAs, load Q and clear value rows past the
+// sequence's end (a page's unwritten rows may hold NaN, and 0 * NaN is not 0): NT = 1 has Q and Q K^T in one,
+// clearing and P V in the other (one thread for both products waited for P while K had landed: 5% slower
+// decode); NT = 2 all MMAs in one, Q and clearing in the other.
 // Every wait is bounded: one that gives up records a status code, and the CTA drains its copies
 // and MMAs, frees TMEM and returns.
 #include <atomic>
@@ -57,30 +63,36 @@ struct AttnParams {
   int blocks;        // token blocks per sequence (units of NT tiles)
   int tile_keys;     // keys per tile: whole pages, or a divisor of a page
   int tile_pages;    // pages per tile (1 where a page holds several tiles)
-  int tile_shift;    // log2 of tile_keys, -1 if it is no power of two
+  int page_shift;    // log2 of page_size, -1 if it is no power of two
+  int tile_shift;    // log2 of tile_keys, the same
   int rows;          // rows a workspace slot has
   float c;           // softmax scale in log2 units
   int64_t wait_limit;
 };
 
+constexpr int SOFTMAX_WARPS = 8, MMA_WARP = 8, K_WARP = 9, V_WARP = 10, AUX_WARP = 11, THREADS = 384;
+// Register split: the launch's registers per thread, what the softmax warps take, what the others keep.
+constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 200, REGS_OTHER = 104;
+static_assert(8 * REGS_SOFTMAX + 4 * REGS_OTHER == 12 * REGS_LAUNCH, "register split must match the launch");
+constexpr int kMaxStages = 6;
+constexpr uint32_t TMEM_COLS = 512;
+
 template <int D, int NT>
 struct Shape {
-  static constexpr int BN = NT == 1 ? 64 : 128;  // keys per tile
-  static constexpr int STAGES = D == 64 ? 4 : 2;  // of K and of V
-  static constexpr int SOFTMAX_WARPS = 4 * NT;
-  static constexpr int MMA_WARP = SOFTMAX_WARPS, K_WARP = MMA_WARP + 1, V_WARP = MMA_WARP + 2, AUX_WARP = MMA_WARP + 3;
-  static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);
-  static constexpr int CTAS_PER_SM = NT == 1 ? 2 : 1;
+  static constexpr int BN = NT == 1 && D == 128 ? 64 : 128;  // keys per tile
+  static constexpr int BUFFERS = NT == 2 ? 2 : D == 128 ? 4 : 3;  // of S: of tile g in g % BUFFERS, or (NT = 2) by row tile
+  static constexpr int K_STAGES = NT == 1 ? (D == 64 ? 4 : 5) : (D == 64 ? 4 : 2);
+  static constexpr int V_STAGES = NT == 1 ? (D == 64 ? 6 : 5) : (D == 64 ? 4 : 2);
   static constexpr int Q_BYTES = BM * D * 2;
   static constexpr int KV_BYTES = BN * D * 2;
   static constexpr int K_OFF = NT * Q_BYTES;
-  static constexpr int V_OFF = K_OFF + STAGES * KV_BYTES;
-  static constexpr int OUT_OFF = V_OFF + STAGES * KV_BYTES;  // staging of the outputs, kOutRow * 32 bytes a warp
+  static constexpr int V_OFF = K_OFF + K_STAGES * KV_BYTES;
+  static constexpr int OUT_OFF = V_OFF + V_STAGES * KV_BYTES;  // staging of the outputs, kOutRow * 32 bytes a warp
   static constexpr int CTL_OFF = OUT_OFF + SOFTMAX_WARPS * 32 * kOutRow;
-  static constexpr uint32_t TMEM_COLS = NT == 1 ? 256 : 512;
-  // S buffer i (NT = 1: of every other key tile; NT = 2: of row tile i), O of row tile i.
+  // S buffer b, O of stream i.
   __host__ __device__ static constexpr uint32_t S_COL(int i) { return static_cast<uint32_t>(i * BN); }
-  __host__ __device__ static constexpr uint32_t O_COL(int i) { return static_cast<uint32_t>(2 * BN + i * D); }
+  __host__ __device__ static constexpr uint32_t O_COL(int i) { return static_cast<uint32_t>(BUFFERS * BN + i * D); }
+  static_assert(BUFFERS * BN + 2 * D <= 512, "tensor memory columns");
 };
 
 struct Unit {
@@ -89,34 +101,47 @@ struct Unit {
   int tiles, sink_tiles, first;  // key tiles; those of the sinks; the window's first
 };
 
+// Beginning and ending a unit takes a CTA as long as several key tiles do, so each unit has that many
+// places of the line after its tiles, and a CTA with many short units gets fewer tiles.
+template <int NT>
+constexpr int kUnitPlaces = NT == 1 ? 6 : 3;
+
 struct __align__(16) Ctl {
   uint64_t q_full, q_empty;
-  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t v_raw[4];    // a V tile with rows past the end has landed: v_full follows once they are cleared
-  uint64_t s_full[2];   // S buffer holds scores
-  uint64_t p_half[2];   // NT = 2: row tile i's exponentials of the first 64 keys (4 warps)
-  uint64_t p_ready[2];  // S buffer holds exponentials (4 warps)
-  uint64_t pv_done[2];  // row tile i: P V of one more key tile is complete
-  uint64_t drain;
+  uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
+  uint64_t v_raw[kMaxStages];  // NT = 2: a V tile with rows past the end has landed: v_full follows once they are cleared
+  uint64_t s_full[4];          // S buffer b holds scores
+  uint64_t p_half[4];          // it holds the exponentials of the first half of the keys (4 warps; see HALVES)
+  uint64_t p_ready[4];         // it holds all exponentials (4 warps)
+  uint64_t pv_done[4];         // P V out of it is complete
+  uint64_t o_free;             // NT = 1: a unit's O has been read out (8 warps)
+  uint64_t streams;            // NT = 1: a unit's (m, l) are in `ml` and its P V are complete (8 warps)
+  uint64_t groups[2];          // stream i's key groups: hand-offs among its four warps
+  uint64_t drain[2];
   uint32_t tmem_base;
   int abort;
-  uint64_t merge;  // the key groups of a row: hand-offs among the four softmax warps
   int start[5];  // first unit's item, key head, tile; tiles of this CTA; total tiles
   Unit unit;     // the first unit
   int sums[32];
-  float2 ml[BM];  // (m, l) of every row and key group
+  float2 ml[2][2][BM];  // NT = 1: (m, l) of this and the next unit, by stream and TMEM lane
+};
+
+// A place in a ring of stages, and the phase its barriers are in there.
+struct Ring {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) s = 0, phase ^= 1;
+  }
 };
 
 template <int D, int NT>
 constexpr int smem_bytes() {
   const int used = Shape<D, NT>::CTL_OFF + static_cast<int>(sizeof(Ctl)) + 1024;
+  static_assert(used <= 232448, "shared memory per CTA");
   // One CTA per SM needs >= 116 KB, so that its 512-column TMEM allocation never contends.
-  return NT == 2 && used < 118784 ? 118784 : used;
+  return used < 118784 ? 118784 : used;
 }
-
-// Register split of the one-CTA-per-SM shape: the softmax threads hold a row's 128 scores.
-constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 200, REGS_OTHER = 104;
-static_assert(8 * REGS_SOFTMAX + 4 * REGS_OTHER == 12 * REGS_LAUNCH, "register split must match the launch");
 
 __device__ __forceinline__ void give_up(Ctl* ctl, uint32_t code) {
   if (!*reinterpret_cast<volatile int*>(&ctl->abort)) atomicCAS(&g_cache_attn_status, 0u, code);
@@ -189,13 +214,13 @@ __device__ __forceinline__ int quotient(int a, int b) {
   return r < 0 ? q - 1 : r >= b ? q + 1 : q;
 }
 
-// The pieces: `total` tiles over `ctas` CTAs, CTA i from piece_start(i).
+// The pieces: `total` places of the line over `ctas` CTAs, CTA i from piece_start(i).
 __device__ __forceinline__ int piece_start(int i, int total, int ctas) {  // floor(i * total / ctas)
   const int each = quotient(total, ctas);
   return i * each + quotient(i * (total - each * ctas), ctas);
 }
-__device__ __forceinline__ int piece_of(int tile, int total, int ctas) {
-  return static_cast<int>(((static_cast<int64_t>(tile) + 1) * ctas - 1) / total);
+__device__ __forceinline__ int piece_of(int place, int total, int ctas) {
+  return static_cast<int>(((static_cast<int64_t>(place) + 1) * ctas - 1) / total);
 }
 
 __device__ __forceinline__ int block_exclusive(int x, int* sums, int& total) {
@@ -219,18 +244,19 @@ __device__ __forceinline__ int block_exclusive(int x, int* sums, int& total) {
   return before + s - x;
 }
 
-// Finds this CTA's piece (ctl->start and its first unit); all threads.  Returns the CTAs that have one.
-__device__ __forceinline__ int find_piece(const AttnParams& p, Ctl* ctl, int block_tokens) {
+// Finds this CTA's piece (ctl->start and its first unit); all threads.  `places`: of the line after each
+// unit's tiles.  Returns the CTAs that have a piece.
+__device__ __forceinline__ int find_piece(const AttnParams& p, Ctl* ctl, int block_tokens, int places) {
   const int items = p.seqs * p.blocks;
   int total = 0, at = 0;
   Unit u;
-  u.tiles = 0;
+  u.tiles = -places;
   for (int e0 = 0; e0 < items; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
-    u.tiles = 0;
+    u.tiles = -places;
     if (e < items) u = unit_of(p, e, block_tokens);
     int sum;
-    at = total + block_exclusive(u.tiles * p.kv_heads, ctl->sums, sum);
+    at = total + block_exclusive((u.tiles + places) * p.kv_heads, ctl->sums, sum);
     total += sum;
   }
   const int ctas = min(static_cast<int>(gridDim.x), total);
@@ -240,18 +266,19 @@ __device__ __forceinline__ int find_piece(const AttnParams& p, Ctl* ctl, int blo
   for (int e0 = 0; e0 < items; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
     if (items > static_cast<int>(blockDim.x)) {
-      u.tiles = 0;
+      u.tiles = -places;
       if (e < items) u = unit_of(p, e, block_tokens);
       int sum;
-      at = seen + block_exclusive(u.tiles * p.kv_heads, ctl->sums, sum);
+      at = seen + block_exclusive((u.tiles + places) * p.kv_heads, ctl->sums, sum);
       seen += sum;
     }
-    if (at <= begin && begin < at + u.tiles * p.kv_heads) {
-      const int head = quotient(begin - at, u.tiles);
+    const int length = u.tiles + places;
+    if (at <= begin && begin < at + length * p.kv_heads) {
+      const int head = quotient(begin - at, length);
       ctl->unit = u;
       ctl->start[0] = e;
       ctl->start[1] = head;
-      ctl->start[2] = begin - at - head * u.tiles;
+      ctl->start[2] = begin - at - head * length;
       ctl->start[3] = piece_start(blockIdx.x + 1, total, ctas) - begin;
       ctl->start[4] = total;
     }
@@ -261,27 +288,30 @@ __device__ __forceinline__ int find_piece(const AttnParams& p, Ctl* ctl, int blo
 
 // The tiles of a CTA in order; every role walks its own copy.
 struct Walk {
-  int item, kv_head, tile, left;
+  int item, kv_head;
+  int place, left;  // where the piece begins in this unit's stretch of the line; places left from there
   Unit u;
   int a0, a1;  // this unit's tiles in this CTA
 
-  __device__ __forceinline__ void begin(const Ctl* ctl) {
+  // The first unit of the piece with tiles in it; false when it has none.
+  __device__ __forceinline__ bool begin(const AttnParams& p, const Ctl* ctl, int block_tokens, int places) {
     item = ctl->start[0];
     kv_head = ctl->start[1];
-    tile = ctl->start[2];
+    place = ctl->start[2];
     left = ctl->start[3];
     u = ctl->unit;
-    a0 = tile;
+    a0 = place;
     a1 = min(u.tiles, a0 + left);
+    return a0 < a1 || next(p, block_tokens, places);
   }
-  __device__ __forceinline__ bool next(const AttnParams& p, int block_tokens) {
-    left -= a1 - a0;
+  __device__ __forceinline__ bool next(const AttnParams& p, int block_tokens, int places) {
+    left -= u.tiles + places - place;
     if (left <= 0) return false;
     if (++kv_head == p.kv_heads) {
       kv_head = 0;
       u = unit_of(p, ++item, block_tokens);
     }
-    a0 = 0;
+    place = a0 = 0;
     a1 = min(u.tiles, left);
     return true;
   }
@@ -298,11 +328,12 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st_32x32b_x16(taddr, r); }
 
 // kind::f16 instruction descriptor (see umma_idesc_f16_f32) with both operands fp16 or both bf16.
 template <bool BF16>
@@ -371,11 +402,13 @@ __device__ __forceinline__ uint64_t visible(const AttnParams& p, const Unit& u, 
 // ------------------------------------------------------------------------------ kernel
 
 template <int D, int NT, int KS, bool BF16>
-__global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_SM)
+__global__ void __launch_bounds__(THREADS, 1)
     cache_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv, const AttnParams p) {
   using C = Shape<D, NT>;
-  constexpr int BN = C::BN, ST = C::STAGES;
+  constexpr int BN = C::BN, NB = C::BUFFERS;
+  // Hand P over in halves: with 128 keys and no key groups (which finish together).
+  constexpr int HALVES = KS == 1 && BN == 128 ? 2 : 1;
   constexpr int KC = BN / KS;          // keys of a tile per key group
   constexpr int GROUP_ROWS = BM / KS;  // rows of the tile per key group
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -387,34 +420,38 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
 
   pdl_trigger();
   if (threadIdx.x < 3) prefetch_tensormap(threadIdx.x == 0 ? &tq : threadIdx.x == 1 ? &tk : &tv);
-  if (warp == C::MMA_WARP) {
-    tmem_alloc(&ctl->tmem_base, C::TMEM_COLS);
+  if (warp == MMA_WARP) {
+    tmem_alloc(&ctl->tmem_base, TMEM_COLS);
     tmem_relinquish();
   } else if (threadIdx.x == 0) {
     mbar_init(&ctl->q_full, 1);
     mbar_init(&ctl->q_empty, 1);
-    for (int s = 0; s < ST; ++s) {
+    for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(&ctl->k_full[s], 1);
       mbar_init(&ctl->k_empty[s], 1);
       mbar_init(&ctl->v_full[s], 1);
       mbar_init(&ctl->v_empty[s], 1);
       mbar_init(&ctl->v_raw[s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&ctl->s_full[i], 1);
       mbar_init(&ctl->p_half[i], 4);
       mbar_init(&ctl->p_ready[i], 4);
       mbar_init(&ctl->pv_done[i], 1);
     }
-    mbar_init(&ctl->merge, 4);
-    mbar_init(&ctl->drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->groups[i], 4);
+      mbar_init(&ctl->drain[i], 1);
+    }
+    mbar_init(&ctl->o_free, 8);
+    mbar_init(&ctl->streams, 8);
     ctl->abort = 0;
     fence_mbar_init();
   }
   if (p.tile_keys < BN) {
     // Rows of the V stages that no page reaches: zero once, no copy writes them.
     const int spare = (BN - p.tile_keys) * 8;  // 16-byte units per 64-column half
-    for (int e = threadIdx.x; e < ST * (D / 64) * spare; e += blockDim.x) {
+    for (int e = threadIdx.x; e < C::V_STAGES * (D / 64) * spare; e += blockDim.x) {
       const int half = e / spare, at = e % spare;
       *reinterpret_cast<uint4*>(smem + C::V_OFF + half * (BN * 128) + p.tile_keys * 128 + at * 16) =
           make_uint4(0, 0, 0, 0);
@@ -422,35 +459,62 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
     fence_proxy_async_smem();
   }
   pdl_wait();
-  const int ctas = find_piece(p, ctl, block_tokens);
+  constexpr int PLACES = kUnitPlaces<NT>;
+  const int ctas = find_piece(p, ctl, block_tokens, PLACES);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (static_cast<int>(blockIdx.x) >= ctas) {
+  if (static_cast<int>(blockIdx.x) >= ctas || !Walk().begin(p, ctl, block_tokens, PLACES)) {  // no tiles
     if (threadIdx.x == 0) p.head[blockIdx.x] = make_int4(0, 0, -1, 0);
-    if (warp == C::MMA_WARP) tmem_dealloc(ctl->tmem_base, C::TMEM_COLS);
+    if (warp == MMA_WARP) tmem_dealloc(ctl->tmem_base, TMEM_COLS);
     return;
   }
   const uint32_t tmem = ctl->tmem_base;
 
-  if (warp >= C::SOFTMAX_WARPS) {
-    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS_OTHER) : "memory");
-    if (warp == C::K_WARP || warp == C::V_WARP) {
+  if (warp >= SOFTMAX_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(REGS_OTHER) : "memory");
+    // One thread: the unit's Q, as row tiles (NT = 2) or copies for the key groups.
+    auto load_q = [&](const Walk& w) {
+      mbar_arrive_expect_tx(&ctl->q_full, static_cast<uint32_t>(NT * KS * (D / 64) * p.tile_tokens * p.group * 128));
+#pragma unroll
+      for (int i = 0; i < NT * KS; ++i)
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d)
+          tma_load_4d(smem + (NT == 2 ? i * C::Q_BYTES : i * GROUP_ROWS * 128) + d * (BM * 128), &tq, &ctl->q_full, d * 64,
+                      w.kv_head * p.group, w.u.t0 + (NT == 2 ? i * p.tile_tokens : 0), w.u.b);
+    };
+    // One warp: zeros over the rows of V stage s past the sequence's end, for the MMAs issued after it.
+    auto clear_v = [&](const Unit& u, int a, int s) {
+      const int first = max(u.len - tile_key(p, u, a), 0);  // rows that hold tokens
+      const int units = (p.tile_keys - first) * 8;          // 16-byte units per 64-column half
+#pragma unroll
+      for (int half = 0; half < D / 64; ++half)
+        for (int at = lane; at < units; at += 32)
+          *reinterpret_cast<uint4*>(smem + C::V_OFF + s * C::KV_BYTES + half * (BN * 128) + first * 128 + at * 16) =
+              make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    if (warp == K_WARP || warp == V_WARP) {
       // ---------------------------------------------- K loads, V loads: one warp each, a lane per page
       // K frees its stages a softmax earlier than V does; one warp for both would hold K back.
       // Lane 0 waits for the whole warp, so that either every lane issues its boxes or none does.
-      const bool is_v = warp == C::V_WARP;
+      const bool is_v = warp == V_WARP;
       uint64_t* full = is_v ? ctl->v_full : ctl->k_full;
       uint64_t* empty = is_v ? ctl->v_empty : ctl->k_empty;
+      const int count = is_v ? C::V_STAGES : C::K_STAGES;
       const CUtensorMap* map = is_v ? &tv : &tk;
       uint8_t* stages = smem + (is_v ? C::V_OFF : C::K_OFF);
       const int boxes = p.tile_pages;
       const int box_keys = p.tile_keys / boxes;
       const int box_bytes = box_keys * 128;  // one page's rows of one 64-column half
       const uint32_t tile_bytes = static_cast<uint32_t>(boxes * box_bytes * (D / 64));
+      // The table is read for several tiles at once, a batch ahead: a lane per page.
+      const int batch = quotient(32, boxes), lane_tile = quotient(lane, boxes), lane_box = lane - lane_tile * boxes;
       bool ok = true;
       Walk w;
-      w.begin(ctl);
+      w.begin(p, ctl, block_tokens, PLACES);
+      Ring ring;
       int issued = 0;
       uint32_t raw = 0, cleared = 0;  // bit s: parity of the next v_raw[s]; stage s's last tile is one to clear
       do {
@@ -458,22 +522,32 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
         const int32_t* row = p.table + w.u.b * p.table_stride;
         // A page that the unit sees nothing of, or that is not there, reads as zeros (the tensor
         // map fills what lies outside it), so a page given back or never written is not touched.
-        auto page_at = [&](int a) -> int {
-          const int k0 = tile_key(p, w.u, a) + lane * box_keys;
-          const int j = k0 / p.page_size;
-          if (lane >= boxes || j >= p.max_pages || k0 >= w.u.len || (k0 + box_keys <= lo && k0 >= p.sinks)) return -1;
+        auto pages_from = [&](int a) -> int {  // of `batch` tiles from a on, one per lane
+          const int k0 = tile_key(p, w.u, a + lane_tile) + lane_box * box_keys;
+          const int j = p.page_shift >= 0 ? k0 >> p.page_shift : k0 / p.page_size;
+          if (lane_tile >= batch || a + lane_tile >= w.a1 || j >= p.max_pages || k0 >= w.u.len ||
+              (k0 + box_keys <= lo && k0 >= p.sinks))
+            return -1;
           return row[j];
         };
-        int next_page = page_at(w.a0);
-        for (int a = w.a0; a < w.a1; ++a) {
-          const int s = issued % ST;
-          const int y = boxes > 1 ? 0 : tile_key(p, w.u, a) % p.page_size;
-          const int page = next_page;
-          if (a + 1 < w.a1) next_page = page_at(a + 1);
-          ok = lane != 0 || wait_bounded(&empty[s], ((issued / ST) & 1) ^ 1, p.wait_limit, abort_flag);
+        int pages = pages_from(w.a0), pages_next = pages_from(w.a0 + batch), at = 0;
+        for (int a = w.a0; a < w.a1; ++a, ++at) {
+          const int s = ring.s;
+          if (at == batch) {
+            at = 0;
+            pages = pages_next;
+            pages_next = pages_from(a + batch);
+          }
+          const int page = __shfl_sync(0xffffffffu, pages, (at * boxes + lane) & 31);
+          int y = 0;  // row of the page
+          if (p.page_size > p.tile_keys) {
+            const int k0 = tile_key(p, w.u, a);
+            y = p.page_shift >= 0 ? k0 & (p.page_size - 1) : k0 % p.page_size;
+          }
+          ok = lane != 0 || wait_bounded(&empty[s], ring.phase ^ 1, p.wait_limit, abort_flag);
           ok = __shfl_sync(0xffffffffu, ok, 0);
           if (!ok) break;
-          const bool clear = is_v && past_end(p, w.u, a);
+          const bool clear = NT == 2 && is_v && past_end(p, w.u, a);
           uint64_t* landed = clear ? &ctl->v_raw[s] : &full[s];
           if (clear) raw ^= 1u << s;
           cleared = clear ? cleared | 1u << s : cleared & ~(1u << s);
@@ -485,186 +559,211 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
             for (int d = 0; d < D / 64; ++d) tma_load_4d(to + d * (BN * 128), map, landed, d * 64, w.kv_head, y, page);
           }
           ++issued;
+          ring.next(count);
         }
-      } while (ok && w.next(p, block_tokens));
+      } while (ok && w.next(p, block_tokens, PLACES));
       if (!ok && lane == 0) {
         give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
         // Drain every copy this warp issued before the CTA exits.
-        for (int j = max(0, issued - ST); j < issued; ++j) {
-          const int s = j % ST;
+        for (int j = max(0, issued - count); j < issued; ++j) {
+          const int s = j % count;
           const bool clear = cleared >> s & 1;
-          if (!wait_bounded(clear ? &ctl->v_raw[s] : &full[s], clear ? ~raw >> s & 1 : (j / ST) & 1,
-                                 int64_t(1) << 24, nullptr))
+          if (!wait_bounded(clear ? &ctl->v_raw[s] : &full[s], clear ? ~raw >> s & 1 : (j / count) & 1, int64_t(1) << 24,
+                            nullptr))
             atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
         }
       }
-    } else if (warp == C::AUX_WARP) {
+    } else if (NT == 2 && warp == AUX_WARP) {
       // ---------------------------------------------- Q loads, and value rows past the end become zeros
-      const uint32_t q_bytes = static_cast<uint32_t>(NT * KS * (D / 64) * p.tile_tokens * p.group * 128);
       bool ok = true;
       Walk w;
-      w.begin(ctl);
-      int n = 0, g = 0;
+      w.begin(p, ctl, block_tokens, PLACES);
+      Ring ring;
+      int n = 0;
       uint32_t raw = 0;  // bit s: parity of v_raw[s]
       do {
         // The next unit's Q once the last Q K^T of the unit before retired.
         if (lane == 0) {
           ok = n == 0 || wait_bounded(&ctl->q_empty, (n - 1) & 1, p.wait_limit, abort_flag);
-          if (ok) {
-            mbar_arrive_expect_tx(&ctl->q_full, q_bytes);
-#pragma unroll
-            for (int i = 0; i < NT * KS; ++i)  // row tiles, or copies for the key groups
-#pragma unroll
-              for (int d = 0; d < D / 64; ++d)
-                tma_load_4d(smem + (NT == 2 ? i * C::Q_BYTES : i * GROUP_ROWS * 128) + d * (BM * 128), &tq, &ctl->q_full,
-                            d * 64, w.kv_head * p.group, w.u.t0 + (NT == 2 ? i * p.tile_tokens : 0), w.u.b);
-          }
+          if (ok) load_q(w);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         ++n;
-        for (int a = w.a0; a < w.a1 && ok; ++a, ++g) {
+        for (int a = w.a0; a < w.a1 && ok; ++a, ring.next(C::V_STAGES)) {
           if (!past_end(p, w.u, a)) continue;
-          const int s = g % ST;
+          const int s = ring.s;
           if (lane == 0) ok = wait_bounded(&ctl->v_raw[s], raw >> s & 1, p.wait_limit, abort_flag);
+          __syncwarp();
           ok = __shfl_sync(0xffffffffu, ok, 0);
           if (!ok) break;
           raw ^= 1u << s;
-          const int first = max(w.u.len - tile_key(p, w.u, a), 0);  // rows that hold tokens
-          const int units = (p.tile_keys - first) * 8;              // 16-byte units per half
-          for (int e = lane; e < (D / 64) * units; e += 32) {
-            const int half = e / units, at = e - half * units;
-            *reinterpret_cast<uint4*>(smem + C::V_OFF + s * C::KV_BYTES + half * (BN * 128) + first * 128 + at * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
+          clear_v(w.u, a, s);
           if (lane == 0) mbar_arrive(&ctl->v_full[s]);
         }
-      } while (ok && w.next(p, block_tokens));
+      } while (ok && w.next(p, block_tokens, PLACES));
       if (lane == 0) {
         if (!ok) give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
         // The MMA thread waits for each Q load; if it gave up, this thread does before the CTA exits.
         if (n > 0 && !wait_bounded(&ctl->q_full, (n - 1) & 1, int64_t(1) << 24, nullptr))
           atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
       }
-    } else if (elect_one_lane()) {
-      // ---------------------------------------------- MMA issue
+    } else if ((NT == 1 && warp == AUX_WARP) || elect_one_lane()) {
+      // ---------------------------------------------- MMA issue (one lane; NT = 1 has its whole P V warp here)
       constexpr uint32_t idesc_s = idesc<BF16>(BN, 0);  // B = K tile, K-major
       constexpr uint32_t idesc_o = idesc<BF16>(D, 1);   // B = V tile, N-major
-      bool ok = true;
+      const uint32_t q_low = desc_low(smem_u32(smem), 16);
+      const uint32_t k_low = desc_low(smem_u32(smem + C::K_OFF), 16);
+      const uint32_t v_low = desc_low(smem_u32(smem + C::V_OFF), BN * 128);
       auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         if (wait_bounded(bar, parity, p.wait_limit, abort_flag)) return true;
         give_up(ctl, NTL_STATUS_MMA_FULL_WAIT);
         return false;
       };
-      // Two cursors over the same tiles: Q K^T runs one tile ahead of P V.
-      Walk w, wq;
-      w.begin(ctl);
-      wq.begin(ctl);
-      int gq = 0, aq = wq.a0, uq = 0;
-      bool more = true;
-      auto qk_ready = [&]() -> bool {
-        if (aq == wq.a0 && !wait(&ctl->q_full, uq & 1)) return false;
-        return wait(&ctl->k_full[gq % ST], (gq / ST) & 1);
-      };
-      const uint32_t q_low = desc_low(smem_u32(smem), 16);
-      const uint32_t k_low = desc_low(smem_u32(smem + C::K_OFF), 16);
-      const uint32_t v_low = desc_low(smem_u32(smem + C::V_OFF), BN * 128);
-      auto qk = [&](int i) {  // S (buffer gq % 2, or row tile i) = Q_i K^T
-        const uint32_t q = q_low + (NT == 2 ? i : 0) * (C::Q_BYTES >> 4), k = k_low + (gq % ST) * (C::KV_BYTES >> 4);
-        const int buf = NT == 2 ? i : gq & 1;
+      bool ok = true;
+      Walk w;
+      w.begin(p, ctl, block_tokens, PLACES);
+      Ring kr, vr;
+      int g = 0;
+      auto qk = [&](int i) {  // S buffer i = Q K^T
+        const uint32_t q = q_low + (NT == 2 ? i : 0) * (C::Q_BYTES >> 4), k = k_low + kr.s * (C::KV_BYTES >> 4);
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          tc_mma_f16_ss(tmem + C::S_COL(buf), desc_at(q, (kk >> 2) * (BM * 128) + (kk & 3) * 32),
+          tc_mma_f16_ss(tmem + C::S_COL(i), desc_at(q, (kk >> 2) * (BM * 128) + (kk & 3) * 32),
                         desc_at(k, (kk >> 2) * (BN * 128) + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
-        tc_commit(&ctl->s_full[buf]);
+        tc_commit(&ctl->s_full[i]);
       };
-      auto qk_end = [&]() {  // after the last row tile's
-        tc_commit(&ctl->k_empty[gq % ST]);
-        ++gq;
-        if (++aq == wq.a1) {
-          tc_commit(&ctl->q_empty);
-          more = wq.next(p, block_tokens);
-          aq = wq.a0;
-          ++uq;
+      // O_i += P V out of buffer `buf`, keys of one half (see HALVES); `add` 0 overwrites O.
+      auto pv = [&](int i, int buf, int half, uint32_t add) {
+        const uint32_t v = v_low + vr.s * (C::KV_BYTES >> 4);
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < BN / 16 / HALVES; ++kk) {
+          const uint32_t from = half * (BN / 16 / HALVES);
+          tc_mma_f16_ts(tmem + C::O_COL(i), tmem + C::S_COL(buf) + (from + kk) * 8, desc_at(v, (from + kk) * 2048), idesc_o,
+                        kk > 0 ? 1u : add);
         }
+        if (half + 1 == HALVES) tc_commit(&ctl->pv_done[buf]);
       };
-      if ((ok = qk_ready())) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) qk(i);
-        qk_end();
-      }
-      int g = 0;
-      bool left = ok;
-      while (left) {
-        for (int a = w.a0; a < w.a1 && ok; ++a, ++g) {
-          const int s = g % ST;
-          auto pv = [&](int i) -> bool {  // O_i += P V; NT = 2 starts on the first half of the keys
-            const int buf = NT == 2 ? i : g & 1;
-            const uint32_t v = v_low + s * (C::KV_BYTES >> 4);
-            constexpr int HALVES = NT;
-#pragma unroll
-            for (int half = 0; half < HALVES; ++half) {
-              if (!wait(half + 1 < HALVES ? &ctl->p_half[buf] : &ctl->p_ready[buf], (NT == 2 ? g : g >> 1) & 1)) return false;
-              tc_fence_after();
-#pragma unroll
-              for (int kk = half * (BN / 16 / HALVES); kk < (half + 1) * (BN / 16 / HALVES); ++kk)
-                tc_mma_f16_ts(tmem + C::O_COL(i), tmem + C::S_COL(buf) + kk * 8, desc_at(v, kk * 2048), idesc_o,
-                              (a > w.a0 || kk > 0) ? 1u : 0u);
+      if constexpr (NT == 1) {
+        if (warp == MMA_WARP) {  // Q and Q K^T
+          uint32_t q_phase = 0;
+          load_q(w);
+          do {
+            if (!(ok = wait(&ctl->q_full, q_phase))) break;
+            for (int a = w.a0; a < w.a1; ++a, ++g, kr.next(C::K_STAGES)) {
+              // S buffer g % NB is free once P V of tile g - NB is complete.
+              if (!(ok = (g < NB || wait(&ctl->pv_done[g % NB], (g / NB - 1) & 1)) && wait(&ctl->k_full[kr.s], kr.phase)))
+                break;
+              qk(g % NB);
+              tc_commit(&ctl->k_empty[kr.s]);
             }
-            tc_commit(&ctl->pv_done[i]);
-            return true;
+            if (!ok || !w.next(p, block_tokens, PLACES)) break;
+            // The next unit's Q once this one's last Q K^T retired.
+            tc_commit(&ctl->q_empty);
+            if (!(ok = wait(&ctl->q_empty, q_phase))) break;
+            load_q(w);
+            q_phase ^= 1;
+          } while (true);
+          // Every Q load has landed before the CTA exits (this thread waited for it, unless it gave up).
+          if (!ok && !wait_bounded(&ctl->q_full, q_phase, int64_t(1) << 24, nullptr))
+            atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
+        } else {  // clearing and P V
+          auto warp_ok = [&](uint64_t* bar, uint32_t parity) -> bool {  // lane 0 waits for the warp
+            const bool got = lane != 0 || wait(bar, parity);
+            __syncwarp();
+            return __shfl_sync(0xffffffffu, got, 0);
           };
-          // The next tile's Q K^T goes out before this tile's P V is done, to run during the softmax; a new
-          // unit's waits for loads that the end of this unit must not wait for, and goes last.
-          bool late = false;
-          if constexpr (NT == 1) {
-            if (more && aq != wq.a0) {
-              if (!(ok = qk_ready())) break;
-              qk(0);
-              qk_end();
-            } else {
-              late = more;
+          int unit = 0;
+          do {
+            // O of the unit before has been read out, by both streams.
+            if (unit > 0 && !(ok = warp_ok(&ctl->o_free, (unit - 1) & 1))) break;
+            for (int a = w.a0; a < w.a1; ++a, ++g, vr.next(C::V_STAGES)) {
+              const int buf = g % NB;
+              const uint32_t phase = (g / NB) & 1, add = a - w.a0 >= 2;  // each stream's first tile overwrites its O
+              if (!(ok = warp_ok(&ctl->v_full[vr.s], vr.phase))) break;
+              if (past_end(p, w.u, a)) clear_v(w.u, a, vr.s);
+              if constexpr (HALVES == 2) {
+                if (!(ok = warp_ok(&ctl->p_half[buf], phase))) break;
+                if (elect_one_lane()) pv(g & 1, buf, 0, add);
+              }
+              if (!(ok = warp_ok(&ctl->p_ready[buf], phase))) break;
+              if (elect_one_lane()) {
+                pv(g & 1, buf, HALVES - 1, HALVES == 2 ? 1u : add);
+                tc_commit(&ctl->v_empty[vr.s]);
+              }
             }
-            if (!(ok = wait(&ctl->v_full[s], (g / ST) & 1) && pv(0))) break;
-          } else {
+            ++unit;
+          } while (ok && w.next(p, block_tokens, PLACES));
+        }
+      } else {
+        // Two cursors over the same tiles: Q K^T runs one tile ahead of P V, right after the P V that frees its
+        // S, during the other row tile's softmax; a new unit's waits for loads that the end of this unit must
+        // not wait for, and goes after it.
+        Walk wq;
+        wq.begin(p, ctl, block_tokens, PLACES);
+        int aq = wq.a0;
+        uint32_t q_phase = 0;
+        bool more = true;
+        auto qk_ready = [&]() -> bool {
+          if (aq == wq.a0 && !wait(&ctl->q_full, q_phase)) return false;
+          return wait(&ctl->k_full[kr.s], kr.phase);
+        };
+        auto qk_end = [&]() {  // after the second row tile's
+          tc_commit(&ctl->k_empty[kr.s]);
+          kr.next(C::K_STAGES);
+          if (++aq == wq.a1) {
+            tc_commit(&ctl->q_empty);
+            more = wq.next(p, block_tokens, PLACES);
+            aq = wq.a0;
+            q_phase ^= 1;
+          }
+        };
+        auto pv_both = [&](int i, uint32_t add) -> bool {
+          if (!wait(&ctl->p_half[i], g & 1)) return false;
+          pv(i, i, 0, add);
+          if (!wait(&ctl->p_ready[i], g & 1)) return false;
+          pv(i, i, 1, 1u);
+          return true;
+        };
+        while ((ok = qk_ready())) {
+          qk(0);
+          qk(1);
+          qk_end();
+          for (int a = w.a0; a < w.a1; ++a, ++g, vr.next(C::V_STAGES)) {
+            // V of this tile and K of the next have landed long before P is ready: only P is on the critical
+            // path.
             const bool ahead = more && aq != wq.a0;
-            late = more && !ahead;
-            // K of the next tile has landed long before P is ready: only P is on the critical path.
-            if (!(ok = wait(&ctl->v_full[s], (g / ST) & 1) && (!ahead || qk_ready()) && pv(0))) break;
+            const uint32_t add = a > w.a0;
+            if (!(ok = wait(&ctl->v_full[vr.s], vr.phase) && (!ahead || qk_ready()) && pv_both(0, add))) break;
             if (ahead) qk(0);
-            if (!(ok = pv(1))) break;
+            if (!(ok = pv_both(1, add))) break;
+            tc_commit(&ctl->v_empty[vr.s]);
             if (ahead) {
               qk(1);
               qk_end();
             }
           }
-          tc_commit(&ctl->v_empty[s]);
-          if (late) {
-            if (!(ok = qk_ready())) break;
-#pragma unroll
-            for (int i = 0; i < NT; ++i) qk(i);
-            qk_end();
-          }
+          if (!ok || !w.next(p, block_tokens, PLACES)) break;
         }
-        left = ok && w.next(p, block_tokens);
       }
-      if (!ok) {
-        tc_commit(&ctl->drain);
-        if (!wait_bounded(&ctl->drain, 0, int64_t(1) << 24, nullptr))
+      if (!ok && (warp == MMA_WARP || elect_one_lane())) {
+        uint64_t* drain = &ctl->drain[warp == MMA_WARP ? 0 : 1];
+        tc_commit(drain);
+        if (!wait_bounded(drain, 0, int64_t(1) << 24, nullptr))
           atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
       }
     }
   } else {
     // ---------------------------------------------- softmax: one thread per row (and key group)
-    if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS_SOFTMAX) : "memory");
-    const int i = warp >> 2;
-    const int group = KS == 1 ? 0 : (warp & 3) / (4 / KS);
-    const int r = (warp & 3) * 32 + lane - group * GROUP_ROWS;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS_SOFTMAX) : "memory");
+    const int i = warp >> 2;                       // stream
+    const int row_lane = (warp & 3) * 32 + lane;   // TMEM lane
+    const int group = row_lane / GROUP_ROWS;       // key group
+    const int r = row_lane - group * GROUP_ROWS;   // row of the tile
     const int row_token = quotient(r, p.group), row_head = r - row_token * p.group;
-    const int t_in_block = i * p.tile_tokens + row_token;
+    const int t_in_block = (NT == 2 ? i * p.tile_tokens : 0) + row_token;
     const bool in_tile = row_token < p.tile_tokens;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + lane_off + C::O_COL(i);
@@ -672,14 +771,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
     int4 cut = make_int4(0, 0, -1, 0);
     bool ok = true;
     Walk w;
-    w.begin(ctl);
-    int g = 0;
-    uint32_t merges = 0;
-    // The four warps meet (key groups only): false when one of them gave up.
-    auto meet = [&]() -> bool {
+    w.begin(p, ctl, block_tokens, PLACES);
+    int g0 = 0;  // tiles before this unit
+    uint32_t units = 0, group_meets = 0, stream_meets = 0;
+    // Several warps meet at a barrier: false when one of them gave up.
+    auto meet = [&](uint64_t* bar, uint32_t& meets) -> bool {
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->merge);
-      return warp_wait(&ctl->merge, merges++ & 1, p.wait_limit, abort_flag);
+      if (lane == 0) mbar_arrive(bar);
+      return warp_wait(bar, meets++ & 1, p.wait_limit, abort_flag);
     };
     do {
       const Unit& u = w.u;
@@ -691,27 +790,30 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
       int whole_from = 0, whole_to = 0;
       if (p.tile_keys == BN) {
         const int prefix = u.len - u.live;
-        const int t_first = u.t0 + i * p.tile_tokens, t_last = min(t_first + p.tile_tokens, u.live) - 1;
+        const int t_first = u.t0 + (NT == 2 ? i * p.tile_tokens : 0), t_last = min(t_first + p.tile_tokens, u.live) - 1;
         const int all_lo = p.tree ? 0 : max(prefix + t_last - p.window + 1, 0);
         const int all_hi = p.tree ? prefix : prefix + t_first + 1;
         whole_from = u.sink_tiles + max((all_lo + BN - 1) / BN - u.first, 0);
         whole_to = u.sink_tiles + all_hi / BN - u.first;
       }
       float m = -INFINITY, l = 0.0f;
+      // This stream's tiles: every one, or (NT = 1) those of its parity.
+      constexpr int STEP = NT == 1 ? 2 : 1;
+      const int a_first = w.a0 + (NT == 1 ? (g0 ^ i) & 1 : 0);
       if (!any) {  // rows past the end: this warp only keeps step
-        for (int a = w.a0; a < w.a1; ++a, ++g) {
-          const int buf = NT == 2 ? i : g & 1;
-          if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g >> 1) & 1, p.wait_limit, abort_flag))) break;
+        for (int a = a_first; a < w.a1; a += STEP) {
+          const int g = g0 + a - w.a0, buf = NT == 2 ? i : g % NB;
+          if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g / NB) & 1, p.wait_limit, abort_flag))) break;
           if (lane == 0) {
-            if (NT == 2) mbar_arrive(&ctl->p_half[buf]);
+            if (HALVES == 2) mbar_arrive(&ctl->p_half[buf]);
             mbar_arrive(&ctl->p_ready[buf]);
           }
         }
       } else {
-        for (int a = w.a0; a < w.a1; ++a, ++g) {
-          const int buf = NT == 2 ? i : g & 1;
+        for (int a = a_first; a < w.a1; a += STEP) {
+          const int g = g0 + a - w.a0, buf = NT == 2 ? i : g % NB;
           const uint32_t s_addr = tmem + lane_off + C::S_COL(buf);
-          if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g >> 1) & 1, p.wait_limit, abort_flag))) break;
+          if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g / NB) & 1, p.wait_limit, abort_flag))) break;
           tc_fence_after();
           uint32_t sv[KC];
           if constexpr (KC == 16) {
@@ -723,11 +825,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           }
           tc_wait_ld();
           if (__builtin_expect(a < whole_from || a >= whole_to, 0)) {
-            const int k0 = tile_key(p, u, a);
+            const int k0 = tile_key(p, u, a), skip = group * KC;
 #pragma unroll
             for (int ch = 0; ch < (KC + 63) / 64; ++ch) {
-              uint64_t see = live ? visible(p, u, t, k0 + ch * 64) & low_bits(p.tile_keys - ch * 64) : 0;
-              if constexpr (KS > 1) see >>= group * KC;
+              const int from = skip + ch * 64;
+              const uint64_t see = live ? visible(p, u, t, k0 + from) & low_bits(p.tile_keys - from) : 0;
 #pragma unroll
               for (int e = 0; e < (KC < 64 ? KC : 64); ++e)
                 if (!(see >> e & 1)) sv[ch * 64 + e] = __float_as_uint(-INFINITY);
@@ -759,14 +861,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
             moved = true;
           }
           const bool rescale = __any_sync(0xffffffffu, moved);
-          // NT = 1: S of this tile was issued before P V of the tile before, which is waited for here
-          // where o is about to change, and on the unit's last tile: before this warp hands over P,
-          // pv_done is at most one phase behind, so the wait after it is not a phase early.
-          // (NT = 2 issued S after that P V: it is complete.)
-          if (NT == 1 && g > 0 && __builtin_expect(rescale || a + 1 == w.a1, 0) &&
-              !(ok = warp_wait(&ctl->pv_done[0], (g - 1) & 1, p.wait_limit, abort_flag)))
-            break;
           if (__builtin_expect(rescale, 0)) {
+            // O is stable once P V of the stream's tile before is complete.  (NT = 2 issued S after it.)
+            if (NT == 1 && !(ok = warp_wait(&ctl->pv_done[(g - 2) % NB], ((g - 2) / NB) & 1, p.wait_limit, abort_flag))) break;
             tc_fence_after();
 #pragma unroll 1
             for (int ch = 0; ch < D / 32; ++ch) {
@@ -796,12 +893,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
               acc[e & 1] = f2_add(acc[e & 1], f2_make(p0, p1));
               packed[e] = pack2<BF16>(p0, p1);
             }
-            if constexpr (PC == 8) {
-              tmem_st_32x32b_x8(s_addr + group * (KC / 2) + ch * PC, packed);
-            } else {
-              tmem_st_32x32b_x16(s_addr + group * (KC / 2) + ch * PC, packed);
-            }
-            if (NT == 2 && ch == KC / (4 * PC) - 1) {  // the first half of the keys may be multiplied
+            tmem_st(s_addr + group * (KC / 2) + ch * PC, packed);
+            if (HALVES == 2 && ch == KC / (4 * PC) - 1) {  // the first half of the keys may be multiplied
               tc_wait_st();
               tc_fence_before();
               __syncwarp();
@@ -809,18 +902,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
             }
           }
           if constexpr (KS > 1) {
-            uint32_t zero[PC];
+            uint32_t zero[PC] = {};
 #pragma unroll
-            for (int e = 0; e < PC; ++e) zero[e] = 0;
-#pragma unroll
-            for (int j = 1; j < KS; ++j) {
-              const uint32_t at = s_addr + ((group + j) % KS) * (KC / 2);
-              if constexpr (PC == 8) {
-                tmem_st_32x32b_x8(at, zero);
-              } else {
-                tmem_st_32x32b_x16(at, zero);
-              }
-            }
+            for (int j = 1; j < KS; ++j) tmem_st(s_addr + ((group + j) % KS) * (KC / 2), zero);
           }
           float s0, s1;
           f2_split(f2_add(acc[0], acc[1]), s0, s1);
@@ -831,7 +915,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           if (lane == 0) mbar_arrive(&ctl->p_ready[buf]);
         }
       }
-      if (!ok || (any && !(ok = warp_wait(&ctl->pv_done[i], (g - 1) & 1, p.wait_limit, abort_flag)))) break;
+      if (!ok) break;
+      const int n = w.a1 - w.a0;
+      const int g_last = g0 + (NT == 1 ? ((n - 1 - ((g0 ^ i) & 1)) | 1) - 1 + ((g0 ^ i) & 1) : n - 1);  // of this stream
+      g0 += n;
+      if (any && a_first < w.a1 &&
+          !(ok = warp_wait(&ctl->pv_done[NT == 2 ? i : g_last % NB], (NT == 2 ? g_last : g_last / NB) & 1,
+                           p.wait_limit, abort_flag)))
+        break;
       tc_fence_after();
       const bool done = w.a0 == 0 && w.a1 == u.tiles;
       const bool here = in_tile && t < p.tokens;  // the output has this row
@@ -839,61 +930,94 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           (static_cast<int64_t>(u.b) * p.tokens + t) * p.heads + w.kv_head * p.group + row_head;
       if (!done && w.a0 == 0 && threadIdx.x == 0) {
         const int total = ctl->start[4];
-        const int unit_start = piece_start(blockIdx.x + 1, total, ctas) - w.a1;
+        const int unit_start = piece_start(blockIdx.x + 1, total, ctas) - w.left;
         cut = make_int4(w.item, w.kv_head, piece_of(unit_start + u.tiles - 1, total, ctas), u.live);
       }
-      // Rows leave through shared memory, so that store instructions write whole sectors (a thread writing
-      // its own row 16 bytes at a time took 5 to 9 us per 108 rows).
-      const int64_t slot_row = (2 * static_cast<int64_t>(blockIdx.x) + (w.a0 == 0 ? 1 : 0)) * p.rows + i * BM;
+      const int64_t slot_row = (2 * static_cast<int64_t>(blockIdx.x) + (w.a0 == 0 ? 1 : 0)) * p.rows + (NT == 2 ? i * BM : 0);
+      // O leaves through shared memory, so that store instructions write whole sectors (a thread writing
+      // its own row 16 bytes at a time took 5 to 9 us per 108 rows).  A unit that is cut leaves its sums
+      // and (m, l) in the workspace.  NT = 1: both streams' O are in this warp's lanes; each stream writes
+      // half of the columns of weight0 * O_0 + weight1 * O_1.
+      float weight[2] = {1.0f, 0.0f};
+      uint32_t o_from[2] = {o_addr, o_addr};
+      float mc = m == -INFINITY ? m : m * c, sum = l;
+      if constexpr (NT == 1) {
+        if (u.t0 < u.live) {
+          float2(*ml)[BM] = ctl->ml[units & 1];
+          ml[i][row_lane] = make_float2(mc, l);
+          tc_fence_before();
+          if (!(ok = meet(&ctl->streams, stream_meets))) break;
+          tc_fence_after();
+          mc = -INFINITY;
+          sum = 0.0f;
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+            mc = fmaxf(mc, fmaxf(ml[0][k * GROUP_ROWS + r].x, ml[1][k * GROUP_ROWS + r].x));
+          // 2^(m - max m); a part that saw nothing has m = -inf and l = 0 (or NaN scores: l NaN).
+          auto weigh = [&](float2 x) { return x.x == -INFINITY ? (x.y == x.y ? 0.0f : x.y) : ex2_approx(x.x - mc); };
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float2 x = ml[j][k * GROUP_ROWS + r];
+              sum += weigh(x) * x.y;
+            }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            // A stream without a tile in this unit weighs nothing; the other's O stands in for what it has not.
+            const bool has = n > (((g0 - n) ^ j) & 1);
+            o_from[j] = tmem + lane_off + (has ? C::O_COL(j) : C::O_COL(1 - j));
+            weight[j] = weigh(ml[j][row_lane]);
+          }
+        }
+      }
+      ++units;
+      if (done) {
+        const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;  // NaN stays
+        weight[0] *= inv;
+        weight[1] *= inv;
+      } else if (live && group == 0 && (NT == 2 || i == 0)) {
+        p.part_ml[slot_row + r] = make_float2(mc, sum);
+      }
       if constexpr (KS > 1) {
         if (any) {
-          // Each row's key groups add up: weights 2^(m_k - max m).
-          const float mc = m == -INFINITY ? m : m * c;
-          ctl->ml[group * GROUP_ROWS + r] = make_float2(mc, l);
-          if (!(ok = meet())) break;
-          float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-          for (int k = 0; k < KS; ++k) top = fmaxf(top, ctl->ml[k * GROUP_ROWS + r].x);
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            const float2 x = ctl->ml[k * GROUP_ROWS + r];
-            sum += x.x == -INFINITY ? (x.y == x.y ? 0.0f : x.y) : ex2_approx(x.x - top) * x.y;
-          }
-          const float inv = !done ? 1.0f : sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
-          const float weight = mc == -INFINITY ? (l == l ? 0.0f : l) : ex2_approx(mc - top) * inv;
-          if (!done && live && group == 0) p.part_ml[slot_row + r] = make_float2(top, sum);
-          // 16 columns of every live row and group are staged at a time, or more where few rows leave room.
+          // Each row's key groups add up.  16 columns of every live row and group are staged at a time, or
+          // more where few rows leave room.
           const int rows = min(p.tile_tokens, u.live - u.t0) * p.group;
-          const int at_once = min(D / 16, (4 * 32) / (KS * rows));
-          const int tid = (warp & 3) * 32 + lane;
+          const int at_once = min(D / 32, quotient(128, KS * rows));
+          uint8_t* stage = smem + C::OUT_OFF + i * (4 * 32 * kOutRow);
 #pragma unroll 1
-          for (int c0 = 0; c0 < D / 16 && ok; c0 += at_once) {
-            const int n = min(at_once, D / 16 - c0);
+          for (int c0 = 0; c0 < D / 32 && ok; c0 += at_once) {
+            const int chunks = min(at_once, D / 32 - c0);
 #pragma unroll 1
-            for (int ch = 0; ch < n; ++ch) {
-              uint32_t o[16];
-              tmem_ld_32x32b_x16(o_addr + (c0 + ch) * 16, o);
+            for (int ch = 0; ch < chunks; ++ch) {
+              const uint32_t column = i * (D / 2) + (c0 + ch) * 16;
+              uint32_t o[2][16];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) tmem_ld_32x32b_x16(o_from[j] + column, o[j]);
               tc_wait_ld();
-              float4* to = reinterpret_cast<float4*>(smem + C::OUT_OFF + ((ch * KS + group) * rows + r) * kOutRow);
+              float x[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                x[e] = __uint_as_float(o[0][e]) * weight[0] + __uint_as_float(o[1][e]) * weight[1];
+              float4* to = reinterpret_cast<float4*>(stage + ((ch * KS + group) * rows + r) * kOutRow);
               if (r < rows)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  to[e] = make_float4(__uint_as_float(o[4 * e]) * weight, __uint_as_float(o[4 * e + 1]) * weight,
-                                      __uint_as_float(o[4 * e + 2]) * weight, __uint_as_float(o[4 * e + 3]) * weight);
+                for (int e = 0; e < 4; ++e) to[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
             }
-            if (!(ok = meet())) break;
+            if (!(ok = meet(&ctl->groups[i], group_meets))) break;
             // 4 columns of a row per thread and round
 #pragma unroll 1
-            for (int e = tid; e < n * rows * 4; e += 128) {
+            for (int e = row_lane; e < chunks * rows * 4; e += 128) {
               const int line = e >> 2, ch = quotient(line, rows), row = line - ch * rows;
               float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
               for (int k = 0; k < KS; ++k) {
-                const float4 y = *reinterpret_cast<const float4*>(smem + C::OUT_OFF + ((ch * KS + k) * rows + row) * kOutRow +
-                                                                  (e & 3) * 16);
+                const float4 y =
+                    *reinterpret_cast<const float4*>(stage + ((ch * KS + k) * rows + row) * kOutRow + (e & 3) * 16);
                 x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
               }
-              const int column = (c0 + ch) * 16 + (e & 3) * 4;
+              const int column = i * (D / 2) + (c0 + ch) * 16 + (e & 3) * 4;
               if (done) {
                 const int token = quotient(row, p.group);
                 const int64_t to = (static_cast<int64_t>(u.b) * p.tokens + u.t0 + token) * p.heads +
@@ -903,13 +1027,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
                 *reinterpret_cast<float4*>(p.part + (slot_row + row) * D + column) = x;
               }
             }
-            ok = meet();
+            ok = meet(&ctl->groups[i], group_meets);
           }
           if (!ok) break;
         }
       } else if (any) {
         // Quad n of a warp writes 64 bytes of row 8 e + n.
-        const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // NaN stays
+        constexpr int CHUNKS = NT == 1 ? D / 64 : D / 32;  // of 32 columns
+        const int column0 = NT == 1 ? i * (D / 2) : 0;
         uint8_t* stage = smem + C::OUT_OFF + warp * 32 * kOutRow;
         uint8_t* to[4];
 #pragma unroll
@@ -918,19 +1043,34 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
           const int64_t at = __shfl_sync(0xffffffffu, out_row, row);
           const bool row_live = __shfl_sync(0xffffffffu, static_cast<int>(live), row);
           to[e] = !row_live ? nullptr
-                  : done    ? reinterpret_cast<uint8_t*>(p.o + at * D)
-                            : reinterpret_cast<uint8_t*>(p.part + (slot_row + (warp & 3) * 32 + row) * D);
+                  : done    ? reinterpret_cast<uint8_t*>(p.o + at * D + column0)
+                            : reinterpret_cast<uint8_t*>(p.part + (slot_row + (warp & 3) * 32 + row) * D + column0);
           if (to[e]) to[e] += (lane & 3) * 16;
         }
 #pragma unroll 1
-        for (int ch = 0; ch < D / 32; ++ch) {
+        for (int ch = 0; ch < CHUNKS; ++ch) {
           uint32_t o[32];
-          tmem_ld_32x32b_x32(o_addr + ch * 32, o);
-          tc_wait_ld();
+          if constexpr (NT == 2) {
+            tmem_ld_32x32b_x32(o_addr + ch * 32, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * weight[0]);
+          } else {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              uint32_t x[2][16];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) tmem_ld_32x32b_x16(o_from[j] + column0 + ch * 32 + part * 16, x[j]);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                o[part * 16 + e] =
+                    __float_as_uint(__uint_as_float(x[0][e]) * weight[0] + __uint_as_float(x[1][e]) * weight[1]);
+            }
+          }
           if (done) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              o[e] = pack2<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            for (int e = 0; e < 16; ++e) o[e] = pack2<BF16>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
           }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {  // 16-bit: one half of 64 bytes; fp32: two
@@ -950,13 +1090,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
               }
           }
         }
-        if (live && !done) p.part_ml[slot_row + r] = make_float2(m == -INFINITY ? m : m * c, l);
       }
-      if (done && here && !live && group == 0)
+      if constexpr (NT == 1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->o_free);
+      }
+      if (done && here && !live && group == 0 && (NT == 2 || i == 0))
 #pragma unroll 1
         for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(p.o + out_row * D)[e] = make_uint4(0, 0, 0, 0);
       tc_fence_before();
-    } while (w.next(p, block_tokens));
+    } while (w.next(p, block_tokens, PLACES));
     if (!ok) give_up(ctl, NTL_STATUS_SOFTMAX_WAIT);
     if (threadIdx.x == 0) p.head[blockIdx.x] = cut;
   }
@@ -964,7 +1108,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::CTAS_PER_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == C::MMA_WARP) tmem_dealloc(tmem, C::TMEM_COLS);
+  if (warp == MMA_WARP) tmem_dealloc(tmem, TMEM_COLS);
 }
 
 // Adds up the parts of the unit that CTA blockIdx.x of the attention kernel began and did not end, in
@@ -1114,7 +1258,7 @@ int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, Plan
   n.tile_tokens = static_cast<int>(BM / group < q->tokens ? BM / group : q->tokens);
   const int64_t block_tokens = int64_t(n.row_tiles) * n.tile_tokens;
   const int64_t blocks = (q->tokens + block_tokens - 1) / block_tokens;
-  const int most = n.row_tiles == 1 ? 64 : 128;
+  const int most = n.row_tiles == 1 && c->head_dim == 128 ? Shape<128, 1>::BN : 128;
   if (c->page_size <= most) {
     n.tile_pages = static_cast<int>(most / c->page_size);
     n.tile_keys = static_cast<int>(n.tile_pages * c->page_size);
@@ -1135,8 +1279,7 @@ int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, Plan
   int sms = 0;
   if (int rc = ntl_num_sms(&sms)) return rc;
   const int64_t work = q->seqs * blocks * c->kv_heads * tiles;
-  const int64_t resident = n.row_tiles == 1 ? 2 * sms : sms;
-  n.ctas = static_cast<int>(work < resident ? work : resident);
+  n.ctas = static_cast<int>(work < sms ? work : sms);
   n.part_bytes = static_cast<uint64_t>(2) * n.ctas * n.rows * c->head_dim * 4;
   n.bytes = n.part_bytes + static_cast<uint64_t>(2) * n.ctas * n.rows * 8 + static_cast<uint64_t>(n.ctas) * 16;
   n.bytes = (n.bytes + 15) / 16 * 16;
@@ -1158,12 +1301,12 @@ int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk,
     // The register split must equal what the launch allocates, or the raising warps would wait for
     // registers forever: refuse a build whose register count differs.
     cudaFuncAttributes fa;
-    if (NT == 2 && (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.numRegs != REGS_LAUNCH))
+    if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.numRegs != REGS_LAUNCH)
       return ntl_fail(NTL_ERR_UNSUPPORTED, "%s: kernel compiled with %d registers, the split needs %d", what,
                       fa.numRegs, REGS_LAUNCH);
     done_mask.fetch_or(bit, std::memory_order_release);
   }
-  cudaError_t e = ntl_launch_pdl(kernel, dim3(n.ctas), dim3(Shape<D, NT>::THREADS), smem, s, mq, mk, mv, p);
+  cudaError_t e = ntl_launch_pdl(kernel, dim3(n.ctas), dim3(THREADS), smem, s, mq, mk, mv, p);
   if (e != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   ntl_note_launch();
   if (int rc = ntl_check_launch(what)) return rc;
@@ -1222,9 +1365,11 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   p.blocks = n.blocks;
   p.tile_keys = n.tile_keys;
   p.tile_pages = n.tile_pages;
-  p.tile_shift = -1;
-  for (int i = 3; i < 8; ++i)
+  p.page_shift = p.tile_shift = -1;
+  for (int i = 3; i <= 20; ++i) {
+    if (p.page_size == 1 << i) p.page_shift = i;
     if (n.tile_keys == 1 << i) p.tile_shift = i;
+  }
   p.rows = n.rows;
   p.c = static_cast<float>(q->scale * 1.4426950408889634);
   p.wait_limit = ntl_wait_limit();
