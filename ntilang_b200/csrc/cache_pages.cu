@@ -102,55 +102,60 @@ __global__ void __launch_bounds__(kRowWarps * 32)
   }
 }
 
-// Row prefix + path[i] moves to prefix + i, in place.  One thread owns one 16-byte column of one
-// layer of K or V and walks the path in order: path is increasing, so path[j] >= j > i for every
-// later j and no row is overwritten before it has been read.
-constexpr int kPathUnroll = 8;
+// Row prefix + path[i] moves to prefix + i, in place.  A block takes one layer of one sequence and up to
+// kPathThreads 16-byte columns of its K and V rows; a thread owns one column and walks the path in order:
+// path is increasing, so path[j] >= j > i for every later j and no row is overwritten before it has been
+// read.  Where the rows lie is worked out once per block, a step per thread (every thread for itself
+// costs two dependent loads per step: 12.4 us against 5.5 us for 16 x 27 drafts in 4 layers).
+constexpr int kPathThreads = 256, kPathSteps = 128, kPathUnroll = 8;
 
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kPathThreads)
     accept_kernel(const View c, const int32_t* table, int64_t table_stride, int max_pages, const int32_t* lens,
                   const int32_t* drafts_of, int drafts, const int32_t* path, int64_t path_stride, int path_len,
                   const int32_t* counts, int32_t* lens_out, int seqs) {
+  __shared__ int64_t from[kPathSteps], to[kPathSteps];  // row offsets; from < 0: nothing to move
   pdl_wait();
-  const int units = c.heads * c.chunks;
-  const int64_t jobs = static_cast<int64_t>(c.layers) * seqs * units * 2;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  for (int64_t b = id; b < seqs; b += step) {
-    const int t = drafts_of ? max(drafts_of[b], 0) : drafts;
-    lens_out[b] = max(lens[b] - t, 0) + min(max(counts[b], 0), min(path_len, t));
-  }
-  for (int64_t job = id; job < jobs; job += step) {
-    const int e = static_cast<int>(job % units);
-    int64_t rest = job / units;
-    uint4* base = (rest & 1) ? c.v : c.k;
-    rest >>= 1;
-    const int b = static_cast<int>(rest % seqs), l = static_cast<int>(rest / seqs);
-    const int t = drafts_of ? max(drafts_of[b], 0) : drafts;
-    const int64_t prefix = max(lens[b] - t, 0);
-    const int n = min(max(counts[b], 0), min(path_len, t));
-    const int32_t* row = table + b * table_stride;
-    const int32_t* steps = path + b * path_stride;
-    const int64_t column = (e / c.chunks) * c.head + e % c.chunks;
-    for (int i0 = 0; i0 < n; i0 += kPathUnroll) {
-      uint4 x[kPathUnroll];
-      uint4* to[kPathUnroll];
-#pragma unroll
-      for (int u = 0; u < kPathUnroll; ++u) {
-        const int i = i0 + u;
-        to[u] = nullptr;
-        if (i >= n) continue;
-        const int from = steps[i];
-        if (from < 0 || from >= t || from == i) continue;
-        const int sp = page_of(row, max_pages, c.pages, prefix + from, c.page_size);
-        const int dp = page_of(row, max_pages, c.pages, prefix + i, c.page_size);
-        if (sp < 0 || dp < 0) continue;
-        x[u] = base[row_offset(c, l, sp, static_cast<int>((prefix + from) % c.page_size)) + column];
-        to[u] = base + row_offset(c, l, dp, static_cast<int>((prefix + i) % c.page_size)) + column;
+  const int units = c.heads * c.chunks, columns = 2 * units;
+  const int slices = max((columns + kPathThreads - 1) / kPathThreads, 1);
+  const int64_t job = blockIdx.x / slices;
+  const int b = static_cast<int>(job % seqs), l = static_cast<int>(job / seqs);
+  const int column = (blockIdx.x % slices) * kPathThreads + threadIdx.x;
+  const int len = max(lens[b], 0), t = drafts_of ? max(drafts_of[b], 0) : drafts;
+  const int prefix = max(len - t, 0);
+  const int n = min(max(counts[b], 0), min(path_len, t));
+  if (l == 0 && column == 0) lens_out[b] = prefix + n;
+  if (c.layers == 0 || units == 0) return;  // nothing to move
+  const int32_t* row = table + b * table_stride;
+  const int e = column < units ? column : column - units;
+  uint4* base = (column < units ? c.k : c.v) + (e / c.chunks) * c.head + e % c.chunks;
+  for (int i0 = 0; i0 < n; i0 += kPathSteps) {
+    const int steps = min(kPathSteps, n - i0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < steps; i += kPathThreads) {
+      const int src = path[b * path_stride + i0 + i], dst = i0 + i;
+      int64_t a = -1, z = 0;
+      if (src >= 0 && src < t && src != dst) {
+        const int64_t sp = static_cast<int64_t>(prefix) + src, dp = static_cast<int64_t>(prefix) + dst;
+        const int s_page = page_of(row, max_pages, c.pages, sp, c.page_size);
+        const int d_page = page_of(row, max_pages, c.pages, dp, c.page_size);
+        if (s_page >= 0 && d_page >= 0) {
+          a = row_offset(c, l, s_page, static_cast<int>(sp % c.page_size));
+          z = row_offset(c, l, d_page, static_cast<int>(dp % c.page_size));
+        }
       }
+      from[i] = a;
+      to[i] = z;
+    }
+    __syncthreads();
+    if (column >= columns) continue;
+    for (int j0 = 0; j0 < steps; j0 += kPathUnroll) {
+      uint4 x[kPathUnroll];
 #pragma unroll
       for (int u = 0; u < kPathUnroll; ++u)
-        if (to[u]) *to[u] = x[u];
+        if (j0 + u < steps && from[j0 + u] >= 0) x[u] = base[from[j0 + u]];
+#pragma unroll
+      for (int u = 0; u < kPathUnroll; ++u)
+        if (j0 + u < steps && from[j0 + u] >= 0) base[to[j0 + u]] = x[u];
     }
   }
 }
@@ -542,13 +547,14 @@ extern "C" int ntl_cache_accept(const ntl_cache_t* cache, const int32_t* table, 
   NTL_REQUIRE(lens && lens_out && counts, NTL_ERR_INVALID, "cache accept: NULL lengths or counts");
   NTL_REQUIRE(lens != lens_out, NTL_ERR_INVALID, "cache accept: lens_out must not be lens");
   NTL_REQUIRE(path_len == 0 || path, NTL_ERR_INVALID, "cache accept: NULL path");
-  unsigned grid;
-  if (int rc = grid_for(static_cast<int64_t>(c.layers) * seqs * c.heads * c.chunks * 2, 128, &grid)) return rc;
+  const int64_t slices = (2ll * c.heads * c.chunks + kPathThreads - 1) / kPathThreads;
+  const int64_t blocks = (c.layers > 0 ? c.layers : 1) * seqs * (slices > 0 ? slices : 1);
+  NTL_REQUIRE(blocks < (int64_t(1) << 31), NTL_ERR_UNSUPPORTED, "cache accept: too large");
   return launched("cache accept",
-                  ntl_launch_pdl(accept_kernel, dim3(grid), dim3(128), 0, static_cast<cudaStream_t>(stream), c, table,
-                                 table_stride, static_cast<int>(max_pages), lens, drafts_of, static_cast<int>(drafts),
-                                 path, path_stride, static_cast<int>(path_len), counts, lens_out,
-                                 static_cast<int>(seqs)));
+                  ntl_launch_pdl(accept_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPathThreads), 0,
+                                 static_cast<cudaStream_t>(stream), c, table, table_stride, static_cast<int>(max_pages),
+                                 lens, drafts_of, static_cast<int>(drafts), path, path_stride,
+                                 static_cast<int>(path_len), counts, lens_out, static_cast<int>(seqs)));
 }
 
 extern "C" int ntl_cache_copy_pages(const ntl_cache_t* cache, const int32_t* src, const int32_t* dst, int64_t n,

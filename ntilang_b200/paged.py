@@ -38,6 +38,7 @@ _TWO = struct.Struct("=2q")
 _FIVE = struct.Struct("=5q")
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _empty, _empty_like, _uint8 = torch.empty, torch.empty_like, torch.uint8
 
 
@@ -45,13 +46,39 @@ def _stream(index):
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
+_functions: dict = {}
+
+
 def _call(index, name, *args):
-    """The entry point ``name`` on device ``index``'s current stream."""
-    if index == torch.cuda.current_device():
-        _lib.call(name, *args, _stream(index))
+    """The entry point ``name`` on device ``index``'s current stream; a non-zero return raises ``KernelError``."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_lib.lib(), name)
+    if index == _current_device():
+        code = fn(*args, _stream(index))
     else:
         with torch.cuda.device(index):
-            _lib.call(name, *args, _stream(index))
+            code = fn(*args, _stream(index))
+    if code:
+        raise _lib.KernelError(name, code, (_lib.lib().ntl_last_error() or b"").decode())
+
+
+_workspaces: dict = {}
+
+
+def _workspace(index, size, device):
+    """At least ``size`` bytes for a call on device ``index``'s current stream.  Calls on one stream follow each
+    other, so they share a buffer; a call that is captured in a graph, which may be replayed on any stream,
+    gets its own."""
+    if torch.cuda.is_current_stream_capturing():
+        return _empty(size, dtype=_uint8, device=device)
+    key = (index, _stream(index))
+    work = _workspaces.get(key)
+    if work is None or work.numel() < size:
+        if len(_workspaces) >= 64:
+            _workspaces.clear()
+        work = _workspaces[key] = _empty(size, dtype=_uint8, device=device)
+    return work
 
 
 # ------------------------------------------------------------------------------ argument checks
@@ -63,14 +90,16 @@ def _call(index, name, *args):
 _plans: dict = {}
 
 
-def _form(x):
-    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
-
-
 def _plan(check, tensors, *values):
     """``check(*tensors, *values)``, or what it returned for arguments of the same form."""
+    key = [check, *values]
     try:
-        key = (check, *map(_form, tensors), *values)
+        for x in tensors:
+            if x is not None:
+                key += (x.shape, x.stride(), x.dtype, x.get_device())
+            else:
+                key.append(None)
+        key = tuple(key)
         plan = _plans.get(key)
     except (AttributeError, TypeError, RuntimeError):  # not tensors, or not hashable: the check says so
         return check(*tensors, *values)
@@ -152,7 +181,7 @@ def _pool_workspace(pages, n):
 # ------------------------------------------------------------------------------ attention
 
 
-def _check_attention(q, k, v, table, lens, q_lens, scale):
+def _check_attention(q, k, v, table, lens, q_lens, tree, scale):
     cache, index = _check_cache(k, v, (4,), False)
     _values("q", q)
     shape, kv = q.shape, k.shape
@@ -173,6 +202,14 @@ def _check_attention(q, k, v, table, lens, q_lens, scale):
     _ints("lens", lens, index, seqs)
     if q_lens is not None:
         _ints("q_lens", q_lens, index, seqs)
+    tree_stride = 0
+    if tree is not None:
+        words = (tokens + 31) // 32
+        shared = isinstance(tree, torch.Tensor) and tree.dim() == 3 and tree.shape[0] == 1
+        _ints("tree", tree, index, 1 if shared else seqs, tokens, words)
+        if tokens > 1 and tree.stride(1) != words:
+            raise ValueError("tree must be dense along its last two dimensions")
+        tree_stride = 0 if shared else tree.stride(0)
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
     elif not 0 < scale < 1e30:
@@ -185,7 +222,7 @@ def _check_attention(q, k, v, table, lens, q_lens, scale):
             _lib.call("ntl_cache_attention_workspace", _TWO.pack(16, 16) + cache, _FIVE.pack(16, 16, 16, 16, 0) + query,
                       ctypes.byref(out))
         size = out.value
-    return cache, query, index, size, q.is_contiguous(), q.device
+    return cache, query, index, size, q.is_contiguous(), q.device, tree_stride
 
 
 def _check_out(out, q, k, v):
@@ -201,8 +238,8 @@ def _check_out(out, q, k, v):
                 raise ValueError(f"Tensor arguments {name} and out must have disjoint storage")
 
 
-def _attend(entry, q, k, v, table, lens, q_lens, scale, out, *args):
-    cache, query, index, size, dense, device = _plan(_check_attention, (q, k, v, table, lens, q_lens), scale)
+def _attend(q, k, v, table, lens, q_lens, scale, out, tree, window, sinks):
+    cache, query, index, size, dense, device, tree_stride = _plan(_check_attention, (q, k, v, table, lens, q_lens, tree), scale)
     qp = q.data_ptr()
     if qp & 15:
         _aligned(q=q)
@@ -212,10 +249,13 @@ def _attend(entry, q, k, v, table, lens, q_lens, scale, out, *args):
         _check_out(out, q, k, v)
     if not size:
         return out
-    work = _empty(size, dtype=_uint8, device=device)
+    work = _workspace(index, size, device)
     query = _FIVE.pack(qp, out.data_ptr(), table.data_ptr(), lens.data_ptr(),
                        0 if q_lens is None else q_lens.data_ptr()) + query
-    _call(index, entry, _cache(k, v, cache), query, *args, work.data_ptr(), size)
+    if tree is None:
+        _call(index, "ntl_window_attention", _cache(k, v, cache), query, window, sinks, work.data_ptr(), size)
+    else:
+        _call(index, "ntl_tree_attention", _cache(k, v, cache), query, tree.data_ptr(), tree_stride, work.data_ptr(), size)
     return out
 
 
@@ -225,22 +265,6 @@ def _check_parents(parents):
     index = parents.get_device()
     _ints("parents", parents, index, None, None)
     return index, (parents.shape[0], parents.shape[1], (parents.shape[1] + 31) // 32), parents.device
-
-
-def _check_tree(tree, q):
-    if not isinstance(tree, torch.Tensor) or tree.dim() != 3:
-        raise TypeError("tree must be a CUDA tensor [seqs or 1, tokens, words]")
-    if not isinstance(q, torch.Tensor) or not q.is_cuda:
-        raise TypeError("q must be a CUDA tensor")
-    if q.dim() != 4:
-        raise ValueError(f"q: expected 4 dimensions [seqs, tokens, heads, head_dim], got shape {tuple(q.shape)}")
-    seqs, tokens = q.shape[:2]
-    words = (tokens + 31) // 32
-    shared = tree.shape[0] == 1
-    _ints("tree", tree, q.get_device(), 1 if shared else seqs, tokens, words)
-    if tokens > 1 and tree.stride(1) != words:
-        raise ValueError("tree must be dense along its last two dimensions")
-    return 0 if shared else tree.stride(0)
 
 
 def tree_mask(parents):
@@ -266,8 +290,9 @@ def tree_attention(q, k, v, table, lens, tree, *, q_lens=None, scale=None, out=N
     Statistics and sums are fp32; the exponentials are rounded to the cache's type for the product
     with V.  A NaN or infinity in a key row reaches the tokens that see it; in a value row that some token
     of the call sees, it may reach tokens of the same sequence that do not."""
-    stride = _plan(_check_tree, (tree, q))
-    return _attend("ntl_tree_attention", q, k, v, table, lens, q_lens, scale, out, tree.data_ptr(), stride)
+    if tree is None:
+        raise TypeError("tree must be a CUDA tensor")
+    return _attend(q, k, v, table, lens, q_lens, scale, out, tree, 0, 0)
 
 
 def window_attention(q, k, v, table, lens, window, sinks=0, *, q_lens=None, scale=None, out=None):
@@ -279,7 +304,7 @@ def window_attention(q, k, v, table, lens, window, sinks=0, *, q_lens=None, scal
     window, sinks = int(window), int(sinks)
     if window < 1 or sinks < 0:
         raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
-    return _attend("ntl_window_attention", q, k, v, table, lens, q_lens, scale, out, window, sinks)
+    return _attend(q, k, v, table, lens, q_lens, scale, out, None, window, sinks)
 
 
 # ------------------------------------------------------------------------------ cache operators
@@ -389,7 +414,7 @@ def fork(k, v, table, lens, refs, src, dst):
     page was left and the child holds nothing."""
     cache, index, sizes, n, size, device = _plan(_check_fork, (k, v, table, lens, refs, src, dst))
     granted = _empty(n, dtype=torch.int32, device=device)
-    work = _empty(size, dtype=_uint8, device=device)
+    work = _workspace(index, size, device)
     _call(index, "ntl_cache_fork", _cache(k, v, cache), table.data_ptr(), *sizes, lens.data_ptr(), refs.data_ptr(),
           src.data_ptr(), dst.data_ptr(), n, granted.data_ptr(), work.data_ptr(), size)
     return granted
@@ -415,7 +440,7 @@ def reserve(table, lens, refs, seqs, extra, page_size):
     each, common = (extra, 0) if isinstance(extra, torch.Tensor) else (None, int(extra))
     index, sizes, n, pages, size, device = _plan(_check_reserve, (table, lens, refs, seqs, each), common, int(page_size))
     granted = _empty(n, dtype=torch.int32, device=device)
-    work = _empty(size, dtype=_uint8, device=device)
+    work = _workspace(index, size, device)
     _call(index, "ntl_cache_reserve", pages, int(page_size), table.data_ptr(), *sizes, lens.data_ptr(), refs.data_ptr(),
           seqs.data_ptr(), n, common, None if each is None else each.data_ptr(), granted.data_ptr(), work.data_ptr(),
           size)
@@ -451,7 +476,7 @@ def compact(k, v, table, refs, *, table_out=None, refs_out=None):
     refs_out = refs if refs_out is None else refs_out
     cache, index, shape, size, device = _plan(_check_compact, (k, v, table, refs, table_out, refs_out))
     live = _empty(1, dtype=torch.int32, device=device)
-    work = _empty(size, dtype=_uint8, device=device)
+    work = _workspace(index, size, device)
     _call(index, "ntl_cache_compact", _cache(k, v, cache), table.data_ptr(), table.stride(0), table_out.data_ptr(),
           table_out.stride(0), *shape, refs.data_ptr(), refs_out.data_ptr(), live.data_ptr(), work.data_ptr(), size)
     return live
