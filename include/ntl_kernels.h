@@ -165,9 +165,9 @@ int ntl_fa2_set_causal_grid(int mode);
  * A cache is [layers, pages, page_size, kv_heads, head_dim] values of 16 bits; K and V have the same
  * strides (in values, multiples of 8), and head_dim is dense.  A sequence is a row of a page table
  * (int32 page numbers, -1 = no page) and a length in tokens (int32, device memory).  Page numbers
- * and lengths are read on the device: what is out of range is skipped, a length is cut to
- * max_pages * page_size, and a position without a page is not visible and takes no row.  All
- * entry points work in stream order; those with a workspace take one of the size that the matching
+ * and lengths are read on the device: what is out of range is skipped, and a length is cut to
+ * max_pages * page_size.  Attention reads a position without a page as a key and value of zeros; a row
+ * written there is dropped.  All entry points work in stream order; those with a workspace take one of the size that the matching
  * size function gives, which calls on different streams must not share. */
 enum { NTL_F16 = 0, NTL_BF16 = 1 };
 

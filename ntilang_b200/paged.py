@@ -494,6 +494,14 @@ class Cache:
         self.lens = torch.zeros(seqs, dtype=torch.int32, device=device)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
 
+    def part(self, seqs):
+        """A cache over some of the sequences (a slice of the slots): the same pool and its rows of the table; its
+        lengths are its own from here on."""
+        part = object.__new__(Cache)
+        part.k, part.v, part.refs = self.k, self.v, self.refs
+        part.table, part.lens = self.table[seqs], self.lens[seqs].clone()
+        return part
+
     def reserve(self, seqs, extra):
         return reserve(self.table, self.lens, self.refs, seqs, extra, self.k.shape[2])
 

@@ -742,3 +742,15 @@ def test_a_serving_round(torch_cuda):
     assert live == int((c.refs > 0).sum()) and int(c.table.max()) < live
     again = c.window_attention(1, one, 20, 4)
     assert torch.equal(again[2:], out[2:]) and not again[:2].any()
+
+
+def test_speculative_decoding_example(torch_cuda):
+    """The example runs the operators together and checks its text against plain decoding itself."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "speculative_decode.py"
+    spec = importlib.util.spec_from_file_location("speculative_decode", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(seqs=3, prompt_len=45, steps=30) <= 31
