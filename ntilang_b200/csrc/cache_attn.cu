@@ -20,7 +20,9 @@
 // streams of four warps, so that one stream's tensor work overlaps the other's exponentials:
 //   NT = 1: one 128-row tile; the streams take alternate key tiles of the same rows, each with its own
 //           (o, m, l), and merge at the unit's end.  For up to 128 rows: decode and small trees, bound by
-//           HBM.  Up to 32 rows are copied to four lane groups that take a quarter of each key tile each.
+//           HBM.  Up to 16 rows (KS = 4 key groups) are copied to the four quarters of a 64-row MMA, and
+//           each softmax warp takes a quarter of the key tile: a quarter of the exponentials per
+//           warp, half of the tensor work.
 //           Tiles are 64 keys with four S buffers at head_dim 128 (3 to 6% faster than 128 keys, whose ring is
 //           only 2 + 3 tiles deep) and 128 keys with three at head_dim 64 (64 keys: 13% slower, each
 //           Q K^T reads all of Q from shared memory, however few keys it covers).
@@ -337,8 +339,8 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16])
 
 // kind::f16 instruction descriptor (see umma_idesc_f16_f32) with both operands fp16 or both bf16.
 template <bool BF16>
-__host__ __device__ constexpr uint32_t idesc(uint32_t n, uint32_t b_mn_major) {
-  return umma_idesc_f16_f32(BM, n, 0, b_mn_major) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+__host__ __device__ constexpr uint32_t idesc(uint32_t m, uint32_t n, uint32_t b_mn_major) {
+  return umma_idesc_f16_f32(m, n, 0, b_mn_major) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
 }
 
 // umma_desc_sw128 as its low word and a constant high word: the descriptor of an operand `bytes` further on
@@ -409,8 +411,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   constexpr int BN = C::BN, NB = C::BUFFERS;
   // Hand P over in halves: with 128 keys and no key groups (which finish together).
   constexpr int HALVES = KS == 1 && BN == 128 ? 2 : 1;
-  constexpr int KC = BN / KS;          // keys of a tile per key group
-  constexpr int GROUP_ROWS = BM / KS;  // rows of the tile per key group
+  constexpr int M = KS == 1 ? BM : 64;  // rows of an MMA; 64 rows lie in the first half of each 32 TMEM lanes
+  constexpr int KC = BN / KS;           // keys of a tile per key group
+  constexpr int GROUP_ROWS = BM / KS;   // TMEM lanes per key group
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL_OFF);
@@ -480,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int i = 0; i < NT * KS; ++i)
 #pragma unroll
         for (int d = 0; d < D / 64; ++d)
-          tma_load_4d(smem + (NT == 2 ? i * C::Q_BYTES : i * GROUP_ROWS * 128) + d * (BM * 128), &tq, &ctl->q_full, d * 64,
+          tma_load_4d(smem + (NT == 2 ? i * C::Q_BYTES : i * (M / KS) * 128) + d * (M * 128), &tq, &ctl->q_full, d * 64,
                       w.kv_head * p.group, w.u.t0 + (NT == 2 ? i * p.tile_tokens : 0), w.u.b);
     };
     // One warp: zeros over the rows of V stage s past the sequence's end, for the MMAs issued after it.
@@ -610,8 +613,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     } else if ((NT == 1 && warp == AUX_WARP) || elect_one_lane()) {
       // ---------------------------------------------- MMA issue (one lane; NT = 1 has its whole P V warp here)
-      constexpr uint32_t idesc_s = idesc<BF16>(BN, 0);  // B = K tile, K-major
-      constexpr uint32_t idesc_o = idesc<BF16>(D, 1);   // B = V tile, N-major
+      constexpr uint32_t idesc_s = idesc<BF16>(M, BN, 0);  // B = K tile, K-major
+      constexpr uint32_t idesc_o = idesc<BF16>(M, D, 1);   // B = V tile, N-major
       const uint32_t q_low = desc_low(smem_u32(smem), 16);
       const uint32_t k_low = desc_low(smem_u32(smem + C::K_OFF), 16);
       const uint32_t v_low = desc_low(smem_u32(smem + C::V_OFF), BN * 128);
@@ -630,7 +633,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          tc_mma_f16_ss(tmem + C::S_COL(i), desc_at(q, (kk >> 2) * (BM * 128) + (kk & 3) * 32),
+          tc_mma_f16_ss(tmem + C::S_COL(i), desc_at(q, (kk >> 2) * (M * 128) + (kk & 3) * 32),
                         desc_at(k, (kk >> 2) * (BN * 128) + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
         tc_commit(&ctl->s_full[i]);
       };
@@ -1272,9 +1275,11 @@ int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, Plan
       }
   }
   n.rows = n.row_tiles == 1 ? static_cast<int>(q->tokens * group) : 2 * BM;
-  const int64_t tiles = q->max_pages * c->page_size / n.tile_keys + 2;  // of one unit, at most
+  // Places of the line that one unit takes, at most.
+  const int64_t tiles = q->max_pages * c->page_size / n.tile_keys + 2 + kUnitPlaces<1>;
   NTL_REQUIRE(q->seqs * blocks < (int64_t(1) << 31) / c->kv_heads / tiles, NTL_ERR_UNSUPPORTED,
               "%s: more than 2^31 tiles of keys", what);
+  static_assert(kUnitPlaces<1> >= kUnitPlaces<2>, "the bound above");
   n.blocks = static_cast<int>(blocks);
   int sms = 0;
   if (int rc = ntl_num_sms(&sms)) return rc;
@@ -1373,18 +1378,20 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   p.rows = n.rows;
   p.c = static_cast<float>(q->scale * 1.4426950408889634);
   p.wait_limit = ntl_wait_limit();
+  // Key groups for up to 16 rows: 64 sequences x 1 token x 4 heads per key head, window 4096: 175 us against
+  // 197 us without (back to back, at the power cap).  Four groups of up to 32 rows need the 128-row MMA
+  // and measured slower than none at head_dim 128 (32 x 8 drafts over 8192 tokens: 213 against 201 us).
 #define NTL_CACHE_ATTN(D, NT, KS)                                          \
   return bf16 ? launch_shape<D, NT, KS, true>(what, mq, mk, mv, p, n, s) \
               : launch_shape<D, NT, KS, false>(what, mq, mk, mv, p, n, s)
-  const int groups = n.row_tiles == 2 ? 0 : n.rows <= 32 ? 4 : 1;
   if (dim == 64) {
-    if (groups == 4) NTL_CACHE_ATTN(64, 1, 4);
-    if (groups == 1) NTL_CACHE_ATTN(64, 1, 1);
-    NTL_CACHE_ATTN(64, 2, 1);
+    if (n.row_tiles == 2) NTL_CACHE_ATTN(64, 2, 1);
+    if (n.rows <= 16) NTL_CACHE_ATTN(64, 1, 4);
+    NTL_CACHE_ATTN(64, 1, 1);
   }
-  if (groups == 4) NTL_CACHE_ATTN(128, 1, 4);
-  if (groups == 1) NTL_CACHE_ATTN(128, 1, 1);
-  NTL_CACHE_ATTN(128, 2, 1);
+  if (n.row_tiles == 2) NTL_CACHE_ATTN(128, 2, 1);
+  if (n.rows <= 16) NTL_CACHE_ATTN(128, 1, 4);
+  NTL_CACHE_ATTN(128, 1, 1);
 #undef NTL_CACHE_ATTN
 }
 
