@@ -3,7 +3,8 @@
 ``python -m ntilang_b200.build`` (or ``__graft_entry__.build()``) compiles every
 ``csrc/*.cu`` to an object under ``ntilang_b200/_build/`` and links
 ``ntilang_b200/libntl_kernels.so``.  The library is plain C ABI (``include/ntl_kernels.h``);
-Python reaches it through ctypes (``ntilang_b200._lib``).
+Python reaches it through ctypes (``ntilang_b200._lib``).  Where torch is installed it also builds
+``csrc/paged_binding.cpp`` into ``ntilang_b200/_paged.so``, the module behind ``ntilang_b200.paged``.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libntl_kernels.so"
+BINDING = PKG / "_paged.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
               "--expt-relaxed-constexpr", f"-I{ROOT / 'include'}"]
@@ -42,10 +44,41 @@ def _stale(target: Path, deps) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> Path | None:
+    """``_paged.so``, linked to the library and to torch's; None where torch is not installed."""
+    import importlib.util
+    import sysconfig
+
+    if importlib.util.find_spec("torch") is None:
+        return None
+    src = CSRC / "paged_binding.cpp"
+    if not force and not _stale(BINDING, [src, ROOT / "include" / "ntl_kernels.h", Path(__file__)]):
+        return BINDING
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    cuda = Path(nvcc_path()).resolve().parents[1]
+    lib = Path(torch.__file__).parent / "lib"
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{sysconfig.get_paths()['include']}",
+           *(f"-isystem{p}" for p in include_paths()), f"-isystem{cuda / 'include'}", str(src), "-o", str(tmp),
+           f"-L{PKG}", "-l:libntl_kernels.so", f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("building _paged.so failed:\n" + res.stdout + res.stderr)
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build_library(force: bool = False, verbose: bool = False) -> Path:
     headers = list(CSRC.glob("*.cuh")) + [ROOT / "include" / "ntl_kernels.h"]
     srcs = sources()
     if not force and not _stale(LIB, srcs + headers + [Path(__file__)]):
+        build_binding(verbose=verbose)
         return LIB
     nvcc = nvcc_path()
     BUILD.mkdir(exist_ok=True)
@@ -75,6 +108,7 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError("link failed:\n" + res.stdout + res.stderr)
     os.replace(tmp, LIB)
+    build_binding(force, verbose)
     return LIB
 
 

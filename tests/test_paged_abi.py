@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import pytest
 
@@ -10,23 +11,19 @@ PTR = 1 << 20  # never read: every call below is refused, or has nothing to do
 
 
 def cache(**change):
-    from ntilang_b200 import paged
-
     names = ["k", "v", "layers", "pages", "page_size", "kv_heads", "head_dim", "layer_stride", "page_stride",
              "row_stride", "head_stride", "dtype"]
     values = dict(zip(names, [PTR, PTR, 1, 10, 16, 2, 64, 0, 2048, 128, 64, 0]))
     assert set(change) <= set(names)
-    return paged._CACHE.pack(*{**values, **change}.values())
+    return struct.pack("=12q", *{**values, **change}.values())
 
 
 def query(**change):
-    from ntilang_b200 import paged
-
     names = ["q", "o", "table", "lens", "q_lens", "seqs", "tokens", "heads", "seq_stride", "token_stride", "head_stride",
              "table_stride", "max_pages", "scale"]
     values = dict(zip(names, [PTR, PTR, PTR, PTR, 0, 2, 3, 4, 768, 256, 64, 8, 8, 0.125]))
     assert set(change) <= set(names)
-    return paged._QUERY.pack(*{**values, **change}.values())
+    return struct.pack("=13qd", *{**values, **change}.values())
 
 
 @pytest.fixture(scope="module")
