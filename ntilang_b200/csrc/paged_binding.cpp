@@ -1,7 +1,8 @@
 // Python binding of the paged cache's entry points (the module ntilang_b200._paged behind
 // ntilang_b200/paged.py): argument checks, output and workspace allocation, and the C-ABI call on torch's
-// current stream.  In C++ because a call's checks in Python took longer than its kernels on small problems
-// (window attention of one token: 24 us of host time, 8 here).
+// current stream.  In C++ because small calls waited for their checks in Python and the ctypes conversions: host
+// time of a window attention 14 -> 8 us, of an append and an accept 22 -> 10, of a tree's mask and attention
+// 21 -> 12, against 8 to 15 us on the device at their smallest.
 //
 // The C ABI itself is libntl_kernels.so, which this module links; nothing here launches kernels.
 #include <ATen/core/Tensor.h>
