@@ -15,6 +15,7 @@
 // runs its piece as one stream of tiles; a unit inside one piece is finished there, a unit cut between
 // pieces leaves (o, m, l) parts in the workspace that cache_attn_join adds up in order.  So ragged
 // lengths balance by themselves, from lengths that only the device knows.
+// Where the sizes say that units are short (few_tiles), pieces begin at units and none is cut.
 //
 // Two shapes of CTA (one per SM), chosen by the rows a unit has (see launch()).  Both run two softmax
 // streams of four warps, so that one stream's tensor work overlaps the other's exponentials:
@@ -71,6 +72,7 @@ struct AttnParams {
   int page_shift;    // log2 of page_size, -1 if it is no power of two
   int tile_shift;    // log2 of tile_keys, the same
   int rows;          // rows a workspace slot has
+  int whole;         // no unit is cut: a CTA takes those that begin in its piece
   float c;           // softmax scale in log2 units
   int64_t wait_limit;
 };
@@ -306,7 +308,7 @@ struct Walk {
     left = ctl->start[3];
     u = ctl->unit;
     a0 = place;
-    a1 = min(u.tiles, a0 + left);
+    a1 = p.whole ? (a0 > 0 ? a0 : u.tiles) : min(u.tiles, a0 + left);
     return a0 < a1 || next(p, block_tokens, places);
   }
   __device__ __forceinline__ bool next(const AttnParams& p, int block_tokens, int places) {
@@ -317,7 +319,7 @@ struct Walk {
       u = unit_of(p, ++item, block_tokens);
     }
     place = a0 = 0;
-    a1 = min(u.tiles, left);
+    a1 = p.whole ? u.tiles : min(u.tiles, left);
     return true;
   }
 };
@@ -1251,13 +1253,25 @@ int make_map(CUtensorMap* map, const char* what, const void* base, bool bf16, co
   return NTL_OK;
 }
 
+// Units of few tiles are not cut, which saves the join: its launch, and for two row tiles ~15 us where every CTA
+// cuts one.  That many tiles in a row must not take longer: at most 8 of 64 keys (30 x 3 tokens, window 40: 13.4 ->
+// 10.6 us; 18 x 1 token over 255 to 482 keys in pages of 8, 8 tiles: 12.8 -> 14.9), 6 of 128 keys; two row tiles as
+// long as the CTA with the most units has at most 4 more tiles than the mean (4 x 512 tokens, window 512, 8 tiles,
+// 1.7 units a CTA: 58.5 -> 41.4 us; 12 x 29 tokens over 351 to 672 keys, 6 tiles, 0.08 units: 20.4 -> 25.4).
+bool few_tiles(int row_tiles, int tile_keys, int64_t tiles, int64_t units, int64_t sms) {
+  if (tiles > (row_tiles == 1 && tile_keys > 64 ? 6 : 8)) return false;
+  return row_tiles == 1 || ((units + sms - 1) / sms * sms - units) * tiles <= 4 * sms;
+}
+
 // What the sizes decide: the shape of CTA, the grid and the workspace.
 struct Plan {
   int row_tiles, tile_tokens, blocks, tile_keys, tile_pages, rows, ctas;
+  bool whole;
   uint64_t part_bytes, bytes;
 };
 
-int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, Plan* plan) {
+// `sees`: keys that a token sees at most, besides the first `sinks`.
+int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, int64_t sees, int64_t sinks, Plan* plan) {
   const int64_t group = q->heads / c->kv_heads;
   Plan& n = *plan;
   n.row_tiles = q->tokens * group > BM ? 2 : 1;
@@ -1288,6 +1302,10 @@ int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, Plan
   if (int rc = ntl_num_sms(&sms)) return rc;
   const int64_t work = q->seqs * blocks * c->kv_heads * tiles;
   n.ctas = static_cast<int>(work < sms ? work : sms);
+  const int64_t keys = q->max_pages * c->page_size, k = n.tile_keys;
+  const int64_t span = sees + block_tokens - 1 < keys ? sees + block_tokens - 1 : keys;
+  const int64_t all = (keys + k - 1) / k, seen = (span + k - 2) / k + 1 + (sinks < keys ? sinks + k - 1 : keys) / k;
+  n.whole = few_tiles(n.row_tiles, n.tile_keys, seen < all ? seen : all, q->seqs * blocks * c->kv_heads, sms);
   n.part_bytes = static_cast<uint64_t>(2) * n.ctas * n.rows * c->head_dim * 4;
   n.bytes = n.part_bytes + static_cast<uint64_t>(2) * n.ctas * n.rows * 8 + static_cast<uint64_t>(n.ctas) * 16;
   n.bytes = (n.bytes + 15) / 16 * 16;
@@ -1318,7 +1336,7 @@ int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk,
   if (e != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   ntl_note_launch();
   if (int rc = ntl_check_launch(what)) return rc;
-  if (n.ctas == 1) return NTL_OK;  // one piece: no unit is cut
+  if (n.ctas == 1 || n.whole) return NTL_OK;  // no unit is cut
   const int join_rows = n.rows > 64 ? 4 : 1;
   const unsigned chunks = static_cast<unsigned>((n.rows + kJoinWarps * join_rows - 1) / (kJoinWarps * join_rows));
   e = ntl_launch_pdl(join_rows == 4 ? cache_attn_join<D, 4, BF16> : cache_attn_join<D, 1, BF16>,
@@ -1331,7 +1349,7 @@ int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk,
 int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const uint32_t* tree, int64_t tree_stride,
            int64_t window, int64_t sinks, void* workspace, uint64_t workspace_bytes, cudaStream_t s) {
   Plan n;
-  if (int rc = make_plan(what, c, q, &n)) return rc;
+  if (int rc = make_plan(what, c, q, tree ? int64_t(1) << 31 : window, tree ? 0 : sinks, &n)) return rc;
   NTL_REQUIRE(workspace && workspace_bytes >= n.bytes && ntl_aligned(workspace, 16), NTL_ERR_INVALID,
               "%s: workspace of %llu bytes, %llu needed (16-byte aligned)", what, (unsigned long long)workspace_bytes,
               (unsigned long long)n.bytes);
@@ -1379,6 +1397,7 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
     if (n.tile_keys == 1 << i) p.tile_shift = i;
   }
   p.rows = n.rows;
+  p.whole = n.whole;
   p.c = static_cast<float>(q->scale * 1.4426950408889634);
   p.wait_limit = ntl_wait_limit();
   // Key groups for up to 16 rows: 64 sequences x 1 token x 4 heads per key head, window 4096: 175 us against
@@ -1444,7 +1463,7 @@ extern "C" int ntl_cache_attention_workspace(const ntl_cache_t* cache, const ntl
   *bytes_out = 0;
   if (query->seqs == 0 || query->tokens == 0 || query->heads == 0) return NTL_OK;
   Plan n;
-  if (int rc = make_plan("cache attention", cache, query, &n)) return rc;
+  if (int rc = make_plan("cache attention", cache, query, int64_t(1) << 31, 0, &n)) return rc;
   *bytes_out = n.bytes;
   return NTL_OK;
 }

@@ -162,6 +162,32 @@ def test_many_units(torch_cuda, kind, dtype, dim, seqs, kv_heads, group, tokens,
         assert torch.equal(out, first)
 
 
+# Short units are not cut between CTAs where the table's width or the window says that they are short: both
+# ways on the same keys, with as many units as CTAs, fewer and more.
+@pytest.mark.parametrize("dtype,dim,seqs,kv_heads,group,tokens,longest", [
+    ("float16", 128, 7, 2, 4, 3, 500), ("bfloat16", 64, 90, 4, 3, 2, 750), ("float16", 64, 5, 2, 8, 20, 400),
+    ("bfloat16", 128, 20, 3, 2, 30, 512), ("float16", 128, 3, 4, 4, 130, 480), ("bfloat16", 64, 40, 8, 3, 100, 900),
+])
+def test_short_units(torch_cuda, dtype, dim, seqs, kv_heads, group, tokens, longest):
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    rng = np.random.default_rng(longest)
+    lens = rng.integers(tokens, longest + 1, seqs)
+    lens[-1] = longest
+    q, k, v, table, n = make(torch, dtype=dtype, dim=dim, heads=kv_heads * group, kv_heads=kv_heads, lens=lens,
+                             tokens=tokens, seed=seqs)
+    wide = torch.full((seqs, 3000), -1, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    bits = np.tril(rng.random((1, tokens, tokens)) < 0.5)
+    for t in (table, wide):
+        out = paged.tree_attention(q, k, v, t, n, pack(torch, bits))
+        check(torch, out, q, k, v, t, n, [tree_mask_of(bits[0], x, tokens) for x in lens.tolist()])
+        for window, sinks in ((40, 0), (120, 3), (longest, 0)):
+            out = paged.window_attention(q, k, v, t, n, window, sinks)
+            check(torch, out, q, k, v, t, n, [window_mask(x, tokens, window, sinks) for x in lens.tolist()])
+
+
 @pytest.mark.parametrize("tokens", [1, 60])
 def test_a_wait_that_gives_up_is_reported(torch_cuda, tokens):
     """With a limit of one poll the kernel's waits give up: it returns, says so, and the next call is right."""
