@@ -685,13 +685,25 @@ __global__ void __launch_bounds__(THREADS, 1)
           };
           int unit = 0;
           do {
+            // Rows past the end are in the unit's last tile: cleared as soon as it has landed, not when its P is ready.
+            bool clear = past_end(p, w.u, w.a1 - 1);
+            auto clear_ahead = [&](int a) {
+              const int ahead = w.a1 - 1 - a, s = vr.s + ahead;
+              if (!clear || ahead >= C::V_STAGES) return;
+              const bool wrapped = s >= C::V_STAGES;
+              const int at = wrapped ? s - C::V_STAGES : s;
+              if (!__all_sync(0xffffffffu, mbar_test_wait(&ctl->v_full[at], vr.phase ^ wrapped))) return;
+              clear_v(w.u, w.a1 - 1, at);
+              clear = false;
+            };
+            clear_ahead(w.a0);
             // O of the unit before has been read out, by both streams.
             if (unit > 0 && !(ok = warp_ok(&ctl->o_free, (unit - 1) & 1))) break;
             for (int a = w.a0; a < w.a1; ++a, ++g, vr.next(C::V_STAGES)) {
               const int buf = g % NB;
               const uint32_t phase = (g / NB) & 1, add = a - w.a0 >= 2;  // each stream's first tile overwrites its O
               if (!(ok = warp_ok(&ctl->v_full[vr.s], vr.phase))) break;
-              if (past_end(p, w.u, a)) clear_v(w.u, a, vr.s);
+              clear_ahead(a);
               if constexpr (HALVES == 2) {
                 if (!(ok = warp_ok(&ctl->p_half[buf], phase))) break;
                 if (elect_one_lane()) pv(g & 1, buf, 0, add);
@@ -821,6 +833,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int a = a_first; a < w.a1; a += STEP) {
           const int g = g0 + a - w.a0, buf = NT == 2 ? i : g % NB;
           const uint32_t s_addr = tmem + lane_off + C::S_COL(buf);
+          // What the row sees, worked out while S is on its way.
+          const bool masked = a < whole_from || a >= whole_to;
+          uint64_t see[(KC + 63) / 64] = {};
+          if (masked && live) {
+            const int k0 = tile_key(p, u, a) + group * KC;
+#pragma unroll
+            for (int ch = 0; ch < (KC + 63) / 64; ++ch)
+              see[ch] = visible(p, u, t, k0 + ch * 64) & low_bits(p.tile_keys - group * KC - ch * 64);
+          }
           if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g / NB) & 1, p.wait_limit, abort_flag))) break;
           tc_fence_after();
           uint32_t sv[KC];
@@ -832,16 +853,10 @@ __global__ void __launch_bounds__(THREADS, 1)
               tmem_ld_32x32b_x32(s_addr + group * KC + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + ch * 32));
           }
           tc_wait_ld();
-          if (__builtin_expect(a < whole_from || a >= whole_to, 0)) {
-            const int k0 = tile_key(p, u, a), skip = group * KC;
+          if (__builtin_expect(masked, 0)) {
 #pragma unroll
-            for (int ch = 0; ch < (KC + 63) / 64; ++ch) {
-              const int from = skip + ch * 64;
-              const uint64_t see = live ? visible(p, u, t, k0 + from) & low_bits(p.tile_keys - from) : 0;
-#pragma unroll
-              for (int e = 0; e < (KC < 64 ? KC : 64); ++e)
-                if (!(see >> e & 1)) sv[ch * 64 + e] = __float_as_uint(-INFINITY);
-            }
+            for (int e = 0; e < KC; ++e)
+              if (!(see[e / 64] >> (e % 64) & 1)) sv[e] = __float_as_uint(-INFINITY);
           }
           float top;
           {
