@@ -1012,6 +1012,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
           for (int c0 = 0; c0 < D / 32 && ok; c0 += at_once) {
             const int chunks = min(at_once, D / 32 - c0);
+            // The lines before have been read.  (Those of the unit before: the warps have met since.)
+            if (c0 > 0 && !(ok = meet(&ctl->groups[i], group_meets))) break;
 #pragma unroll 1
             for (int ch = 0; ch < chunks; ++ch) {
               const uint32_t column = i * (D / 2) + (c0 + ch) * 16;
@@ -1019,14 +1021,17 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int j = 0; j < 2; ++j) tmem_ld_32x32b_x16(o_from[j] + column, o[j]);
               tc_wait_ld();
-              float x[16];
+              if (r < rows) {
+                float4* to = reinterpret_cast<float4*>(stage + ((ch * KS + group) * rows + r) * kOutRow);
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                x[e] = __uint_as_float(o[0][e]) * weight[0] + __uint_as_float(o[1][e]) * weight[1];
-              float4* to = reinterpret_cast<float4*>(stage + ((ch * KS + group) * rows + r) * kOutRow);
-              if (r < rows)
+                for (int e = 0; e < 4; ++e) {
+                  float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) to[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+                  for (int k = 0; k < 4; ++k)
+                    x[k] = __uint_as_float(o[0][4 * e + k]) * weight[0] + __uint_as_float(o[1][4 * e + k]) * weight[1];
+                  to[e] = make_float4(x[0], x[1], x[2], x[3]);
+                }
+              }
             }
             if (!(ok = meet(&ctl->groups[i], group_meets))) break;
             // 4 columns of a row per thread and round
@@ -1050,7 +1055,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 *reinterpret_cast<float4*>(p.part + (slot_row + row) * D + column) = x;
               }
             }
-            ok = meet(&ctl->groups[i], group_meets);
           }
           if (!ok) break;
         }
