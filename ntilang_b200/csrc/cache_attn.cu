@@ -54,7 +54,7 @@ constexpr int kOutRow = 80;            // bytes from one staged output row to th
 // heads, window 2048: 172 against 169 us.)
 constexpr float kRescaleLog2 = 15.0f;
 
-struct AttnParams {
+struct AttnBase {
   uint16_t* o;
   const int32_t* table;
   const int32_t* lens;
@@ -67,14 +67,22 @@ struct AttnParams {
   int seqs, tokens, heads, kv_heads, group, pages, page_size, max_pages, words, window, sinks;
   int tile_tokens;   // tokens per 128-row tile
   int blocks;        // token blocks per sequence (units of NT tiles)
-  int tile_keys;     // keys per tile: whole pages, or a divisor of a page
+  int tile_keys;     // keys per tile: whole pages, or a part of a page
   int tile_pages;    // pages per tile (1 where a page holds several tiles)
+  int page_tiles;    // tiles per page where the last is shorter, else 0
   int page_shift;    // log2 of page_size, -1 if it is no power of two
   int tile_shift;    // log2 of tile_keys, the same
   int rows;          // rows a workspace slot has
   int whole;         // no unit is cut: a CTA takes those that begin in its piece
   float c;           // softmax scale in log2 units
   int64_t wait_limit;
+};
+
+// SPLIT: a page holds several tiles and the last is shorter (page_tiles is set).  In the type, because the divisions
+// cost the kernels that need none of them 1 to 17% (4096 tokens x 32 heads, window 2048: 159 against 186 us).
+template <bool SPLIT>
+struct AttnParams : AttnBase {
+  static constexpr bool kSplit = SPLIT;
 };
 
 constexpr int SOFTMAX_WARPS = 8, MMA_WARP = 8, K_WARP = 9, V_WARP = 10, AUX_WARP = 11, THREADS = 384;
@@ -179,11 +187,17 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int64_
 
 // ------------------------------------------------------------------------------ units
 
-__device__ __forceinline__ int tile_index(const AttnParams& p, int key) {
+template <class P>
+__device__ __forceinline__ int tile_index(const P& p, int key) {
+  if constexpr (P::kSplit) {
+    const int page = key / p.page_size;
+    return page * p.page_tiles + (key - page * p.page_size) / p.tile_keys;
+  }
   return p.tile_shift >= 0 ? key >> p.tile_shift : key / p.tile_keys;
 }
 
-__device__ __forceinline__ Unit unit_of(const AttnParams& p, int item, int block_tokens) {
+template <class P>
+__device__ __forceinline__ Unit unit_of(const P& p, int item, int block_tokens) {
   Unit u;
   u.b = p.blocks == 1 ? item : item / p.blocks;
   u.t0 = (item - u.b * p.blocks) * block_tokens;
@@ -193,24 +207,36 @@ __device__ __forceinline__ Unit unit_of(const AttnParams& p, int item, int block
   u.sink_tiles = u.first = 0;
   if (u.t0 >= u.live) return u;
   if (p.tree) {
-    u.tiles = max(1, tile_index(p, u.len + p.tile_keys - 1));
+    u.tiles = tile_index(p, u.len - 1) + 1;
   } else {
     const int prefix = u.len - u.live;
     const int last = prefix + min(u.t0 + block_tokens, u.live) - 1;
     u.first = tile_index(p, max(0, prefix + u.t0 - p.window + 1));
-    u.sink_tiles = min(u.first, tile_index(p, p.sinks + p.tile_keys - 1));
+    u.sink_tiles = p.sinks > 0 ? min(u.first, tile_index(p, p.sinks - 1) + 1) : 0;
     u.tiles = u.sink_tiles + tile_index(p, last) - u.first + 1;
   }
   return u;
 }
 
-__device__ __forceinline__ int tile_key(const AttnParams& p, const Unit& u, int a) {
-  return (a < u.sink_tiles ? a : u.first + a - u.sink_tiles) * p.tile_keys;
+template <class P>
+__device__ __forceinline__ int tile_key(const P& p, const Unit& u, int a) {
+  const int x = a < u.sink_tiles ? a : u.first + a - u.sink_tiles;
+  if constexpr (P::kSplit) return x / p.page_tiles * p.page_size + x % p.page_tiles * p.tile_keys;
+  return x * p.tile_keys;
+}
+
+// Keys of the tile that begins at key k0.  (Rows of a page's last tile past the page are zeros.)
+template <class P>
+__device__ __forceinline__ int tile_span(const P& p, int k0) {
+  if constexpr (P::kSplit) return min(p.tile_keys, p.page_size - k0 % p.page_size);
+  return p.tile_keys;
 }
 
 // Whether the tile holds rows at or past the sequence's end, which V must not multiply as they are.
-__device__ __forceinline__ bool past_end(const AttnParams& p, const Unit& u, int a) {
-  return u.len - tile_key(p, u, a) < p.tile_keys;
+template <class P>
+__device__ __forceinline__ bool past_end(const P& p, const Unit& u, int a) {
+  const int k0 = tile_key(p, u, a);
+  return u.len - k0 < tile_span(p, k0);
 }
 
 // a / b for a >= 0, b > 0: the fast divide is within one of it below 2^22.
@@ -253,7 +279,8 @@ __device__ __forceinline__ int block_exclusive(int x, int* sums, int& total) {
 
 // Finds this CTA's piece (ctl->start and its first unit); all threads.  `places`: of the line after each
 // unit's tiles.  Returns the CTAs that have a piece.
-__device__ __forceinline__ int find_piece(const AttnParams& p, Ctl* ctl, int block_tokens, int places) {
+template <class P>
+__device__ __forceinline__ int find_piece(const P& p, Ctl* ctl, int block_tokens, int places) {
   const int items = p.seqs * p.blocks;
   int total = 0, at = 0;
   Unit u;
@@ -301,7 +328,8 @@ struct Walk {
   int a0, a1;  // this unit's tiles in this CTA
 
   // The first unit of the piece with tiles in it; false when it has none.
-  __device__ __forceinline__ bool begin(const AttnParams& p, const Ctl* ctl, int block_tokens, int places) {
+  template <class P>
+  __device__ __forceinline__ bool begin(const P& p, const Ctl* ctl, int block_tokens, int places) {
     item = ctl->start[0];
     kv_head = ctl->start[1];
     place = ctl->start[2];
@@ -311,7 +339,8 @@ struct Walk {
     a1 = p.whole ? (a0 > 0 ? a0 : u.tiles) : min(u.tiles, a0 + left);
     return a0 < a1 || next(p, block_tokens, places);
   }
-  __device__ __forceinline__ bool next(const AttnParams& p, int block_tokens, int places) {
+  template <class P>
+  __device__ __forceinline__ bool next(const P& p, int block_tokens, int places) {
     left -= u.tiles + places - place;
     if (left <= 0) return false;
     if (++kv_head == p.kv_heads) {
@@ -383,7 +412,8 @@ __device__ __forceinline__ uint64_t low_bits(int x) {
 }
 
 // Which of the 64 keys from k0 on the row sees.
-__device__ __forceinline__ uint64_t visible(const AttnParams& p, const Unit& u, int t, int k0) {
+template <class P>
+__device__ __forceinline__ uint64_t visible(const P& p, const Unit& u, int t, int k0) {
   const int prefix = u.len - u.live;
   if (!p.tree) {
     const int pos = prefix + t;
@@ -408,10 +438,10 @@ __device__ __forceinline__ uint64_t visible(const AttnParams& p, const Unit& u, 
 
 // ------------------------------------------------------------------------------ kernel
 
-template <int D, int NT, int KS, bool BF16>
+template <int D, int NT, int KS, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
     cache_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                      const __grid_constant__ CUtensorMap tv, const AttnParams p) {
+                      const __grid_constant__ CUtensorMap tv, const AttnParams<SPLIT> p) {
   using C = Shape<D, NT>;
   constexpr int BN = C::BN, NB = C::BUFFERS;
   // Hand P over in halves: with 128 keys and no key groups (which finish together).
@@ -808,7 +838,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // Tiles that every row of this row tile sees whole: [whole_from, whole_to).  (Tiles of sinks alone
       // are left to the masked path.)
       int whole_from = 0, whole_to = 0;
-      if (p.tile_keys == BN) {
+      if (!SPLIT && p.tile_keys == BN) {
         const int prefix = u.len - u.live;
         const int t_first = u.t0 + (NT == 2 ? i * p.tile_tokens : 0), t_last = min(t_first + p.tile_tokens, u.live) - 1;
         const int all_lo = p.tree ? 0 : max(prefix + t_last - p.window + 1, 0);
@@ -837,10 +867,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           const bool masked = a < whole_from || a >= whole_to;
           uint64_t see[(KC + 63) / 64] = {};
           if (masked && live) {
-            const int k0 = tile_key(p, u, a) + group * KC;
+            const int k0 = tile_key(p, u, a), from = group * KC, span = tile_span(p, k0) - from;
 #pragma unroll
             for (int ch = 0; ch < (KC + 63) / 64; ++ch)
-              see[ch] = visible(p, u, t, k0 + ch * 64) & low_bits(p.tile_keys - group * KC - ch * 64);
+              see[ch] = visible(p, u, t, k0 + from + ch * 64) & low_bits(span - ch * 64);
           }
           if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g / NB) & 1, p.wait_limit, abort_flag))) break;
           tc_fence_after();
@@ -1146,7 +1176,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 constexpr int kJoinWarps = 4;
 
 template <int D, int R, bool BF16>
-__global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const AttnParams p, int row_tiles) {
+__global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const AttnBase p, int row_tiles) {
   constexpr int kJoinRows = R, kJoinParts = 32 / R, kJoinAhead = 16 / R;
   constexpr int E = D / 32;
   using Vec = typename std::conditional<E == 4, float4, float2>::type;
@@ -1284,7 +1314,7 @@ bool few_tiles(int row_tiles, int tile_keys, int64_t tiles, int64_t units, int64
 
 // What the sizes decide: the shape of CTA, the grid and the workspace.
 struct Plan {
-  int row_tiles, tile_tokens, blocks, tile_keys, tile_pages, rows, ctas;
+  int row_tiles, tile_tokens, blocks, tile_keys, tile_pages, page_tiles, rows, ctas;
   bool whole;
   uint64_t part_bytes, bytes;
 };
@@ -1295,6 +1325,7 @@ int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, int6
   Plan& n = *plan;
   n.row_tiles = q->tokens * group > BM ? 2 : 1;
   n.tile_tokens = static_cast<int>(BM / group < q->tokens ? BM / group : q->tokens);
+  n.page_tiles = 0;
   const int64_t block_tokens = int64_t(n.row_tiles) * n.tile_tokens;
   const int64_t blocks = (q->tokens + block_tokens - 1) / block_tokens;
   const int most = n.row_tiles == 1 && c->head_dim == 128 ? Shape<128, 1>::BN : 128;
@@ -1302,17 +1333,17 @@ int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, int6
     n.tile_pages = static_cast<int>(most / c->page_size);
     n.tile_keys = static_cast<int>(n.tile_pages * c->page_size);
   } else {
+    // As few tiles as possible, equal but for the last: pages of 136 are 3 tiles of 48, 48 and 40.  (Their largest
+    // even part is 8 keys: 16 x 1 token over 4000 to 8000, 357 against 82 us.)
+    const int64_t parts = (c->page_size + most - 1) / most;
     n.tile_pages = 1;
-    n.tile_keys = 8;  // page_size is a multiple of 8
-    for (int k = most; k > 8; k -= 8)
-      if (c->page_size % k == 0) {
-        n.tile_keys = k;
-        break;
-      }
+    n.tile_keys = static_cast<int>((c->page_size + parts * 8 - 1) / (parts * 8) * 8);
+    if (parts * n.tile_keys != c->page_size) n.page_tiles = static_cast<int>(parts);
   }
   n.rows = n.row_tiles == 1 ? static_cast<int>(q->tokens * group) : 2 * BM;
   // Places of the line that one unit takes, at most.
-  const int64_t tiles = q->max_pages * c->page_size / n.tile_keys + 2 + kUnitPlaces<1>;
+  const int64_t tiles =
+      (n.page_tiles ? q->max_pages * n.page_tiles : q->max_pages * c->page_size / n.tile_keys) + 2 + kUnitPlaces<1>;
   NTL_REQUIRE(q->seqs * blocks < (int64_t(1) << 31) / c->kv_heads / tiles, NTL_ERR_UNSUPPORTED,
               "%s: more than 2^31 tiles of keys", what);
   static_assert(kUnitPlaces<1> >= kUnitPlaces<2>, "the bound above");
@@ -1331,11 +1362,11 @@ int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, int6
   return NTL_OK;
 }
 
-template <int D, int NT, int KS, bool BF16>
+template <int D, int NT, int KS, bool BF16, bool SPLIT>
 int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                 const AttnParams& p, const Plan& n, cudaStream_t s) {
+                 const AttnBase& p, const Plan& n, cudaStream_t s) {
   static std::atomic<uint64_t> done_mask{0};
-  auto kernel = cache_attn_kernel<D, NT, KS, BF16>;
+  auto kernel = cache_attn_kernel<D, NT, KS, BF16, SPLIT>;
   constexpr int smem = smem_bytes<D, NT>();
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "cudaGetDevice failed");
@@ -1351,7 +1382,7 @@ int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk,
                       fa.numRegs, REGS_LAUNCH);
     done_mask.fetch_or(bit, std::memory_order_release);
   }
-  cudaError_t e = ntl_launch_pdl(kernel, dim3(n.ctas), dim3(THREADS), smem, s, mq, mk, mv, p);
+  cudaError_t e = ntl_launch_pdl(kernel, dim3(n.ctas), dim3(THREADS), smem, s, mq, mk, mv, AttnParams<SPLIT>{p});
   if (e != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   ntl_note_launch();
   if (int rc = ntl_check_launch(what)) return rc;
@@ -1383,7 +1414,7 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   const int64_t box[4] = {64, 1, n.tile_keys / n.tile_pages, 1};
   if (int rc = make_map(&mk, what, c->k, bf16, dims, strides, box)) return rc;
   if (int rc = make_map(&mv, what, c->v, bf16, dims, strides, box)) return rc;
-  AttnParams p = {};
+  AttnBase p = {};
   p.o = static_cast<uint16_t*>(q->o);
   p.table = q->table;
   p.lens = q->lens;
@@ -1410,6 +1441,7 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   p.blocks = n.blocks;
   p.tile_keys = n.tile_keys;
   p.tile_pages = n.tile_pages;
+  p.page_tiles = n.page_tiles;
   p.page_shift = p.tile_shift = -1;
   for (int i = 3; i <= 20; ++i) {
     if (p.page_size == 1 << i) p.page_shift = i;
@@ -1422,9 +1454,11 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   // Key groups for up to 16 rows: 64 sequences x 1 token x 4 heads per key head, window 4096: 175 us against
   // 197 us without (back to back, at the power cap).  Four groups of up to 32 rows need the 128-row MMA
   // and measured slower than none at head_dim 128 (32 x 8 drafts over 8192 tokens: 213 against 201 us).
-#define NTL_CACHE_ATTN(D, NT, KS)                                          \
-  return bf16 ? launch_shape<D, NT, KS, true>(what, mq, mk, mv, p, n, s) \
-              : launch_shape<D, NT, KS, false>(what, mq, mk, mv, p, n, s)
+#define NTL_CACHE_ATTN(D, NT, KS)                                                                       \
+  return n.page_tiles ? bf16 ? launch_shape<D, NT, KS, true, true>(what, mq, mk, mv, p, n, s)           \
+                             : launch_shape<D, NT, KS, false, true>(what, mq, mk, mv, p, n, s)          \
+         : bf16       ? launch_shape<D, NT, KS, true, false>(what, mq, mk, mv, p, n, s)                 \
+                      : launch_shape<D, NT, KS, false, false>(what, mq, mk, mv, p, n, s)
   if (dim == 64) {
     if (n.row_tiles == 2) NTL_CACHE_ATTN(64, 2, 1);
     if (n.rows <= 16) NTL_CACHE_ATTN(64, 1, 4);

@@ -97,6 +97,7 @@ SHAPES = [  # dtype, dim, heads, kv_heads, page
     ("float16", 128, 8, 2, 16), ("bfloat16", 128, 4, 4, 64), ("float16", 64, 6, 2, 24), ("bfloat16", 64, 5, 1, 8),
     ("float16", 128, 16, 1, 128), ("bfloat16", 64, 2, 2, 256), ("float16", 64, 3, 1, 48), ("bfloat16", 128, 96, 1, 32),
     ("float16", 128, 2, 1, 200), ("float16", 64, 128, 1, 16),
+    ("float16", 128, 4, 1, 136), ("bfloat16", 64, 6, 2, 184), ("bfloat16", 128, 8, 2, 72), ("float16", 64, 4, 2, 272),
 ]
 
 
