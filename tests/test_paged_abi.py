@@ -111,7 +111,7 @@ def test_cache_refusals(call):
     assert call("ntl_tree_mask", None, 4, 0, 4, None, None) == (0, "")
 
 
-def test_refusals_before_any_gpu():
+def test_refusals_before_any_gpu(built_library):
     """CPU tensors and wrong sizes are Python errors, on a machine without a GPU too."""
     torch = pytest.importorskip("torch")
     from ntilang_b200 import paged
