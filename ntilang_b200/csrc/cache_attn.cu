@@ -972,7 +972,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int n = w.a1 - w.a0;
       const int g_last = g0 + (NT == 1 ? ((n - 1 - ((g0 ^ i) & 1)) | 1) - 1 + ((g0 ^ i) & 1) : n - 1);  // of this stream
       g0 += n;
-      if (any && a_first < w.a1 &&
+      // Rows that see nothing wait too: P V of the unit must not fall two units behind (it waits for o_free by parity).
+      if (a_first < w.a1 &&
           !(ok = warp_wait(&ctl->pv_done[NT == 2 ? i : g_last % NB], (NT == 2 ? g_last : g_last / NB) & 1,
                            p.wait_limit, abort_flag)))
         break;
@@ -995,34 +996,33 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t o_from[2] = {o_addr, o_addr};
       float mc = m == -INFINITY ? m : m * c, sum = l;
       if constexpr (NT == 1) {
-        if (u.t0 < u.live) {
-          float2(*ml)[BM] = ctl->ml[units & 1];
-          ml[i][row_lane] = make_float2(mc, l);
-          tc_fence_before();
-          if (!(ok = meet(&ctl->streams, stream_meets))) break;
-          tc_fence_after();
-          mc = -INFINITY;
-          sum = 0.0f;
+        // Units that nothing sees meet too: a stream that ran ahead would count twice in o_free.
+        float2(*ml)[BM] = ctl->ml[units & 1];
+        ml[i][row_lane] = make_float2(mc, l);
+        tc_fence_before();
+        if (!(ok = meet(&ctl->streams, stream_meets))) break;
+        tc_fence_after();
+        mc = -INFINITY;
+        sum = 0.0f;
 #pragma unroll
-          for (int k = 0; k < KS; ++k)
-            mc = fmaxf(mc, fmaxf(ml[0][k * GROUP_ROWS + r].x, ml[1][k * GROUP_ROWS + r].x));
-          // 2^(m - max m), 0 for a part that saw nothing (m = -inf; l is 0, or NaN for NaN scores and stays it).
-          const float top = mc == -INFINITY ? 0.0f : mc;
-          auto weigh = [&](float2 x) { return ex2_approx(x.x - top); };
+        for (int k = 0; k < KS; ++k)
+          mc = fmaxf(mc, fmaxf(ml[0][k * GROUP_ROWS + r].x, ml[1][k * GROUP_ROWS + r].x));
+        // 2^(m - max m), 0 for a part that saw nothing (m = -inf; l is 0, or NaN for NaN scores and stays it).
+        const float top = mc == -INFINITY ? 0.0f : mc;
+        auto weigh = [&](float2 x) { return ex2_approx(x.x - top); };
 #pragma unroll
-          for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float2 x = ml[j][k * GROUP_ROWS + r];
-              sum += weigh(x) * x.y;
-            }
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            // A stream without a tile in this unit weighs nothing; the other's O stands in for what it has not.
-            const bool has = n > (((g0 - n) ^ j) & 1);
-            o_from[j] = tmem + lane_off + (has ? C::O_COL(j) : C::O_COL(1 - j));
-            weight[j] = weigh(ml[j][row_lane]);
+            const float2 x = ml[j][k * GROUP_ROWS + r];
+            sum += weigh(x) * x.y;
           }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          // A stream without a tile in this unit weighs nothing; the other's O stands in for what it has not.
+          const bool has = n > (((g0 - n) ^ j) & 1);
+          o_from[j] = tmem + lane_off + (has ? C::O_COL(j) : C::O_COL(1 - j));
+          weight[j] = weigh(ml[j][row_lane]);
         }
       }
       ++units;

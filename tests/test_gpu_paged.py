@@ -189,6 +189,31 @@ def test_short_units(torch_cuda, dtype, dim, seqs, kv_heads, group, tokens, long
             check(torch, out, q, k, v, t, n, [window_mask(x, tokens, window, sinks) for x in lens.tolist()])
 
 
+# Sequences without keys or without new tokens: several units in a row in which a CTA has nothing to do but zeros.
+@pytest.mark.parametrize("dtype,dim,kv_heads,group,tokens,longest", [
+    ("float16", 128, 8, 1, 8, 35), ("bfloat16", 64, 8, 4, 1, 31), ("float16", 64, 8, 8, 4, 10), ("bfloat16", 128, 8, 5, 2, 270),
+    ("float16", 128, 8, 4, 60, 200), ("bfloat16", 64, 16, 16, 8, 90),
+])
+def test_runs_of_empty_units(torch_cuda, dtype, dim, kv_heads, group, tokens, longest):
+    from ntilang_b200 import _lib, paged
+
+    torch = torch_cuda
+    for seed in range(12):
+        rng = np.random.default_rng(seed)
+        lens = rng.integers(0, longest + 1, 60) * (rng.random(60) < 0.6)
+        lens[3] = longest
+        live = np.minimum(rng.integers(0, tokens + 1, 60) * (rng.random(60) < 0.7), lens).astype(np.int64)
+        q, k, v, table, n = make(torch, dtype=dtype, dim=dim, heads=kv_heads * group, kv_heads=kv_heads, lens=lens,
+                                 tokens=tokens, seed=seed)
+        fresh = torch.tensor(live, dtype=torch.int32, device="cuda")
+        bits = np.tril(rng.random((1, tokens, tokens)) < 0.7)
+        out = paged.tree_attention(q, k, v, table, n, pack(torch, bits), q_lens=fresh)
+        check(torch, out, q, k, v, table, n, [tree_mask_of(bits[0], x, m) for x, m in zip(lens.tolist(), live.tolist())])
+        out = paged.window_attention(q, k, v, table, n, 50, 2, q_lens=fresh)
+        check(torch, out, q, k, v, table, n, [window_mask(x, m, 50, 2) for x, m in zip(lens.tolist(), live.tolist())])
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("tokens", [1, 60])
 def test_a_wait_that_gives_up_is_reported(torch_cuda, tokens):
     """With a limit of one poll the kernel's waits give up: it returns, says so, and the next call is right."""
