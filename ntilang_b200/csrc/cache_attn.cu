@@ -600,9 +600,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           ring.next(count);
         }
       } while (ok && w.next(p, block_tokens, PLACES));
-      if (!ok && lane == 0) {
-        give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
-        // Drain every copy this warp issued before the CTA exits.
+      if (lane == 0) {
+        if (!ok) give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
+        // Every copy of this warp lands before the CTA exits.  (The MMA threads waited for all of them, unless one
+        // gave up; that may be after this warp's last copy, so it waits whether or not its own waits held.)
         for (int j = max(0, issued - count); j < issued; ++j) {
           const int s = j % count;
           const bool clear = cleared >> s & 1;
@@ -798,7 +799,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (!ok || !w.next(p, block_tokens, PLACES)) break;
         }
       }
-      if (!ok && (warp == MMA_WARP || elect_one_lane())) {
+      // Every MMA retires before the CTA exits.  (The softmax waits for each, unless it gave up, which this thread may
+      // not see.)
+      if (warp == MMA_WARP || elect_one_lane()) {
         uint64_t* drain = &ctl->drain[warp == MMA_WARP ? 0 : 1];
         tc_commit(drain);
         if (!wait_bounded(drain, 0, int64_t(1) << 24, nullptr))

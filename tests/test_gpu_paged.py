@@ -238,6 +238,39 @@ def test_a_wait_that_gives_up_is_reported(torch_cuda, tokens):
     assert _lib.device_status() == 0
 
 
+# One shape per kind of CTA, with pieces of one tile (all of a loader's copies are out before another role gives up)
+# and of more tiles than the rings hold.
+@pytest.mark.parametrize("dtype,dim,heads,kv_heads,page,tokens,lens", [
+    ("float16", 128, 8, 2, 16, 1, [300, 5]), ("bfloat16", 128, 8, 8, 64, 1, [40000, 30000]),
+    ("float16", 64, 8, 2, 24, 2, [700]), ("bfloat16", 64, 8, 2, 64, 2, [60000, 100]),
+    ("bfloat16", 128, 8, 2, 136, 20, [400, 90]), ("float16", 64, 8, 2, 16, 30, [30000]),
+    ("float16", 128, 8, 2, 16, 60, [130, 61]), ("bfloat16", 128, 8, 1, 64, 200, [9000, 5000]),
+    ("bfloat16", 64, 8, 2, 200, 70, [300]), ("float16", 64, 8, 2, 64, 150, [20000, 170]),
+])
+def test_calls_after_ones_that_gave_up(torch_cuda, dtype, dim, heads, kv_heads, page, tokens, lens):
+    """A CTA that gives up lets its copies and products end before it exits: the call launched right behind it, on the
+    same SMs, is right every time."""
+    from ntilang_b200 import _lib, paged
+
+    torch = torch_cuda
+    q, k, v, table, n = make(torch, dtype=dtype, dim=dim, heads=heads, kv_heads=kv_heads, page=page, lens=lens,
+                             tokens=tokens, seed=page)
+    want = paged.window_attention(q, k, v, table, n, 1 << 20)
+    check(torch, want, q, k, v, table, n, [window_mask(x, tokens, 1 << 20, 0) for x in lens])
+    got = []
+    try:
+        for limit in (1, 2, 20) * 5:
+            _lib.set_wait_limit(limit)
+            paged.window_attention(q, k, v, table, n, 1 << 20)
+            _lib.set_wait_limit(1 << 26)
+            got.append(paged.window_attention(q, k, v, table, n, 1 << 20))
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_wait_limit(1 << 26)
+        _lib.clear_device_status()
+    assert all(torch.equal(x, want) for x in got)
+
+
 @pytest.mark.parametrize("tokens", [1, 5, 64, 200])
 def test_tree_of_parents(torch_cuda, tokens):
     """tree_mask, one tree shared by every sequence, and a chain's equality with causal attention."""
