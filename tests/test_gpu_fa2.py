@@ -159,6 +159,42 @@ def test_fa2_timeout_path_reports_error(torch_cuda, causal, grid):
     torch.testing.assert_close(out.float(), sdpa_fp32(torch, q, k, v, causal), rtol=0, atol=ATOL)
 
 
+@pytest.mark.parametrize("causal,grid", [(False, "auto"), (True, "per_block"), (True, "persistent")])
+@pytest.mark.parametrize("s,d", [(100, 128), (1024, 64), (2048, 128)])
+def test_fa2_calls_after_ones_that_gave_up(torch_cuda, causal, grid, s, d):
+    """A CTA that gives up lets its copies and products end before it exits: the call launched right
+    behind it, on the same SMs, is right every time."""
+    torch = torch_cuda
+    from ntilang_b200 import _lib
+
+    mode = {"auto": _lib.FA2_GRID_AUTO, "persistent": _lib.FA2_GRID_PERSISTENT,
+            "per_block": _lib.FA2_GRID_PER_BLOCK}[grid]
+    b, h = 2, 8
+    q, k, v = (torch.randn(b, h, s, d, device="cuda", dtype=torch.float16) for _ in range(3))
+
+    def attend(limit):
+        o = torch.empty_like(q)
+        _lib.set_wait_limit(limit)
+        _lib.call("ntl_fa2_fwd_f16", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), b, h, s, d,
+                  math.log2(math.e) / math.sqrt(d), int(causal), torch.cuda.current_stream().cuda_stream)
+        return o
+
+    _lib.set_fa2_causal_grid(mode)
+    try:
+        want = attend(1 << 26)
+        got = []
+        for limit in (1, 2, 20) * 5:
+            attend(limit)
+            got.append(attend(1 << 26))
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_wait_limit(1 << 26)
+        _lib.set_fa2_causal_grid(_lib.FA2_GRID_AUTO)
+        _lib.clear_device_status()
+    torch.testing.assert_close(want.float(), sdpa_fp32(torch, q, k, v, causal), rtol=0, atol=ATOL)
+    assert all(torch.equal(x, want) for x in got)
+
+
 @pytest.mark.parametrize("b,h,s", [(3, 5, 600), (1, 1, 100), (2, 3, 4096), (64, 16, 512), (2, 32, 4096)])
 def test_fa2_causal_grids_agree(torch_cuda, b, h, s):
     """Causal attention on each grid, pinned with ntl_fa2_set_causal_grid, and on the automatic
