@@ -301,8 +301,9 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tc_kernel(const __grid_consta
           if (++stage == STAGES) stage = 0, phase ^= 1;
         }
       }
-      if (!ok) {
-        // Drain: the last min(issued, STAGES) stages may still have loads in flight.
+      {
+        // Drain: the last min(issued, STAGES) stages may still have loads in flight, also when
+        // another role gives up after the last of them.
         int s = stage;
         uint32_t ph = phase;
         for (int i = 0; i < STAGES && i < issued; ++i) {

@@ -147,6 +147,38 @@ def test_gemm_timeout_path_reports_error(torch_cuda):
     check(torch, c2, ref_gemm(torch, a, b))
 
 
+@pytest.mark.parametrize("m,n,k,trans", [(64, 512, 64, 0), (100, 4096, 512, 0), (128, 4096, 2048, 1), (512, 1024, 512, 0)])
+def test_gemm_calls_after_ones_that_gave_up(torch_cuda, m, n, k, trans):
+    """A CTA that gives up lets its copies and products end before it exits: the call launched right
+    behind it, on the same SMs, is right every time."""
+    torch = torch_cuda
+    from ntilang_b200 import _lib
+
+    a = torch.randn(m, k, device="cuda").half()
+    b = torch.randn(k, n, device="cuda").half()
+    bt = b.T.contiguous() if trans else b
+
+    def product(limit):
+        c = torch.empty(m, n, device="cuda")
+        _lib.set_wait_limit(limit)
+        _lib.call("ntl_gemm_f16_f32", a.data_ptr(), bt.data_ptr(), c.data_ptr(), None, 0, 1.0, 0, m, n, k, trans,
+                  torch.cuda.current_stream().cuda_stream)
+        return c
+
+    try:
+        want = product(1 << 26)
+        got = []
+        for limit in (1, 2, 20) * 5:
+            product(limit)
+            got.append(product(1 << 26))
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_wait_limit(1 << 26)
+        _lib.clear_device_status()
+    check(torch, want, ref_gemm(torch, a, b))
+    assert all(torch.equal(x, want) for x in got)
+
+
 @pytest.mark.parametrize("m,n,k", [(4096, 4096, 4096), (512, 4096, 4096), (1000, 1024, 1032), (384, 768, 4096)])
 def test_gemm_stream_k_repeated_calls(torch_cuda, m, n, k):
     """Shapes whose last wave is split along K (stream-K through the cached workspace), called
