@@ -30,13 +30,21 @@
 //   NT = 2: two 128-row tiles that share every K and V tile of 128 keys; a stream is a row tile.  For
 //           wide trees and prompt chunks, bound by the tensor cores and the exponentials.
 // Warps: 8 softmax (one thread per row = TMEM lane; the same thread rescales and writes out the row),
-// one for K loads, one for V loads, and two that issue MMAs, load Q and clear value rows past the
-// sequence's end (a page's unwritten rows may hold NaN, and 0 * NaN is not 0): NT = 1 has Q and Q K^T in one,
-// clearing and P V in the other (one thread for both products waited for P while K had landed: 5% slower
-// decode); NT = 2 all MMAs in one, Q and clearing in the other.
+// one for K loads, one for V loads, and two that issue MMAs and load Q: NT = 1 has Q and Q K^T in one, P V in the
+// other (one thread for both products waited for P while K had landed: 5% slower decode); NT = 2 all MMAs in
+// one, Q in the other.
+// A value row that no token of the unit sees (past the sequence's end, between the sinks and the window, a draft that
+// no mask names) must not be multiplied as it is: it may never have been written, and 0 * NaN is not 0.
+// Whole pages of such rows are loaded from outside the tensor map, which reads as zeros.  Of a page seen in part,
+//   with key groups: the softmax warps clear them in shared memory before they hand over P;
+//   without: V comes in boxes of 8 rows, and of single rows where 8 are seen in part, each from its page or from outside.
+// (Boxes with key groups: 64 x 1 token, window 4096: 175 -> 180 us, 59 x 1 token, window 86: 9.5 -> 11.6.  Clearing
+// without: 16 x 27 drafts 55.1 -> 57.1, 1 x 9 drafts x 3 heads over 348 keys 10.6 -> 11.4.  Clearing by the warp that issues
+// P V: 1 to 8% slower than either.)
 // Every wait is bounded: one that gives up records a status code, and the CTA drains its copies
 // and MMAs, frees TMEM and returns.
 #include <atomic>
+#include <climits>
 #include <cuda_bf16.h>
 #include <mutex>
 #include <type_traits>
@@ -124,7 +132,6 @@ constexpr int kUnitPlaces = NT == 1 ? 6 : 3;
 struct __align__(16) Ctl {
   uint64_t q_full, q_empty;
   uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
-  uint64_t v_raw[kMaxStages];  // NT = 2: a V tile with rows past the end has landed: v_full follows once they are cleared
   uint64_t s_full[4];          // S buffer b holds scores
   uint64_t p_half[4];          // it holds the exponentials of the first half of the keys (4 warps; see HALVES)
   uint64_t p_ready[4];         // it holds all exponentials (4 warps)
@@ -232,11 +239,19 @@ __device__ __forceinline__ int tile_span(const P& p, int k0) {
   return p.tile_keys;
 }
 
-// Whether the tile holds rows at or past the sequence's end, which V must not multiply as they are.
+// The first key inside the window of the unit's first token.
 template <class P>
-__device__ __forceinline__ bool past_end(const P& p, const Unit& u, int a) {
-  const int k0 = tile_key(p, u, a);
-  return u.len - k0 < tile_span(p, k0);
+__device__ __forceinline__ int window_from(const P& p, const Unit& u) {
+  return max(0, u.len - u.live + u.t0 - p.window + 1);
+}
+
+// Whether the tile may hold rows that no token of the unit sees: rows past the sequence's end, rows between the sinks
+// and the window, drafts.
+template <class P>
+__device__ __forceinline__ bool may_be_unseen(const P& p, const Unit& u, int a) {
+  const int k0 = tile_key(p, u, a), end = k0 + tile_span(p, k0);
+  if (p.tree) return end > u.len - u.live;
+  return end > u.len || max(k0, p.sinks) < min(end, window_from(p, u));
 }
 
 // a / b for a >= 0, b > 0: the fast divide is within one of it below 2^22.
@@ -436,12 +451,31 @@ __device__ __forceinline__ uint64_t visible(const P& p, const Unit& u, int t, in
   return bits & low_bits(u.len - k0);
 }
 
+__device__ __forceinline__ uint64_t or_sync(uint64_t x) {  // of a whole warp
+  return static_cast<uint64_t>(__reduce_or_sync(0xffffffffu, static_cast<uint32_t>(x >> 32))) << 32 |
+         __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(x));
+}
+
+// Which of the 64 keys from k0 on some token of the unit sees (window: all from its first token's first to the
+// sequence's end).  One warp.
+template <class P>
+__device__ __forceinline__ uint64_t unit_sees(const P& p, const Unit& u, int block_tokens, int k0) {
+  if (!p.tree) return low_bits(u.len - k0) & (~low_bits(window_from(p, u) - k0) | low_bits(p.sinks - k0));
+  uint64_t bits = low_bits(u.len - u.live - k0);
+  if (k0 + 64 > u.len - u.live) {
+    for (int t = u.t0 + (threadIdx.x & 31); t < min(u.t0 + block_tokens, u.live); t += 32) bits |= visible(p, u, t, k0);
+    bits = or_sync(bits);
+  }
+  return bits;
+}
+
 // ------------------------------------------------------------------------------ kernel
 
 template <int D, int NT, int KS, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
     cache_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                      const __grid_constant__ CUtensorMap tv, const AttnParams<SPLIT> p) {
+                      const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tv8,
+                      const __grid_constant__ CUtensorMap tv1, const AttnParams<SPLIT> p) {
   using C = Shape<D, NT>;
   constexpr int BN = C::BN, NB = C::BUFFERS;
   // Hand P over in halves: with 128 keys and no key groups (which finish together).
@@ -457,7 +491,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int block_tokens = NT * p.tile_tokens;
 
   pdl_trigger();
-  if (threadIdx.x < 3) prefetch_tensormap(threadIdx.x == 0 ? &tq : threadIdx.x == 1 ? &tk : &tv);
+  if (threadIdx.x < (KS > 1 ? 3 : 5))
+    prefetch_tensormap(threadIdx.x == 0   ? &tq
+                       : threadIdx.x == 1 ? &tk
+                       : threadIdx.x == 2 ? &tv
+                       : threadIdx.x == 3 ? &tv8
+                                          : &tv1);
   if (warp == MMA_WARP) {
     tmem_alloc(&ctl->tmem_base, TMEM_COLS);
     tmem_relinquish();
@@ -469,7 +508,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&ctl->k_empty[s], 1);
       mbar_init(&ctl->v_full[s], 1);
       mbar_init(&ctl->v_empty[s], 1);
-      mbar_init(&ctl->v_raw[s], 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&ctl->s_full[i], 1);
@@ -521,18 +559,6 @@ __global__ void __launch_bounds__(THREADS, 1)
           tma_load_4d(smem + (NT == 2 ? i * C::Q_BYTES : i * (M / KS) * 128) + d * (M * 128), &tq, &ctl->q_full, d * 64,
                       w.kv_head * p.group, w.u.t0 + (NT == 2 ? i * p.tile_tokens : 0), w.u.b);
     };
-    // One warp: zeros over the rows of V stage s past the sequence's end, for the MMAs issued after it.
-    auto clear_v = [&](const Unit& u, int a, int s) {
-      const int first = max(u.len - tile_key(p, u, a), 0);  // rows that hold tokens
-      const int units = (p.tile_keys - first) * 8;          // 16-byte units per 64-column half
-#pragma unroll
-      for (int half = 0; half < D / 64; ++half)
-        for (int at = lane; at < units; at += 32)
-          *reinterpret_cast<uint4*>(smem + C::V_OFF + s * C::KV_BYTES + half * (BN * 128) + first * 128 + at * 16) =
-              make_uint4(0, 0, 0, 0);
-      fence_proxy_async_smem();
-      __syncwarp();
-    };
     if (warp == K_WARP || warp == V_WARP) {
       // ---------------------------------------------- K loads, V loads: one warp each, a lane per page
       // K frees its stages a softmax earlier than V does; one warp for both would hold K back.
@@ -554,9 +580,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       w.begin(p, ctl, block_tokens, PLACES);
       Ring ring;
       int issued = 0;
-      uint32_t raw = 0, cleared = 0;  // bit s: parity of the next v_raw[s]; stage s's last tile is one to clear
       do {
-        const int lo = p.tree ? 0 : max(0, w.u.len - w.u.live + w.u.t0 - p.window + 1);  // the window's first key
+        const int lo = p.tree ? 0 : window_from(p, w.u);
         const int32_t* row = p.table + w.u.b * p.table_stride;
         // A page that the unit sees nothing of, or that is not there, reads as zeros (the tensor
         // map fills what lies outside it), so a page given back or never written is not touched.
@@ -569,6 +594,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           return row[j];
         };
         int pages = pages_from(w.a0), pages_next = pages_from(w.a0 + batch), at = 0;
+        // Tiles that may be seen in part: from here on, and the sinks' last and the window's first.
+        const int part_from = KS > 1 || !is_v ? INT_MAX : p.tree ? tile_index(p, w.u.len - w.u.live) : w.u.tiles - 1;
+        const int part_at = KS > 1 || !is_v || p.tree ? INT_MIN : w.u.sink_tiles - 1;
         for (int a = w.a0; a < w.a1; ++a, ++at) {
           const int s = ring.s;
           if (at == batch) {
@@ -582,19 +610,50 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int k0 = tile_key(p, w.u, a);
             y = p.page_shift >= 0 ? k0 & (p.page_size - 1) : k0 % p.page_size;
           }
+          const bool in_part =
+              KS == 1 && (a >= part_from || static_cast<unsigned>(a) - static_cast<unsigned>(part_at) < 2u) && may_be_unseen(p, w.u, a);
+          uint64_t seen[BN / 64] = {};
+          if (in_part) {
+#pragma unroll
+            for (int ch = 0; ch < BN / 64; ++ch) seen[ch] = unit_sees(p, w.u, block_tokens, tile_key(p, w.u, a) + ch * 64);
+          }
           ok = lane != 0 || wait_bounded(&empty[s], ring.phase ^ 1, p.wait_limit, abort_flag);
           ok = __shfl_sync(0xffffffffu, ok, 0);
           if (!ok) break;
-          const bool clear = NT == 2 && is_v && past_end(p, w.u, a);
-          uint64_t* landed = clear ? &ctl->v_raw[s] : &full[s];
-          if (clear) raw ^= 1u << s;
-          cleared = clear ? cleared | 1u << s : cleared & ~(1u << s);
-          if (lane == 0) mbar_arrive_expect_tx(landed, tile_bytes);
+          if (lane == 0) mbar_arrive_expect_tx(&full[s], tile_bytes);
           __syncwarp();
-          uint8_t* to = stages + s * C::KV_BYTES + lane * box_bytes;
-          if (lane < boxes) {
+          uint8_t* to = stages + s * C::KV_BYTES;
+          uint32_t in_eights = 0;  // boxes that are loaded 8 rows at a time
+          if (in_part) {
+            // Lane l: rows 8 l to 8 l + 7, if the tile has them, of box `box`, their page's row y8.
+            const int box = quotient(lane * 8, box_keys);
+            const int page8 = __shfl_sync(0xffffffffu, pages, (at * boxes + box) & 31), y8 = y + lane * 8 - box * box_keys;
+            const uint32_t rows = static_cast<uint32_t>((lane < 8 ? seen[0] : seen[BN / 64 - 1]) >> (lane & 7) * 8) & 0xff;
+            const bool has = lane < p.tile_keys / 8 && page8 != -1;
+            in_eights = __reduce_or_sync(0xffffffffu, has && rows != 0xff ? 1u << box : 0u);
+            const bool mine = has && (in_eights >> box & 1);
+            if (mine && (rows == 0 || rows == 0xff)) {
 #pragma unroll
-            for (int d = 0; d < D / 64; ++d) tma_load_4d(to + d * (BN * 128), map, landed, d * 64, w.kv_head, y, page);
+              for (int d = 0; d < D / 64; ++d)
+                tma_load_4d(to + lane * 1024 + d * (BN * 128), &tv8, &full[s], d * 64, w.kv_head, y8, rows ? page8 : -1);
+            }
+#pragma unroll 1
+            for (uint32_t left = __ballot_sync(0xffffffffu, mine && rows != 0 && rows != 0xff); left; left &= left - 1) {
+              const int from = __ffs(left) - 1;
+              const uint32_t which = __shfl_sync(0xffffffffu, rows, from);
+              const int page1 = __shfl_sync(0xffffffffu, page8, from), y1 = __shfl_sync(0xffffffffu, y8, from) + lane;
+              if (lane < 8) {
+#pragma unroll
+                for (int d = 0; d < D / 64; ++d)
+                  tma_load_4d(to + (from * 8 + lane) * 128 + d * (BN * 128), &tv1, &full[s], d * 64, w.kv_head, y1,
+                              which >> lane & 1 ? page1 : -1);
+              }
+            }
+          }
+          if (lane < boxes && !(in_eights >> lane & 1)) {
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+              tma_load_4d(to + lane * box_bytes + d * (BN * 128), map, &full[s], d * 64, w.kv_head, y, page);
           }
           ++issued;
           ring.next(count);
@@ -605,50 +664,30 @@ __global__ void __launch_bounds__(THREADS, 1)
         // Every copy of this warp lands before the CTA exits.  (The MMA threads waited for all of them, unless one
         // gave up; that may be after this warp's last copy, so it waits whether or not its own waits held.)
         for (int j = max(0, issued - count); j < issued; ++j) {
-          const int s = j % count;
-          const bool clear = cleared >> s & 1;
-          if (!wait_bounded(clear ? &ctl->v_raw[s] : &full[s], clear ? ~raw >> s & 1 : (j / count) & 1, int64_t(1) << 24,
-                            nullptr))
+          if (!wait_bounded(&full[j % count], (j / count) & 1, int64_t(1) << 24, nullptr))
             atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
         }
       }
     } else if (NT == 2 && warp == AUX_WARP) {
-      // ---------------------------------------------- Q loads, and value rows past the end become zeros
-      bool ok = true;
-      Walk w;
-      w.begin(p, ctl, block_tokens, PLACES);
-      Ring ring;
-      int n = 0;
-      uint32_t raw = 0;  // bit s: parity of v_raw[s]
-      do {
-        // The next unit's Q once the last Q K^T of the unit before retired.
-        if (lane == 0) {
-          ok = n == 0 || wait_bounded(&ctl->q_empty, (n - 1) & 1, p.wait_limit, abort_flag);
-          if (ok) load_q(w);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
-        ++n;
-        for (int a = w.a0; a < w.a1 && ok; ++a, ring.next(C::V_STAGES)) {
-          if (!past_end(p, w.u, a)) continue;
-          const int s = ring.s;
-          if (lane == 0) ok = wait_bounded(&ctl->v_raw[s], raw >> s & 1, p.wait_limit, abort_flag);
-          __syncwarp();
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
-          raw ^= 1u << s;
-          clear_v(w.u, a, s);
-          if (lane == 0) mbar_arrive(&ctl->v_full[s]);
-        }
-      } while (ok && w.next(p, block_tokens, PLACES));
+      // ---------------------------------------------- Q loads (one lane)
       if (lane == 0) {
+        bool ok = true;
+        Walk w;
+        w.begin(p, ctl, block_tokens, PLACES);
+        int n = 0;
+        do {
+          // The next unit's Q once the last Q K^T of the unit before retired.
+          if (!(ok = n == 0 || wait_bounded(&ctl->q_empty, (n - 1) & 1, p.wait_limit, abort_flag))) break;
+          load_q(w);
+          ++n;
+        } while (w.next(p, block_tokens, PLACES));
         if (!ok) give_up(ctl, NTL_STATUS_TMA_EMPTY_WAIT);
         // The MMA thread waits for each Q load; if it gave up, this thread does before the CTA exits.
         if (n > 0 && !wait_bounded(&ctl->q_full, (n - 1) & 1, int64_t(1) << 24, nullptr))
           atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
       }
-    } else if ((NT == 1 && warp == AUX_WARP) || elect_one_lane()) {
-      // ---------------------------------------------- MMA issue (one lane; NT = 1 has its whole P V warp here)
+    } else if (elect_one_lane()) {
+      // ---------------------------------------------- MMA issue (one lane)
       constexpr uint32_t idesc_s = idesc<BF16>(M, BN, 0);  // B = K tile, K-major
       constexpr uint32_t idesc_o = idesc<BF16>(M, D, 1);   // B = V tile, N-major
       const uint32_t q_low = desc_low(smem_u32(smem), 16);
@@ -708,42 +747,22 @@ __global__ void __launch_bounds__(THREADS, 1)
           // Every Q load has landed before the CTA exits (this thread waited for it, unless it gave up).
           if (!ok && !wait_bounded(&ctl->q_full, q_phase, int64_t(1) << 24, nullptr))
             atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
-        } else {  // clearing and P V
-          auto warp_ok = [&](uint64_t* bar, uint32_t parity) -> bool {  // lane 0 waits for the warp
-            const bool got = lane != 0 || wait(bar, parity);
-            __syncwarp();
-            return __shfl_sync(0xffffffffu, got, 0);
-          };
+        } else {  // P V
           int unit = 0;
           do {
-            // Rows past the end are in the unit's last tile: cleared as soon as it has landed, not when its P is ready.
-            bool clear = past_end(p, w.u, w.a1 - 1);
-            auto clear_ahead = [&](int a) {
-              const int ahead = w.a1 - 1 - a, s = vr.s + ahead;
-              if (!clear || ahead >= C::V_STAGES) return;
-              const bool wrapped = s >= C::V_STAGES;
-              const int at = wrapped ? s - C::V_STAGES : s;
-              if (!__all_sync(0xffffffffu, mbar_test_wait(&ctl->v_full[at], vr.phase ^ wrapped))) return;
-              clear_v(w.u, w.a1 - 1, at);
-              clear = false;
-            };
-            clear_ahead(w.a0);
             // O of the unit before has been read out, by both streams.
-            if (unit > 0 && !(ok = warp_ok(&ctl->o_free, (unit - 1) & 1))) break;
+            if (unit > 0 && !(ok = wait(&ctl->o_free, (unit - 1) & 1))) break;
             for (int a = w.a0; a < w.a1; ++a, ++g, vr.next(C::V_STAGES)) {
               const int buf = g % NB;
               const uint32_t phase = (g / NB) & 1, add = a - w.a0 >= 2;  // each stream's first tile overwrites its O
-              if (!(ok = warp_ok(&ctl->v_full[vr.s], vr.phase))) break;
-              clear_ahead(a);
+              if (!(ok = wait(&ctl->v_full[vr.s], vr.phase))) break;
               if constexpr (HALVES == 2) {
-                if (!(ok = warp_ok(&ctl->p_half[buf], phase))) break;
-                if (elect_one_lane()) pv(g & 1, buf, 0, add);
+                if (!(ok = wait(&ctl->p_half[buf], phase))) break;
+                pv(g & 1, buf, 0, add);
               }
-              if (!(ok = warp_ok(&ctl->p_ready[buf], phase))) break;
-              if (elect_one_lane()) {
-                pv(g & 1, buf, HALVES - 1, HALVES == 2 ? 1u : add);
-                tc_commit(&ctl->v_empty[vr.s]);
-              }
+              if (!(ok = wait(&ctl->p_ready[buf], phase))) break;
+              pv(g & 1, buf, HALVES - 1, HALVES == 2 ? 1u : add);
+              tc_commit(&ctl->v_empty[vr.s]);
             }
             ++unit;
           } while (ok && w.next(p, block_tokens, PLACES));
@@ -801,12 +820,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       // Every MMA retires before the CTA exits.  (The softmax waits for each, unless it gave up, which this thread may
       // not see.)
-      if (warp == MMA_WARP || elect_one_lane()) {
-        uint64_t* drain = &ctl->drain[warp == MMA_WARP ? 0 : 1];
-        tc_commit(drain);
-        if (!wait_bounded(drain, 0, int64_t(1) << 24, nullptr))
-          atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
-      }
+      uint64_t* drain = &ctl->drain[warp == MMA_WARP ? 0 : 1];
+      tc_commit(drain);
+      if (!wait_bounded(drain, 0, int64_t(1) << 24, nullptr))
+        atomicCAS(&g_cache_attn_status, 0u, NTL_STATUS_DRAIN_WAIT);
     }
   } else {
     // ---------------------------------------------- softmax: one thread per row (and key group)
@@ -832,6 +849,36 @@ __global__ void __launch_bounds__(THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
       return warp_wait(bar, meets++ & 1, p.wait_limit, abort_flag);
+    };
+    // Key groups: the stream's 128 threads write zeros over V rows of tile a that no row sees: past the sequence's end
+    // and between the sinks and the window, 8 threads to a row; drafts, each warp those of its keys (`see`: of a lane's row).
+    auto clear_unseen = [&](const Unit& u, int a, int g, uint64_t see) -> bool {
+      if (!warp_wait(&ctl->v_full[g % C::V_STAGES], (g / C::V_STAGES) & 1, p.wait_limit, abort_flag)) return false;
+      uint8_t* tile = smem + C::V_OFF + g % C::V_STAGES * C::KV_BYTES;
+      const int k0 = tile_key(p, u, a);
+      auto row_at = [&](int key) { return min(max(key - k0, 0), p.tile_keys); };
+      int from = p.tree ? 0 : row_at(p.sinks), to = p.tree ? 0 : row_at(window_from(p, u));
+#pragma unroll 1
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll 2
+        for (int e = from * 8 + row_lane; e < to * 8; e += 128)
+#pragma unroll
+          for (int half = 0; half < D / 64; ++half)
+            *reinterpret_cast<uint4*>(tile + half * (BN * 128) + e * 16) = make_uint4(0, 0, 0, 0);
+        from = row_at(u.len);
+        to = p.tile_keys;
+      }
+      if (p.tree) {
+        const int first = k0 + group * KC;
+        const uint32_t drafts = static_cast<uint32_t>(low_bits(min(u.len - first, KC)) & ~low_bits(u.len - u.live - first));
+        for (uint32_t left = drafts & ~__reduce_or_sync(0xffffffffu, static_cast<uint32_t>(see)); left; left &= left - 1) {
+          const int row = group * KC + __ffs(left) - 1;
+          if (row < p.tile_keys && lane < 8 * (D / 64))
+            *reinterpret_cast<uint4*>(tile + (lane >> 3) * (BN * 128) + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_proxy_async_smem();
+      return true;
     };
     do {
       const Unit& u = w.u;
@@ -876,6 +923,10 @@ __global__ void __launch_bounds__(THREADS, 1)
               see[ch] = visible(p, u, t, k0 + from + ch * 64) & low_bits(span - ch * 64);
           }
           if (!(ok = warp_wait(&ctl->s_full[buf], (NT == 2 ? g : g / NB) & 1, p.wait_limit, abort_flag))) break;
+          if constexpr (KS > 1) {
+            // Not before S is there: until then the barrier of V may be a lap behind.
+            if (masked && may_be_unseen(p, u, a) && !(ok = clear_unseen(u, a, g, see[0]))) break;
+          }
           tc_fence_after();
           uint32_t sv[KC];
           if constexpr (KC == 16) {
@@ -1371,7 +1422,7 @@ int make_plan(const char* what, const ntl_cache_t* c, const ntl_query_t* q, int6
 
 template <int D, int NT, int KS, bool BF16, bool SPLIT>
 int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                 const AttnBase& p, const Plan& n, cudaStream_t s) {
+                 const CUtensorMap& mv8, const CUtensorMap& mv1, const AttnBase& p, const Plan& n, cudaStream_t s) {
   static std::atomic<uint64_t> done_mask{0};
   auto kernel = cache_attn_kernel<D, NT, KS, BF16, SPLIT>;
   constexpr int smem = smem_bytes<D, NT>();
@@ -1389,7 +1440,7 @@ int launch_shape(const char* what, const CUtensorMap& mq, const CUtensorMap& mk,
                       fa.numRegs, REGS_LAUNCH);
     done_mask.fetch_or(bit, std::memory_order_release);
   }
-  cudaError_t e = ntl_launch_pdl(kernel, dim3(n.ctas), dim3(THREADS), smem, s, mq, mk, mv, AttnParams<SPLIT>{p});
+  cudaError_t e = ntl_launch_pdl(kernel, dim3(n.ctas), dim3(THREADS), smem, s, mq, mk, mv, mv8, mv1, AttnParams<SPLIT>{p});
   if (e != cudaSuccess) return ntl_fail(NTL_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   ntl_note_launch();
   if (int rc = ntl_check_launch(what)) return rc;
@@ -1412,7 +1463,7 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
               (unsigned long long)n.bytes);
   const int64_t group = q->heads / c->kv_heads, dim = c->head_dim;
   const bool bf16 = c->dtype == NTL_BF16;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mv8 = {}, mv1 = {};
   if (int rc = make_map(&mq, what, q->q, bf16, {dim, q->heads, q->tokens, q->seqs},
                         {q->head_stride, q->token_stride, q->seq_stride}, {64, group, n.tile_tokens, 1}))
     return rc;
@@ -1421,6 +1472,11 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   const int64_t box[4] = {64, 1, n.tile_keys / n.tile_pages, 1};
   if (int rc = make_map(&mk, what, c->k, bf16, dims, strides, box)) return rc;
   if (int rc = make_map(&mv, what, c->v, bf16, dims, strides, box)) return rc;
+  const bool key_groups = n.rows <= 16;
+  if (!key_groups) {
+    if (int rc = make_map(&mv8, what, c->v, bf16, dims, strides, {64, 1, 8, 1})) return rc;
+    if (int rc = make_map(&mv1, what, c->v, bf16, dims, strides, {64, 1, 1, 1})) return rc;
+  }
   AttnBase p = {};
   p.o = static_cast<uint16_t*>(q->o);
   p.table = q->table;
@@ -1462,17 +1518,17 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   // 197 us without (back to back, at the power cap).  Four groups of up to 32 rows need the 128-row MMA
   // and measured slower than none at head_dim 128 (32 x 8 drafts over 8192 tokens: 213 against 201 us).
 #define NTL_CACHE_ATTN(D, NT, KS)                                                                       \
-  return n.page_tiles ? bf16 ? launch_shape<D, NT, KS, true, true>(what, mq, mk, mv, p, n, s)           \
-                             : launch_shape<D, NT, KS, false, true>(what, mq, mk, mv, p, n, s)          \
-         : bf16       ? launch_shape<D, NT, KS, true, false>(what, mq, mk, mv, p, n, s)                 \
-                      : launch_shape<D, NT, KS, false, false>(what, mq, mk, mv, p, n, s)
+  return n.page_tiles ? bf16 ? launch_shape<D, NT, KS, true, true>(what, mq, mk, mv, mv8, mv1, p, n, s)           \
+                             : launch_shape<D, NT, KS, false, true>(what, mq, mk, mv, mv8, mv1, p, n, s)          \
+         : bf16       ? launch_shape<D, NT, KS, true, false>(what, mq, mk, mv, mv8, mv1, p, n, s)                 \
+                      : launch_shape<D, NT, KS, false, false>(what, mq, mk, mv, mv8, mv1, p, n, s)
   if (dim == 64) {
     if (n.row_tiles == 2) NTL_CACHE_ATTN(64, 2, 1);
-    if (n.rows <= 16) NTL_CACHE_ATTN(64, 1, 4);
+    if (key_groups) NTL_CACHE_ATTN(64, 1, 4);
     NTL_CACHE_ATTN(64, 1, 1);
   }
   if (n.row_tiles == 2) NTL_CACHE_ATTN(128, 2, 1);
-  if (n.rows <= 16) NTL_CACHE_ATTN(128, 1, 4);
+  if (key_groups) NTL_CACHE_ATTN(128, 1, 4);
   NTL_CACHE_ATTN(128, 1, 1);
 #undef NTL_CACHE_ATTN
 }

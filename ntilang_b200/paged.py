@@ -52,8 +52,9 @@ def tree_attention(q, k, v, table, lens, tree, *, q_lens=None, scale=None, out=N
     single-token decode.  Returns [seqs, tokens, heads, head_dim] in q's dtype (``out`` if given).
 
     Statistics and sums are fp32; the exponentials are rounded to the cache's type for the product
-    with V.  A NaN or infinity in a key row reaches the tokens that see it; in a value row that some token
-    of the call sees, it may reach tokens of the same sequence that do not."""
+    with V.  Key and value rows that no token of the call sees may hold anything.  A NaN or infinity in a key
+    row reaches the tokens that see it; in a value row that some token of the call sees, it may reach
+    tokens of the same sequence that do not."""
     if tree is None:
         raise TypeError("tree must be a CUDA tensor")
     return _paged.attend(q, k, v, table, lens, q_lens, tree, 0, 0, scale, out)

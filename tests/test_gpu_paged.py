@@ -349,6 +349,46 @@ def test_evicted_pages_are_not_read(torch_cuda, tokens):
         assert torch.equal(got, want), gone
 
 
+@pytest.mark.parametrize("dtype,dim,heads,kv_heads,page", SHAPES)
+@pytest.mark.parametrize("tokens", [1, 5, 40, 200])
+def test_keys_and_values_that_no_token_sees(torch_cuda, dtype, dim, heads, kv_heads, page, tokens):
+    """NaN and infinity in rows of the pages that a call reads: between the sinks and the window, and in drafts that
+    no token's mask names."""
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    lens = [2000 + tokens, 640 + tokens, 1111 + tokens, 100 + tokens]
+    q, k, v, table, n = make(torch, dtype=dtype, dim=dim, heads=heads, kv_heads=kv_heads, page=page, lens=lens,
+                             tokens=tokens, seed=page + tokens)
+
+    def spoil(b, at):
+        rows = torch.from_numpy(table[b].cpu().numpy()[at // page]).cuda().long(), torch.from_numpy(at % page).cuda()
+        k2[rows] = math.nan
+        v2[rows] = torch.tensor([math.nan, math.inf, -math.inf], device="cuda", dtype=v.dtype)[
+            torch.arange(len(at), device="cuda") % 3][:, None, None]
+
+    for window, sinks in ((50, 4), (129, 0), (300, 70), (1000, 1), (5, 1 << 30), (5, 1 << 40)):
+        want = paged.window_attention(q, k, v, table, n, window, sinks)
+        k2, v2 = k.clone(), v.clone()
+        for b, x in enumerate(lens):
+            spoil(b, np.arange(min(sinks, x), max(min(sinks, x), x - tokens - window + 1)))
+        out = paged.window_attention(q, k2, v2, table, n, window, sinks)
+        check(torch, out, q, k, v, table, n, [window_mask(x, tokens, window, sinks) for x in lens])
+        assert torch.equal(out, want), (window, sinks)
+    rng = np.random.default_rng(tokens)
+    bits = rng.random((len(lens), tokens, tokens)) < 0.5
+    bits[:, :, rng.random(tokens) < 0.4] = False
+    bits[0, :, -1] = bits[1, :, 0] = False
+    tree = pack(torch, bits)
+    want = paged.tree_attention(q, k, v, table, n, tree)
+    k2, v2 = k.clone(), v.clone()
+    for b, x in enumerate(lens):
+        spoil(b, x - tokens + np.nonzero(~bits[b].any(axis=0))[0])
+    out = paged.tree_attention(q, k2, v2, table, n, tree)
+    check(torch, out, q, k, v, table, n, [tree_mask_of(bits[b], x, tokens) for b, x in enumerate(lens)])
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("tokens", [1, 70])
 def test_strides_and_layouts(torch_cuda, tokens):
     """One layer of a cache, heads before rows, transposed queries, a table inside a wider one."""
