@@ -116,7 +116,8 @@ def free(table, lens, refs, seqs):
 
 def compact(k, v, table, refs, *, table_out=None, refs_out=None):
     """Move the live pages (refs > 0) to the lowest numbers: of n, the k-th at or past n goes into the k-th hole
-    before n.  ``table_out`` and ``refs_out`` (default: in place) follow.  Returns int32 [1]: n."""
+    before n.  ``table_out`` and ``refs_out`` (default: in place) follow; ``table`` has every sequence that holds
+    pages.  Returns int32 [1]: n."""
     return _paged.compact(k, v, table, refs, table if table_out is None else table_out,
                           refs if refs_out is None else refs_out)
 
@@ -132,12 +133,16 @@ class Cache:
         self.table = torch.full((seqs, max_pages), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(seqs, dtype=torch.int32, device=device)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
+        self.whole = None  # of a part: the cache with every sequence of the pool
 
     def part(self, seqs):
         """A cache over some of the sequences (a slice of the slots): the same pool and its rows of the table; its
-        lengths are its own from here on."""
+        lengths are its own from here on.  Before the whole is used for these sequences again, write them back:
+        ``cache.lens[seqs] = part.lens``."""
+        if not isinstance(seqs, slice):
+            raise TypeError(f"seqs must be a slice of the slots, got {type(seqs).__name__}")
         part = object.__new__(Cache)
-        part.k, part.v, part.refs = self.k, self.v, self.refs
+        part.k, part.v, part.refs, part.whole = self.k, self.v, self.refs, self.whole or self
         part.table, part.lens = self.table[seqs], self.lens[seqs].clone()
         return part
 
@@ -160,7 +165,8 @@ class Cache:
         copy_pages(self.k, self.v, src, dst)
 
     def compact(self):
-        return compact(self.k, self.v, self.table, self.refs)
+        """As the function, for every sequence of the pool, of a part too."""
+        return compact(self.k, self.v, (self.whole or self).table, self.refs)
 
     def tree_attention(self, layer, q, tree, **kwargs):
         return tree_attention(q, self.k[layer], self.v[layer], self.table, self.lens, tree, **kwargs)

@@ -778,6 +778,32 @@ def test_compact(torch_cuda, pages, share, in_place):
         assert np.array_equal(t.cpu().numpy(), table) and np.array_equal(r.cpu().numpy(), refs)
 
 
+def test_part_of_a_cache(torch_cuda):
+    """Closing up the pool through a part, or through the whole while a part is in use, moves every sequence's pages
+    with its table; a part is a slice of the slots."""
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    for whole in (False, True):
+        c = paged.Cache(layers=1, pages=24, page_size=8, kv_heads=1, head_dim=64, seqs=4, max_pages=5)
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        rnd = lambda *s: torch.randn(*s, device="cuda", generator=gen, dtype=torch.float16)  # noqa: E731
+        for b in (1, 3, 2, 0):  # sequence 0's pages are the ones that move
+            assert c.reserve(i32(torch, [b]), 30).tolist() == [1]
+        c.append(rnd(1, 4, 30, 1, 64), rnd(1, 4, 30, 1, 64), i32(torch, [30, 17, 25, 9]))
+        c.free(i32(torch, [1]))
+        part = c.part(slice(2, 4))
+        q = rnd(4, 1, 2, 64)
+        want = c.window_attention(0, q, 1 << 20)
+        live = int((c if whole else part).compact())
+        assert live == int((c.refs > 0).sum()) and int(c.table.max()) == live - 1
+        assert torch.equal(c.window_attention(0, q, 1 << 20), want)
+        assert torch.equal(part.window_attention(0, q[2:], 1 << 20), want[2:])
+        for seqs in ([2, 3], 2, i32(torch, [2, 3])):
+            with pytest.raises(TypeError, match="slice"):
+                c.part(seqs)
+
+
 def test_copy_pages(torch_cuda):
     from ntilang_b200 import paged
 
