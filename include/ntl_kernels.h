@@ -242,8 +242,9 @@ int ntl_cache_workspace_size(int64_t pages, int64_t n, uint64_t* bytes_out);
 
 /* Sequences dst[i] (holding nothing) become copies of src[i]: full pages are shared (refs + 1), the
  * part of a page at the end is copied into the lowest free page (refs <= 0), children served in
- * order.  granted[i] = 0, and dst[i] stays empty, where no page is left.  dst and src are disjoint
- * and dst has no repeats. */
+ * order.  granted[i] = 0, and dst[i] stays empty, where no page is left, where the parent has no page for
+ * the part at its end, and where a sequence is out of range or dst[i] is src[i]; such a pair takes no page.
+ * dst and src are disjoint and dst has no repeats. */
 int ntl_cache_fork(const ntl_cache_t* cache, int32_t* table, int64_t table_stride, int64_t seqs, int64_t max_pages,
                    int32_t* lens, int32_t* refs, const int32_t* src, const int32_t* dst, int64_t n, int32_t* granted,
                    void* workspace, uint64_t workspace_bytes, ntl_stream_t stream);

@@ -208,11 +208,10 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
   return before + s - x;
 }
 
-// Pages that a sequence lacks: of reserve, the unmapped entries from the page of its next token up to
-// its length + extra (entries before that may be pages a window left behind, and stay as they are); of
-// fork (extra < 0), one for the part of a page at its end.  -1 when the table is too narrow.
+// Pages that a sequence lacks in reserve: the unmapped entries from the page of its next token up to its
+// length + extra (entries before that may be pages a window left behind, and stay as they are).  -1 when the
+// table is too narrow.
 __device__ __forceinline__ int pages_needed(const int32_t* row, int len, int extra, int page_size, int max_pages) {
-  if (extra < 0) return len % page_size != 0;
   const int64_t want = (static_cast<int64_t>(len) + extra + page_size - 1) / page_size;
   if (want > max_pages) return -1;
   int n = 0;
@@ -220,14 +219,32 @@ __device__ __forceinline__ int pages_needed(const int32_t* row, int len, int ext
   return n;
 }
 
+// Whether a child can be forked: both sequences there, and not the same.
+__device__ __forceinline__ bool fork_pair(int from, int to, int seqs) {
+  return from >= 0 && from < seqs && to >= 0 && to < seqs && from != to;
+}
+
+// A parent's length as fork sees it, and the page that holds the part of a page at its end (-1: none there).
+struct ForkParent {
+  int len, full, part, last;
+  __device__ __forceinline__ ForkParent(const int32_t* row, int length, int max_pages, int pages, int page_size) {
+    len = static_cast<int>(min(static_cast<int64_t>(max(length, 0)), static_cast<int64_t>(max_pages) * page_size));
+    full = len / page_size;
+    part = len % page_size;
+    last = part ? row[full] : -1;
+    if (last >= pages) last = -1;
+  }
+};
+
 // One CTA.  Ranks the needs of n sequences in order (first[i] = pages needed before sequence i),
-// lists the lowest free pages in order, and for reserve (extra >= 0) hands them out.  A sequence
-// whose pages do not all exist gets none; those after it that need pages get none either.
+// lists the lowest free pages in order, and for reserve hands them out.  A sequence whose pages do not
+// all exist gets none; those after it that need pages get none either.  For fork (`child` is not null) seq[i]
+// is the parent and needs a page for the part at its end; pairs that are refused need none.
 // work: first[n + 1], list[pages].  fork reads first, list and found in the next kernel.
 __global__ void __launch_bounds__(kPlanThreads)
     plan_kernel(int32_t* table, int64_t table_stride, int max_pages, const int32_t* lens, int32_t* refs, int pages,
-                int page_size, const int32_t* seq, int n, int seqs, int extra, const int32_t* extra_of,
-                int32_t* granted, int32_t* found_out, int32_t* first, int32_t* list) {
+                int page_size, const int32_t* seq, const int32_t* child, int n, int seqs, int extra,
+                const int32_t* extra_of, int32_t* granted, int32_t* found_out, int32_t* first, int32_t* list) {
   __shared__ int warp_sums[32];
   pdl_wait();
   pdl_trigger();
@@ -237,8 +254,11 @@ __global__ void __launch_bounds__(kPlanThreads)
     int mine = 0;
     if (i < n) {
       const int b = seq[i];
-      if (b >= 0 && b < seqs) {
-        const int add = extra < 0 ? -1 : extra_of ? max(extra_of[i], 0) : extra;
+      if (child) {
+        if (fork_pair(b, child[i], seqs))
+          mine = ForkParent(table + b * table_stride, lens[b], max_pages, pages, page_size).last >= 0;
+      } else if (b >= 0 && b < seqs) {
+        const int add = extra_of ? max(extra_of[i], 0) : extra;
         mine = max(pages_needed(table + b * table_stride, max(lens[b], 0), add, page_size, max_pages), 0);
       }
     }
@@ -266,7 +286,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     found = min(need, found + total);
   }
   if (threadIdx.x == 0) *found_out = found;
-  if (extra < 0) return;
+  if (child) return;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int b = seq[i];
@@ -295,14 +315,14 @@ __global__ void __launch_bounds__(kRowWarps * 32)
   pdl_wait();
   const int i = blockIdx.y;
   const int from = src[i], to = dst[i];
-  if (from < 0 || from >= seqs || to < 0 || to >= seqs || from == to) {
+  if (!fork_pair(from, to, seqs)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) granted[i] = 0;
     return;
   }
   const int32_t* parent = table + from * table_stride;
-  const int len = min(static_cast<int64_t>(max(lens[from], 0)), static_cast<int64_t>(max_pages) * c.page_size);
-  const int full = len / c.page_size, part = len % c.page_size;
-  const bool ok = part == 0 || first[i] < *found;
+  const ForkParent end(parent, lens[from], max_pages, c.pages, c.page_size);
+  const int full = end.full, part = end.part;
+  const bool ok = part == 0 || (end.last >= 0 && first[i] < *found);
   const int fresh = part && ok ? list[first[i]] : -1;
   if (blockIdx.x == 0) {
     int32_t* row = table + to * table_stride;
@@ -314,15 +334,14 @@ __global__ void __launch_bounds__(kRowWarps * 32)
       row[j] = p;
     }
     if (threadIdx.x == 0) {
-      lens[to] = ok ? len : 0;
+      lens[to] = ok ? end.len : 0;
       granted[i] = ok;
       if (fresh >= 0) refs[fresh] = 1;
     }
     return;
   }
   if (fresh < 0) return;
-  const int old = parent[full];
-  if (old < 0 || old >= c.pages) return;
+  const int old = end.last;
   const int lane = threadIdx.x & 31;
   const int64_t rows = static_cast<int64_t>(c.layers) * part;
   for (int64_t r = (blockIdx.x - 1) * kRowWarps + (threadIdx.x >> 5); r < rows; r += (gridDim.x - 1) * kRowWarps) {
@@ -599,8 +618,8 @@ extern "C" int ntl_cache_fork(const ntl_cache_t* cache, int32_t* table, int64_t 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int rc = launched("cache fork",
                         ntl_launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, table, table_stride,
-                                       static_cast<int>(max_pages), lens, refs, c.pages, c.page_size, src,
-                                       static_cast<int>(n), static_cast<int>(seqs), -1, nullptr, granted, found, first,
+                                       static_cast<int>(max_pages), lens, refs, c.pages, c.page_size, src, dst,
+                                       static_cast<int>(n), static_cast<int>(seqs), 0, nullptr, granted, found, first,
                                        list)))
     return rc;
   const int64_t rows = static_cast<int64_t>(c.layers) * (c.page_size - 1);
@@ -635,7 +654,7 @@ extern "C" int ntl_cache_reserve(int64_t pages, int64_t page_size, int32_t* tabl
   return launched("cache reserve",
                   ntl_launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<cudaStream_t>(stream), table,
                                  table_stride, static_cast<int>(max_pages), lens, refs, static_cast<int>(pages),
-                                 static_cast<int>(page_size), seq, static_cast<int>(n), static_cast<int>(seqs),
+                                 static_cast<int>(page_size), seq, nullptr, static_cast<int>(n), static_cast<int>(seqs),
                                  static_cast<int>(extra), extra_of, granted, found, first, list));
 }
 

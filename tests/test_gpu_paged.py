@@ -717,6 +717,40 @@ def test_fork_and_free(torch_cuda, pages):
     assert not r.any() and not n.any() and (t == -1).all()
 
 
+def test_fork_of_pairs_that_cannot_be(torch_cuda):
+    """A pair that is refused takes no page from the others: sequences out of range, a child that is its parent, a parent
+    without a page for the tokens at its end."""
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    page, pages = 8, 12
+    k, v = pool(torch, pages=pages, page=page, kv_heads=1, dim=64)
+    table = np.full((12, 3), -1)
+    table[0, :2], table[1, :3], table[2, 0], table[3, :2] = [0, 1], [2, 3, 4], 5, [6, 7]
+    table[4, :2] = [6, 7]
+    table[5, :2] = [6, 900]  # no such page
+    lens = np.array([12, 21, 8, 20, 13, 11] + [0] * 6)  # 3: its last page is missing
+    refs = np.ones(pages, dtype=np.int64)
+    refs[[6, 7]] = [3, 2]
+    refs[[8, 10, 11]] = 0  # three free pages
+    src = [0, 0, -1, 3, 5, 1, 2, 0, 99, 1, 4]
+    dst = [99, 0, 6, 6, 7, 8, 9, 10, 11, -5, 11]
+    want_granted = [0, 0, 0, 0, 0, 1, 1, 1, 0, 0, 1]
+    before = [x.clone() for x in (k, v)]
+    t, n, r = (i32(torch, x) for x in (table, lens, refs))
+    got = paged.fork(k, v, t, n, r, i32(torch, src), i32(torch, dst))
+    ok = [i for i, x in enumerate(want_granted) if x]
+    granted, copies = plain_fork(table, lens, refs, [src[i] for i in ok], [dst[i] for i in ok], page)
+    assert all(granted) and [c[1] for c in copies] == [8, 10, 11]
+    assert got.tolist() == want_granted
+    for x, w in ((t, table), (n, lens), (r, refs)):
+        assert np.array_equal(x.cpu().numpy(), w)
+    for x, w in zip((k, v), before):
+        for old, new, part in copies:
+            w[:, new, :part] = w[:, old, :part]
+        assert torch.equal(x, w)
+
+
 def test_reserve(torch_cuda):
     from ntilang_b200 import paged
 
