@@ -290,13 +290,14 @@ __global__ void __launch_bounds__(kPlanThreads)
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int b = seq[i];
-    bool ok = b >= 0 && b < seqs && first[i + 1] <= found;
-    if (ok) {
+    bool ok = false;
+    if (b >= 0 && b < seqs) {
       int32_t* row = table + b * table_stride;
       const int len = max(lens[b], 0), add = extra_of ? max(extra_of[i], 0) : extra;
-      ok = pages_needed(row, len, add, page_size, max_pages) >= 0;
+      const int lacks = pages_needed(row, len, add, page_size, max_pages);
+      ok = lacks == 0 || (lacks > 0 && first[i + 1] <= found);
       int at = first[i];
-      for (int j = len / page_size; j < max_pages && at < first[i + 1]; ++j)
+      for (int j = len / page_size; ok && lacks > 0 && j < max_pages && at < first[i + 1]; ++j)
         if (row[j] < 0) {
           refs[list[at]] = 1;
           row[j] = list[at++];

@@ -778,6 +778,18 @@ def test_reserve(torch_cuda):
     assert got.tolist() == [1] and t[5, :12].tolist() == unused[48:].tolist()
 
 
+def test_reserve_of_nothing_behind_a_shortage(torch_cuda):
+    """A sequence that needs no page is served, whatever those before it lacked."""
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    table = [[0, -1, -1], [1, -1, -1], [-1, -1, -1], [-1, -1, -1], [3, -1, -1]]
+    t, n, r = i32(torch, table), i32(torch, [8, 3, 0, 0, 8]), i32(torch, [1, 1, 0, 1])
+    got = paged.reserve(t, n, r, i32(torch, [0, 1, 2, 3, 4]), i32(torch, [16, 5, 8, 0, 0]), 8)
+    assert got.tolist() == [0, 1, 0, 1, 1]
+    assert t.tolist() == table and r.tolist() == [1, 1, 0, 1]
+
+
 @pytest.mark.parametrize("pages,share", [(1, 1.0), (37, 0.5), (37, 0.0), (64, 1.0), (9001, 0.3)])
 @pytest.mark.parametrize("in_place", [True, False])
 def test_compact(torch_cuda, pages, share, in_place):
