@@ -10,6 +10,8 @@
 // access, K and V of a row in flight together.  Bound: HBM, each moved byte read and written once.
 // Page numbers, positions and sequence numbers come from device memory: each is checked against its
 // range before it is used, and what is out of range is skipped.
+#include <climits>
+
 #include "ntl_common.cuh"
 
 namespace {
@@ -182,28 +184,29 @@ __global__ void __launch_bounds__(kRowWarps * 32)
 // ------------------------------------------------------------------------------ allocation
 
 // Exclusive prefix sum of one value per thread over the block, and the block's total.
-__device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
+template <class T>
+__device__ __forceinline__ T block_scan(T x, T* warp_sums, T& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int s = x;
+  T s = x;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, s, d);
+    const T y = __shfl_up_sync(0xffffffffu, s, d);
     if (lane >= d) s += y;
   }
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
   if (warp == 0) {
-    int w = lane < warps ? warp_sums[lane] : 0;
+    T w = lane < warps ? warp_sums[lane] : 0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, d);
+      const T y = __shfl_up_sync(0xffffffffu, w, d);
       if (lane >= d) w += y;
     }
     if (lane < warps) warp_sums[lane] = w;
   }
   __syncthreads();
   total = warp_sums[warps - 1];
-  const int before = warp ? warp_sums[warp - 1] : 0;
+  const T before = warp ? warp_sums[warp - 1] : 0;
   __syncthreads();
   return before + s - x;
 }
@@ -239,19 +242,22 @@ struct ForkParent {
 // One CTA.  Ranks the needs of n sequences in order (first[i] = pages needed before sequence i),
 // lists the lowest free pages in order, and for reserve hands them out.  A sequence whose pages do not
 // all exist gets none; those after it that need pages get none either.  For fork (`child` is not null) seq[i]
-// is the parent and needs a page for the part at its end; pairs that are refused need none.
+// is the parent and needs a page for the part at its end; pairs that are refused need none.  Needs are summed in 64
+// bits (2^11 sequences with 2^20 unmapped entries each pass 2^31); first[] stops at pages + 1, which is not to be had.
 // work: first[n + 1], list[pages].  fork reads first, list and found in the next kernel.
 __global__ void __launch_bounds__(kPlanThreads)
     plan_kernel(int32_t* table, int64_t table_stride, int max_pages, const int32_t* lens, int32_t* refs, int pages,
                 int page_size, const int32_t* seq, const int32_t* child, int n, int seqs, int extra,
                 const int32_t* extra_of, int32_t* granted, int32_t* found_out, int32_t* first, int32_t* list) {
   __shared__ int warp_sums[32];
+  __shared__ int64_t need_sums[32];
+  const int64_t most = min(static_cast<int64_t>(pages) + 1, static_cast<int64_t>(INT_MAX));
   pdl_wait();
   pdl_trigger();
-  int need = 0;
+  int64_t need = 0;
   for (int i0 = 0; i0 < n; i0 += blockDim.x) {
     const int i = i0 + threadIdx.x;
-    int mine = 0;
+    int64_t mine = 0;
     if (i < n) {
       const int b = seq[i];
       if (child) {
@@ -262,12 +268,13 @@ __global__ void __launch_bounds__(kPlanThreads)
         mine = max(pages_needed(table + b * table_stride, max(lens[b], 0), add, page_size, max_pages), 0);
       }
     }
-    int total;
-    const int at = need + block_scan(mine, warp_sums, total);
-    if (i < n) first[i] = at;
+    int64_t total;
+    const int64_t at = need + block_scan(mine, need_sums, total);
+    if (i < n) first[i] = static_cast<int32_t>(min(at, most));
     need += total;
   }
-  if (threadIdx.x == 0) first[n] = need;
+  need = min(need, most);
+  if (threadIdx.x == 0) first[n] = static_cast<int32_t>(need);
   int found = 0;
   for (int p0 = 0; p0 < pages && found < need; p0 += blockDim.x * kPlanPages) {
     const int base = p0 + threadIdx.x * kPlanPages;
@@ -283,7 +290,7 @@ __global__ void __launch_bounds__(kPlanThreads)
         if (at < need) list[at] = base + u;
         ++at;
       }
-    found = min(need, found + total);
+    found = static_cast<int>(min(need, static_cast<int64_t>(found) + total));
   }
   if (threadIdx.x == 0) *found_out = found;
   if (child) return;
@@ -473,13 +480,16 @@ __global__ void tree_mask_kernel(const int32_t* parents, int64_t stride, int tok
 
 // ------------------------------------------------------------------------------ host side
 
+// The plans' passes over pages and sequences, kPlanThreads * kPlanPages at a time, count in 32 bits.
+constexpr int64_t kMostPages = (int64_t(1) << 31) - 2 * kPlanThreads * kPlanPages;
+
 int make_view(const char* what, const ntl_cache_t* c, View* view) {
   NTL_REQUIRE(c != nullptr, NTL_ERR_INVALID, "%s: NULL cache", what);
   NTL_REQUIRE(c->layers >= 0 && c->pages >= 0 && c->kv_heads >= 0, NTL_ERR_INVALID, "%s: negative cache size", what);
   NTL_REQUIRE(c->page_size >= 1 && c->head_dim >= 8 && c->head_dim % 8 == 0, NTL_ERR_UNSUPPORTED,
               "%s: page_size %lld must be positive and head_dim %lld a multiple of 8", what, (long long)c->page_size,
               (long long)c->head_dim);
-  NTL_REQUIRE(c->layers < (1 << 20) && c->pages < (int64_t(1) << 31) && c->page_size <= (1 << 20) &&
+  NTL_REQUIRE(c->layers < (1 << 20) && c->pages <= kMostPages && c->page_size <= (1 << 20) &&
                   c->kv_heads * c->head_dim < (int64_t(1) << 24),
               NTL_ERR_UNSUPPORTED, "%s: cache too large", what);
   NTL_REQUIRE(c->layer_stride % 8 == 0 && c->page_stride % 8 == 0 && c->row_stride % 8 == 0 && c->head_stride % 8 == 0,
@@ -638,9 +648,9 @@ extern "C" int ntl_cache_reserve(int64_t pages, int64_t page_size, int32_t* tabl
                                  int64_t extra, const int32_t* extra_of, int32_t* granted, void* workspace,
                                  uint64_t workspace_bytes, ntl_stream_t stream) {
   if (int rc = check_table("cache reserve", table, table_stride, seqs, max_pages)) return rc;
-  NTL_REQUIRE(pages >= 0 && pages < (int64_t(1) << 31) && page_size >= 1 && page_size <= (1 << 20), NTL_ERR_INVALID,
+  NTL_REQUIRE(pages >= 0 && pages <= kMostPages && page_size >= 1 && page_size <= (1 << 20), NTL_ERR_INVALID,
               "cache reserve: bad pool size");
-  NTL_REQUIRE(n >= 0 && n < (int64_t(1) << 31) && extra >= 0 && extra < (int64_t(1) << 31), NTL_ERR_INVALID,
+  NTL_REQUIRE(n >= 0 && n <= kMostPages && extra >= 0 && extra < (int64_t(1) << 31), NTL_ERR_INVALID,
               "cache reserve: bad count");
   if (n == 0) return NTL_OK;
   NTL_REQUIRE(lens && refs && seq && granted, NTL_ERR_INVALID, "cache reserve: NULL pointer");

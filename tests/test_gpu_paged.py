@@ -790,6 +790,29 @@ def test_reserve_of_nothing_behind_a_shortage(torch_cuda):
     assert t.tolist() == table and r.tolist() == [1, 1, 0, 1]
 
 
+def test_reserve_of_more_than_31_bits(torch_cuda):
+    """Needs whose sum passes 2^31 and 2^32 are a shortage like any other: those before it are served, the others not."""
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    seqs, width, page = 2200, 1 << 20, 16
+    t = torch.full((seqs, width), -1, dtype=torch.int32, device="cuda")
+    n, r = torch.zeros(seqs, dtype=torch.int32, device="cuda"), torch.zeros(40, dtype=torch.int32, device="cuda")
+    r[7] = 1
+    extra = torch.full((seqs,), width * page, dtype=torch.int32, device="cuda")
+    extra[:2], extra[2100] = i32(torch, [30, 5]), 0
+    for order in (torch.arange(seqs), torch.cat([torch.arange(2, seqs), torch.arange(2)])):
+        got = paged.reserve(t, n, r, order.int().cuda(), extra[order.cuda()], page).cpu()
+        want = torch.zeros(seqs, dtype=torch.int32)
+        want[order == 2100] = 1
+        if order[0] == 0:
+            want[:2] = 1
+            assert t[:2, :3].tolist() == [[0, 1, -1], [2, -1, -1]] and int(r.sum()) == 4
+            paged.free(t, n, r, i32(torch, [0, 1]))
+        assert torch.equal(got, want)
+        assert int(r.sum()) == 1 and int(t.max()) == -1
+
+
 @pytest.mark.parametrize("pages,share", [(1, 1.0), (37, 0.5), (37, 0.0), (64, 1.0), (9001, 0.3)])
 @pytest.mark.parametrize("in_place", [True, False])
 def test_compact(torch_cuda, pages, share, in_place):
