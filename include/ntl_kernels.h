@@ -167,7 +167,8 @@ int ntl_fa2_set_causal_grid(int mode);
  * (int32 page numbers, -1 = no page) and a length in tokens (int32, device memory).  Page numbers
  * and lengths are read on the device: what is out of range is skipped, and a length is cut to
  * max_pages * page_size.  Attention reads a position without a page as a key and value of zeros; a row
- * written there is dropped.  All entry points work in stream order; those with a workspace take one of the size that the matching
+ * written there is dropped.  Rows of a table that a call writes must not overlap (table_stride >= max_pages).
+ * All entry points work in stream order; those with a workspace take one of the size that the matching
  * size function gives, which calls on different streams must not share. */
 enum { NTL_F16 = 0, NTL_BF16 = 1 };
 

@@ -513,11 +513,13 @@ int make_view(const char* what, const ntl_cache_t* c, View* view) {
   return NTL_OK;
 }
 
-int check_table(const char* what, const int32_t* table, int64_t stride, int64_t seqs, int64_t max_pages) {
+int check_table(const char* what, const int32_t* table, int64_t stride, int64_t seqs, int64_t max_pages, bool written) {
   NTL_REQUIRE(seqs >= 0 && max_pages >= 0 && stride >= 0, NTL_ERR_INVALID, "%s: negative table size", what);
   NTL_REQUIRE(seqs < (int64_t(1) << 31) && max_pages < (int64_t(1) << 31), NTL_ERR_UNSUPPORTED,
               "%s: table too large", what);
   NTL_REQUIRE(seqs == 0 || max_pages == 0 || table, NTL_ERR_INVALID, "%s: NULL table", what);
+  NTL_REQUIRE(!written || seqs <= 1 || stride >= max_pages, NTL_ERR_INVALID,
+              "%s: rows of a table that is written must not overlap", what);
   return NTL_OK;
 }
 
@@ -544,7 +546,7 @@ extern "C" int ntl_cache_append(const ntl_cache_t* cache, const void* k_new, con
                                 const int32_t* counts, int64_t tokens, int32_t* lens_out, ntl_stream_t stream) {
   View c = {};
   if (int rc = make_view("cache append", cache, &c)) return rc;
-  if (int rc = check_table("cache append", table, table_stride, seqs, max_pages)) return rc;
+  if (int rc = check_table("cache append", table, table_stride, seqs, max_pages, false)) return rc;
   NTL_REQUIRE(tokens >= 0 && tokens < (int64_t(1) << 31), NTL_ERR_INVALID, "cache append: bad token count %lld",
               (long long)tokens);
   if (seqs == 0) return NTL_OK;
@@ -570,7 +572,7 @@ extern "C" int ntl_cache_accept(const ntl_cache_t* cache, const int32_t* table, 
                                 int32_t* lens_out, ntl_stream_t stream) {
   View c = {};
   if (int rc = make_view("cache accept", cache, &c)) return rc;
-  if (int rc = check_table("cache accept", table, table_stride, seqs, max_pages)) return rc;
+  if (int rc = check_table("cache accept", table, table_stride, seqs, max_pages, false)) return rc;
   NTL_REQUIRE(drafts >= 0 && drafts < (int64_t(1) << 31) && path_len >= 0 && path_len < (int64_t(1) << 31),
               NTL_ERR_INVALID, "cache accept: bad draft count or path length");
   if (seqs == 0) return NTL_OK;
@@ -613,7 +615,7 @@ extern "C" int ntl_cache_fork(const ntl_cache_t* cache, int32_t* table, int64_t 
                               ntl_stream_t stream) {
   View c = {};
   if (int rc = make_view("cache fork", cache, &c)) return rc;
-  if (int rc = check_table("cache fork", table, table_stride, seqs, max_pages)) return rc;
+  if (int rc = check_table("cache fork", table, table_stride, seqs, max_pages, true)) return rc;
   NTL_REQUIRE(n >= 0 && n <= 65535, NTL_ERR_UNSUPPORTED, "cache fork: %lld children (at most 65535 per call)",
               (long long)n);
   if (n == 0) return NTL_OK;
@@ -647,7 +649,7 @@ extern "C" int ntl_cache_reserve(int64_t pages, int64_t page_size, int32_t* tabl
                                  int64_t max_pages, const int32_t* lens, int32_t* refs, const int32_t* seq, int64_t n,
                                  int64_t extra, const int32_t* extra_of, int32_t* granted, void* workspace,
                                  uint64_t workspace_bytes, ntl_stream_t stream) {
-  if (int rc = check_table("cache reserve", table, table_stride, seqs, max_pages)) return rc;
+  if (int rc = check_table("cache reserve", table, table_stride, seqs, max_pages, true)) return rc;
   NTL_REQUIRE(pages >= 0 && pages <= kMostPages && page_size >= 1 && page_size <= (1 << 20), NTL_ERR_INVALID,
               "cache reserve: bad pool size");
   NTL_REQUIRE(n >= 0 && n <= kMostPages && extra >= 0 && extra < (int64_t(1) << 31), NTL_ERR_INVALID,
@@ -671,7 +673,7 @@ extern "C" int ntl_cache_reserve(int64_t pages, int64_t page_size, int32_t* tabl
 
 extern "C" int ntl_cache_free(int64_t pages, int32_t* table, int64_t table_stride, int64_t seqs, int64_t max_pages,
                               int32_t* lens, int32_t* refs, const int32_t* seq, int64_t n, ntl_stream_t stream) {
-  if (int rc = check_table("cache free", table, table_stride, seqs, max_pages)) return rc;
+  if (int rc = check_table("cache free", table, table_stride, seqs, max_pages, true)) return rc;
   NTL_REQUIRE(pages >= 0 && pages < (int64_t(1) << 31) && n >= 0 && n < (int64_t(1) << 31), NTL_ERR_INVALID,
               "cache free: bad size");
   if (n == 0) return NTL_OK;
@@ -688,8 +690,8 @@ extern "C" int ntl_cache_compact(const ntl_cache_t* cache, const int32_t* table,
                                  uint64_t workspace_bytes, ntl_stream_t stream) {
   View c = {};
   if (int rc = make_view("cache compact", cache, &c)) return rc;
-  if (int rc = check_table("cache compact", table, table_stride, seqs, max_pages)) return rc;
-  if (int rc = check_table("cache compact", table_out, out_stride, seqs, max_pages)) return rc;
+  if (int rc = check_table("cache compact", table, table_stride, seqs, max_pages, false)) return rc;
+  if (int rc = check_table("cache compact", table_out, out_stride, seqs, max_pages, true)) return rc;
   NTL_REQUIRE(live, NTL_ERR_INVALID, "cache compact: NULL live count");
   NTL_REQUIRE(c.pages == 0 || (refs && refs_out), NTL_ERR_INVALID, "cache compact: NULL counts");
   uint64_t need = 0;

@@ -83,6 +83,12 @@ const Tensor& ints(const char* name, PyObject* o, int index, std::initializer_li
   same_device(x, index);
   return x;
 }
+// A table whose rows are written.
+const Tensor& written_table(const char* name, const Tensor& x) {
+  if (x.size(0) > 1 && x.stride(0) < x.size(1))
+    raise(PyExc_ValueError, "%s must not be broadcast: its rows are written", name);
+  return x;
+}
 int32_t* int_ptr(const Tensor& x) { return x.data_ptr<int32_t>(); }
 
 // A 16-bit CUDA tensor that the kernels can read 16 bytes at a time along its last dimension.
@@ -349,7 +355,7 @@ struct Sequences {
 };
 
 Sequences sequences_of(PyObject* table, PyObject* lens, PyObject* refs, int64_t pages, int index) {
-  const Tensor& t = ints("table", table, index, {-1, -1});
+  const Tensor& t = written_table("table", ints("table", table, index, {-1, -1}));
   return {t, ints("lens", lens, index, {t.size(0)}), ints("refs", refs, index, {pages})};
 }
 
@@ -415,7 +421,7 @@ PyObject* compact(PyObject* const* a) {
   const int index = cache.index;
   const Tensor& table = ints("table", a[2], index, {-1, -1});
   const Tensor& refs = ints("refs", a[3], index, {cache.c.pages});
-  const Tensor& table_out = ints("table_out", a[4], index, {table.size(0), table.size(1)});
+  const Tensor& table_out = written_table("table_out", ints("table_out", a[4], index, {table.size(0), table.size(1)}));
   const Tensor& refs_out = ints("refs_out", a[5], index, {cache.c.pages});
   Device device(index);
   Tensor live = new_ints({1}, index);

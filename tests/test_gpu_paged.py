@@ -914,6 +914,48 @@ def test_cache_refusals(torch_cuda):
             call()
 
 
+def test_tables_that_are_written_are_not_broadcast(torch_cuda):
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    k, v = pool(torch, pages=8, page=8, kv_heads=1, dim=64)
+    one = torch.full((1, 4), -1, dtype=torch.int32, device="cuda")
+    n, r, seqs = i32(torch, [0, 0, 0]), i32(torch, [0] * 8), i32(torch, [0, 1])
+    lapping = torch.full((12,), -1, dtype=torch.int32, device="cuda").as_strided((3, 4), (2, 1))
+    for table in (one.expand(3, 4), lapping):
+        for call in (lambda: paged.reserve(table, n, r, seqs, 3, 8), lambda: paged.free(table, n, r, seqs),
+                     lambda: paged.fork(k, v, table, n, r, seqs[:1], seqs[1:]), lambda: paged.compact(k, v, table, r),
+                     lambda: paged.compact(k, v, one.repeat(3, 1), r, table_out=table)):
+            with pytest.raises(ValueError, match="broadcast"):
+                call()
+    # Reading is another matter: three sequences over the same pages.
+    one[0, :2] = i32(torch, [5, 2])
+    q = torch.randn(3, 2, 2, 64, device="cuda", dtype=torch.float16)
+    lens = i32(torch, [16, 9, 3])
+    want = paged.window_attention(q, k[0], v[0], one.repeat(3, 1), lens, 5, 1)
+    assert torch.equal(paged.window_attention(q, k[0], v[0], one.expand(3, 4), lens, 5, 1), want)
+    out = torch.empty(3, 4, dtype=torch.int32, device="cuda")
+    paged.compact(k, v, one.expand(3, 4), i32(torch, [0, 0, 1, 0, 0, 1, 0, 0]), table_out=out,
+                  refs_out=torch.empty_like(r))
+    assert out.tolist() == [[1, 0, -1, -1]] * 3
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_broadcast_queries_and_heads(torch_cuda, dtype):
+    """Expanded tensors (stride 0): one sequence's queries for all, one key head's rows for several."""
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    for tokens in (1, 5, 70):
+        q, k, v, table, n = make(torch, dtype=dtype, lens=[300 + tokens, 77 + tokens], tokens=tokens, heads=4, kv_heads=1)
+        for x in (q[:1].expand(2, -1, -1, -1), q[:, :, :1].expand(-1, -1, 4, -1), q[:, :1].expand(-1, tokens, -1, -1)):
+            assert torch.equal(paged.window_attention(x, k, v, table, n, 100, 2),
+                               paged.window_attention(x.contiguous(), k, v, table, n, 100, 2))
+        wide = [x.expand(-1, -1, 2, -1) for x in (k, v)]
+        assert torch.equal(paged.window_attention(q, *wide, table, n, 100, 2),
+                           paged.window_attention(q, *(x.contiguous() for x in wide), table, n, 100, 2))
+
+
 def test_a_serving_round(torch_cuda):
     """Prompt, fork, drafts, verification and windowed decode, against dense tensors kept beside."""
     from ntilang_b200 import paged

@@ -111,6 +111,17 @@ def test_cache_refusals(call):
     assert call("ntl_tree_mask", None, 4, 0, 4, None, None) == (0, "")
 
 
+@pytest.mark.parametrize("stride", [0, 7])
+def test_written_tables_do_not_overlap(call, stride):
+    """Rows closer than max_pages (8): refused where they are written."""
+    big = 1 << 30
+    for got in (call("ntl_cache_fork", cache(), PTR, stride, 2, 8, PTR, PTR, PTR, PTR, 2, PTR, PTR, big, None),
+                call("ntl_cache_reserve", 10, 16, PTR, stride, 2, 8, PTR, PTR, PTR, 2, 3, None, PTR, PTR, big, None),
+                call("ntl_cache_free", 10, PTR, stride, 2, 8, PTR, PTR, PTR, 2, None),
+                call("ntl_cache_compact", cache(), PTR, 8, PTR, stride, 2, 8, PTR, PTR, PTR, PTR, big, None)):
+        assert got[0] == INVALID and "overlap" in got[1], got
+
+
 def test_refusals_before_any_gpu(built_library):
     """CPU tensors and wrong sizes are Python errors, on a machine without a GPU too."""
     torch = pytest.importorskip("torch")
