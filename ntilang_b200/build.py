@@ -3,7 +3,7 @@
 ``python -m ntilang_b200.build`` (or ``__graft_entry__.build()``) compiles every
 ``csrc/*.cu`` to an object under ``ntilang_b200/_build/`` and links
 ``ntilang_b200/libntl_kernels.so``.  The library is plain C ABI (``include/ntl_kernels.h``);
-Python reaches it through ctypes (``ntilang_b200._lib``).  Where torch is installed it also builds
+Python reaches it through ctypes (``ntilang_b200._lib``).  Where a torch built for CUDA is installed it also builds
 ``csrc/paged_binding.cpp`` into ``ntilang_b200/_paged.so``, the module behind ``ntilang_b200.paged``.
 """
 
@@ -44,12 +44,25 @@ def _stale(target: Path, deps) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
-def build_binding(force: bool = False, verbose: bool = False) -> Path | None:
-    """``_paged.so``, linked to the library and to torch's; None where torch is not installed."""
+def _torch_build() -> tuple[str, str | None] | None:
+    """Version of the torch that would be imported, and of its CUDA (None: built without); None where there is no
+    torch.  Read from ``torch/version.py``: importing torch takes seconds."""
     import importlib.util
+    import runpy
+
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        return None
+    version = runpy.run_path(str(Path(spec.origin).parent / "version.py"))
+    return version["__version__"], version.get("cuda")
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path | None:
+    """``_paged.so``, linked to the library and to torch's; None where there is no torch built for CUDA."""
     import sysconfig
 
-    if importlib.util.find_spec("torch") is None:
+    torch_build = _torch_build()
+    if torch_build is None or torch_build[1] is None:
         return None
     src = CSRC / "paged_binding.cpp"
     if not force and not _stale(BINDING, [src, ROOT / "include" / "ntl_kernels.h", Path(__file__)]):

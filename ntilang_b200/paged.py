@@ -27,7 +27,7 @@ import torch
 try:
     from . import _paged
 except ImportError as error:
-    raise ImportError("ntilang_b200/_paged.so is missing or does not load; build it with: "
+    raise ImportError("ntilang_b200/_paged.so is missing or does not load; build it, with a torch that has CUDA, by: "
                       f"python -m ntilang_b200.build ({error})") from error
 
 
