@@ -65,7 +65,10 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path | None:
     if torch_build is None or torch_build[1] is None:
         return None
     src = CSRC / "paged_binding.cpp"
-    if not force and not _stale(BINDING, [src, ROOT / "include" / "ntl_kernels.h", Path(__file__)]):
+    # What it was built for; another torch or interpreter needs its own.
+    note, built_for = BUILD / "_paged.torch", f"{torch_build[0]} {sysconfig.get_config_var('SOABI')}"
+    if (not force and not _stale(BINDING, [src, ROOT / "include" / "ntl_kernels.h", Path(__file__)])
+            and note.exists() and note.read_text() == built_for):
         return BINDING
     import torch
     from torch.utils.cpp_extension import include_paths
@@ -84,6 +87,8 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path | None:
     if res.returncode != 0:
         raise RuntimeError("building _paged.so failed:\n" + res.stdout + res.stderr)
     os.replace(tmp, BINDING)
+    BUILD.mkdir(exist_ok=True)
+    note.write_text(built_for)
     return BINDING
 
 

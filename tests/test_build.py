@@ -48,3 +48,14 @@ def test_no_binding_for_a_torch_without_cuda(tmp_path):
     """There is no libc10_cuda to link: the library builds alone, as where torch is not installed."""
     assert build(tmp_path, "2.9.0+cpu", None) == (0, "None")
     assert build(tmp_path, "2.9.0+cu128", "12.8") == (1, str(tmp_path / "_paged.so"))
+
+
+def test_the_binding_follows_torch(tmp_path):
+    """Built for one torch and interpreter, it is built again for another, without --force."""
+    built = str(tmp_path / "_paged.so")
+    assert build(tmp_path, "2.9.0+cu128", "12.8") == (1, built)
+    assert build(tmp_path, "2.9.0+cu128", "12.8") == (0, built)
+    assert build(tmp_path, "2.10.0+cu128", "12.8") == (1, built)
+    assert build(tmp_path, "2.10.0+cu128", "12.8") == (0, built)
+    (tmp_path / "_build" / "_paged.torch").write_text("of another interpreter")
+    assert build(tmp_path, "2.10.0+cu128", "12.8") == (1, built)
