@@ -72,7 +72,7 @@ struct AttnBase {
   float2* part_ml;
   int4* head;             // [ctas] the unit a CTA begins and does not end: {item, key head, last CTA, new tokens}
   int64_t table_stride, tree_stride;
-  int seqs, tokens, heads, kv_heads, group, pages, page_size, max_pages, words, window, sinks;
+  int seqs, tokens, heads, kv_heads, group, page_size, max_pages, words, window, sinks;
   int tile_tokens;   // tokens per 128-row tile
   int blocks;        // token blocks per sequence (units of NT tiles)
   int tile_keys;     // keys per tile: whole pages, or a part of a page
@@ -1494,7 +1494,6 @@ int launch(const char* what, const ntl_cache_t* c, const ntl_query_t* q, const u
   p.heads = static_cast<int>(q->heads);
   p.kv_heads = static_cast<int>(c->kv_heads);
   p.group = static_cast<int>(group);
-  p.pages = static_cast<int>(c->pages);
   p.page_size = static_cast<int>(c->page_size);
   p.max_pages = static_cast<int>(q->max_pages);
   p.words = static_cast<int>((q->tokens + 31) / 32);
