@@ -296,6 +296,23 @@ def test_tree_of_parents(torch_cuda, tokens):
     check(torch, a, q, k, v, table, n, [window_mask(x, tokens, 1 << 20, 0) for x in lens])
 
 
+@pytest.mark.parametrize("tokens", [257, 1030])
+def test_tree_mask_of_large_trees(torch_cuda, tokens):
+    """Chains and random trees of many words, against parents' rows: a draft sees what its parent sees, and itself."""
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    parents = np.stack([np.arange(tokens) - 1, np.random.default_rng(tokens).integers(-1, np.arange(tokens))])
+    bits = np.zeros((2, tokens, tokens), dtype=bool)
+    for b in range(2):
+        for t in range(tokens):
+            if parents[b, t] >= 0:
+                bits[b, t] = bits[b, parents[b, t]]
+            bits[b, t, t] = True
+    tree = paged.tree_mask(torch.tensor(parents, dtype=torch.int32, device="cuda"))
+    assert torch.equal(tree, pack(torch, bits))
+
+
 def test_tree_mask_odd_parents(torch_cuda):
     """A parent that is not an earlier draft makes a root: no walk is endless."""
     from ntilang_b200 import paged
@@ -788,6 +805,23 @@ def test_reserve_of_nothing_behind_a_shortage(torch_cuda):
     got = paged.reserve(t, n, r, i32(torch, [0, 1, 2, 3, 4]), i32(torch, [16, 5, 8, 0, 0]), 8)
     assert got.tolist() == [0, 1, 0, 1, 1]
     assert t.tolist() == table and r.tolist() == [1, 1, 0, 1]
+
+
+def test_reserve_for_a_long_prompt(torch_cuda):
+    """Thousands of pages for one sequence, from a pool with holes, beside a few for others."""
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    pages, page, width = 20000, 16, 9000
+    refs = (np.random.default_rng(1).random(pages) < 0.4).astype(np.int64)
+    free = np.nonzero(refs == 0)[0]
+    table = np.full((3, width), -1)
+    t, r = i32(torch, table), i32(torch, refs)
+    got = paged.reserve(t, i32(torch, [0, 0, 0]), r, i32(torch, [2, 0, 1]), i32(torch, [40, 131072, 1]), page)
+    assert got.tolist() == [1, 1, 1]
+    table[2, :3], table[0, :8192], table[1, 0] = free[:3], free[3:8195], free[8195]
+    refs[free[:8196]] = 1
+    assert np.array_equal(t.cpu().numpy(), table) and np.array_equal(r.cpu().numpy(), refs)
 
 
 def test_reserve_of_more_than_31_bits(torch_cuda):
