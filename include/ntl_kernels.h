@@ -214,7 +214,8 @@ int ntl_window_attention(const ntl_cache_t* cache, const ntl_query_t* query, int
 int ntl_cache_attention_workspace(const ntl_cache_t* cache, const ntl_query_t* query, uint64_t* bytes_out);
 
 /* words[b, t] (ceil(tokens / 32) words): bit s set where s is t or an ancestor of t, from
- * parents [seqs, tokens] (stride in entries); a parent that is not an earlier token ends the walk. */
+ * parents [seqs, tokens] (stride in entries); a parent that is not an earlier token ends the walk.
+ * Up to 8192 tokens. */
 int ntl_tree_mask(const int32_t* parents, int64_t stride, int64_t seqs, int64_t tokens, uint32_t* words,
                   ntl_stream_t stream);
 
@@ -245,7 +246,7 @@ int ntl_cache_workspace_size(int64_t pages, int64_t n, uint64_t* bytes_out);
  * part of a page at the end is copied into the lowest free page (refs <= 0), children served in
  * order.  granted[i] = 0, and dst[i] stays empty, where no page is left, where the parent has no page for
  * the part at its end, and where a sequence is out of range or dst[i] is src[i]; such a pair takes no page.
- * dst and src are disjoint and dst has no repeats. */
+ * dst and src are disjoint and dst has no repeats; n is at most 65535. */
 int ntl_cache_fork(const ntl_cache_t* cache, int32_t* table, int64_t table_stride, int64_t seqs, int64_t max_pages,
                    int32_t* lens, int32_t* refs, const int32_t* src, const int32_t* dst, int64_t n, int32_t* granted,
                    void* workspace, uint64_t workspace_bytes, ntl_stream_t stream);

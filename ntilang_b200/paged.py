@@ -9,6 +9,7 @@ each page.  ``Cache`` keeps the five together.
 Tables, lengths and counts stay on the GPU: no call here waits for the device, every call is
 launched on ``torch.cuda.current_stream()`` and may be captured in a CUDA graph.  What a table or
 list says is checked where it is read: a page, position or sequence out of range is skipped.
+No call takes part in autograd: outputs carry no gradient, whatever the inputs require.
 
     cache = Cache(layers=2, pages=256, page_size=16, kv_heads=8, head_dim=128, seqs=4, max_pages=64)
     cache.reserve(seqs, 100)
@@ -37,7 +38,7 @@ except ImportError as error:
 def tree_mask(parents):
     """Visibility words of draft trees: int32 [seqs, tokens, ceil(tokens / 32)], bit s % 32 of word
     s // 32 set where draft s is draft t itself or an ancestor.  ``parents`` int32 [seqs, tokens] holds
-    each draft's parent; what is not an earlier draft (-1) is a root."""
+    each draft's parent; what is not an earlier draft (-1) is a root.  Up to 8192 tokens."""
     return _paged.tree_mask(parents)
 
 
@@ -78,7 +79,8 @@ def window_attention(q, k, v, table, lens, window, sinks=0, *, q_lens=None, scal
 def append_tokens(k, v, k_new, v_new, table, lens, counts=None):
     """Write new tokens' rows, ``k_new`` / ``v_new`` [layers, seqs, tokens, kv_heads, head_dim] (4-D without
     layers for a 4-D cache), at positions lens[b] + t, t < counts[b] (default: all); returns the new
-    lengths.  A row whose position has no page is dropped: ``reserve`` first."""
+    lengths.  A row whose position has no page is dropped, and the length grows all the same (attention reads
+    such a position as zeros): ``reserve`` first, and look at what it granted."""
     return _paged.append_tokens(k, v, k_new, v_new, table, lens, counts)
 
 
@@ -95,7 +97,7 @@ def copy_pages(k, v, src, dst):
 
 
 def fork(k, v, table, lens, refs, src, dst):
-    """Make sequences ``dst[i]`` (int32, holding nothing, no repeats) copies of ``src[i]``: full pages are shared,
+    """Make sequences ``dst[i]`` (int32, holding nothing, no repeats, up to 65535) copies of ``src[i]``: full pages are shared,
     the part of a page at the end is copied into the lowest free page, in order.  ``dst`` and ``src`` have no
     sequence in common.  Updates table, lens and refs in place; returns int32 [n]: 1, or 0 where no page was
     left, the parent has no page for the tokens at its end, or a number is no sequence: the child holds nothing.
