@@ -97,9 +97,9 @@ def copy_pages(k, v, src, dst):
 
 
 def fork(k, v, table, lens, refs, src, dst):
-    """Make sequences ``dst[i]`` (int32, holding nothing, no repeats, up to 65535) copies of ``src[i]``: full pages are shared,
-    the part of a page at the end is copied into the lowest free page, in order.  ``dst`` and ``src`` have no
-    sequence in common.  Updates table, lens and refs in place; returns int32 [n]: 1, or 0 where no page was
+    """Make sequences ``dst[i]`` (int32, holding nothing, no repeats, up to 65535) copies of ``src[i]``: full pages
+    are shared, the part of a page at the end is copied into the lowest free page, in order.  ``dst`` and ``src``
+    have no sequence in common.  Updates table, lens and refs in place; returns int32 [n]: 1, or 0 where no page was
     left, the parent has no page for the tokens at its end, or a number is no sequence: the child holds nothing.
     Pages are not copied when they are written: a sequence that shares pages may append, but not ``accept``
     into a page that was full when it was shared."""

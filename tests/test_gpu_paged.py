@@ -530,6 +530,35 @@ def test_streams_graphs_and_repeats(torch_cuda):
     assert torch.equal(a, want) and torch.equal(b, tree)
 
 
+def test_threads(torch_cuda):
+    """Threads with a stream each, whose calls need workspaces of different sizes: every call's own result."""
+    import threading
+
+    from ntilang_b200 import paged
+
+    torch = torch_cuda
+    work = [make(torch, lens=[4000 // tokens, 3000], tokens=tokens, heads=8, seed=tokens) for tokens in (1, 9, 40, 2)]
+    want = [paged.window_attention(*w, 1000, 4) for w in work]
+    torch.cuda.synchronize()
+    got = [[] for _ in work]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for n in range(40):
+                j = (i + n) % len(work)
+                got[i].append((j, paged.window_attention(*work[j], 1000, 4)))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(work))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(len(x) == 40 for x in got)
+    for j, out in sum(got, []):
+        assert torch.equal(out, want[j])
+
+
 def test_no_rows(torch_cuda):
     from ntilang_b200 import paged
 
